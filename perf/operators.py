@@ -376,7 +376,7 @@ def run(s):
         return {"append": _plain_append, "attend": _plain_attend, "norm": _plain_norm, "matmul": _plain_matmul}[op](s)
     if op == "append":
         q = s["cache"].append(s["k"], s["v"], s["batch"], q=s["q"], rope=s.get("rope"))
-        k, v = s["cache"].read(s["batch"])
+        k, v = s["cache"].read(s["batch"], len(s["k"]))
         return {"q": q, "k": k, "v": v}
     if op == "attend":
         return s["cache"].attend(s["q"], s["batch"], window=s["case"]["window"])
