@@ -680,6 +680,117 @@ KL_API kl_status kl_ffn_stack_destroy(kl_ffn_stack_t s);
 KL_API kl_status kl_ffn_stack_decode(kl_ffn_stack_t s, float* hidden, int n_tokens, float neuron_sparsity);
 
 /* ------------------------------------------------------------------------ */
+/* The attention half of a decode step: rotary positions, a paged cache of   */
+/* 4-bit keys and values, attention over it, and 8-bit projections.  It      */
+/* writes the residual stream that kl_ffn_stack_decode goes on from          */
+/* (klearu-llm's attention and f32 cache, crates/klearu-llm/src/model/       */
+/* kv_cache.rs, stay on the CPU).                                            */
+/*                                                                           */
+/* All of these calls only launch kernels on the context's stream: they      */
+/* allocate nothing, wait for nothing, and can be captured in a CUDA graph   */
+/* (the context's stream is then the capturing one).  Creating and           */
+/* destroying handles allocates and synchronises.                            */
+/* ------------------------------------------------------------------------ */
+typedef struct kl_rope_s* kl_rope_t;
+typedef struct kl_kv4_s* kl_kv4_t;
+typedef struct kl_q8_linear_s* kl_q8_linear_t;
+
+/* Rotary positions: a table of cos(p * inv_freq[i]) * attention_factor and the
+ * sines, p < max_positions, i < rot_dim / 2, computed in 64 bits and held in 32.
+ * inv_freq_host [rot_dim / 2].  The pairs are dims (2i, 2i + 1) with
+ * interleaved, else (i, i + rot_dim / 2); dims from rot_dim on are not turned. */
+KL_API kl_status kl_rope_create(kl_ctx_t ctx, int rot_dim, int64_t max_positions, const double* inv_freq_host,
+                                float attention_factor, int interleaved, kl_rope_t* out);
+KL_API kl_status kl_rope_destroy(kl_rope_t rope);
+
+/* A paged cache of keys and values in 4 bits.  A head vector x is held as codes
+ * c of 4 bits, a step s and a minimum m: x ~ s c + m with m = bf16(min x),
+ * s = bf16((max x - min x) / 15), c = clamp(rint((x - m) / s), 0, 15) (0 where
+ * s is 0); a vector with a value that is not finite reads back as NaN.
+ * page_size: tokens per page, a multiple of 16; head_dim: 64 or 128
+ * (KL_EUNSUPPORTED otherwise).  head_dim + 8 bytes per token and head. */
+KL_API kl_status kl_kv4_create(kl_ctx_t ctx, int64_t num_pages, int page_size, int kv_heads, int head_dim,
+                               kl_kv4_t* out);
+KL_API kl_status kl_kv4_destroy(kl_kv4_t cache);
+
+/* The sequences of a call (device arrays, int32).  Rows cu_q[b] .. cu_q[b + 1]
+ * of the call's token tensors are sequence b's new tokens: the last of its
+ * kv_len[b] tokens, so row cu_q[b] + i is token kv_len[b] - q_len[b] + i.  Token
+ * j of sequence b is in page page_table[b * table_stride + j / page_size].
+ * A row whose token number is negative is padding in front.  Rows behind the
+ * last sequence, and rows of no sequence, are left as they are in every output.
+ * max_q and max_kv are the largest q_len and kv_len: they choose the launch
+ * (a wrong one is slow, not wrong).  Page ids outside the cache, lengths beyond
+ * the table and row ranges beyond num_tokens are reported as KL_EBOUNDS by the
+ * next synchronising call; such tokens are neither written nor attended to. */
+typedef struct {
+  const int32_t* cu_q;       /* [num_seqs + 1], not decreasing */
+  const int32_t* kv_len;     /* [num_seqs] */
+  const int32_t* page_table; /* [num_seqs][table_stride] */
+  int64_t table_stride;
+  int32_t table_width;       /* pages per row */
+  int32_t num_seqs;
+  int32_t num_tokens;        /* rows of the token tensors */
+  int32_t max_q;
+  int32_t max_kv;
+} kl_seq_batch;
+/* bf16 head vectors of tokens, head_dim contiguous; strides in elements. */
+typedef struct {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} kl_head_rows;
+
+/* Turns q and k by their positions (rope NULL: not at all) and writes k and v to
+ * the cache.  positions (nullable, [num_tokens]): else a token's number in its
+ * sequence.  q (nullable with q_heads 0) goes to q_out, which may be q itself.
+ * A padding row's q_out is zero.  A position
+ * outside the rope's table is KL_EBOUNDS (zero q_out, nothing stored).  Two
+ * rows must not name the same token of the same page. */
+KL_API kl_status kl_kv4_append(kl_kv4_t cache, kl_rope_t rope, const kl_seq_batch* seqs_host,
+                               const int32_t* positions, int q_heads, const kl_head_rows* q_host,
+                               const kl_head_rows* k_host, const kl_head_rows* v_host,
+                               const kl_head_rows* q_out_host);
+/* The values that the cached keys and values of the call's tokens stand for
+ * (bf16); zeros for padding rows. */
+KL_API kl_status kl_kv4_read(kl_kv4_t cache, const kl_seq_batch* seqs_host, const kl_head_rows* k_host,
+                             const kl_head_rows* v_host);
+/* out = softmax(scale q . K^T) . V for each token and query head, over the
+ * tokens j <= i of its sequence, and with window > 0 only i - window < j.
+ * Query head h reads key head h / (q_heads / kv_heads).  A token that sees
+ * nothing gets zeros; keys that a token does not see have no effect on it, be
+ * they NaN.  workspace: kl_kv4_attend_workspace bytes for the same arguments,
+ * 16-byte aligned, used until the launched work is done (graphs that may run at
+ * the same time need one each). */
+KL_API kl_status kl_kv4_attend_workspace(kl_kv4_t cache, const kl_seq_batch* seqs_host, int q_heads, int window,
+                                         size_t* bytes_host);
+KL_API kl_status kl_kv4_attend(kl_kv4_t cache, const kl_seq_batch* seqs_host, int q_heads,
+                               const kl_head_rows* q_host, const kl_head_rows* out_host, float scale, int window,
+                               void* workspace, size_t workspace_bytes);
+
+/* Rows of 8-bit codes: h = x (+ residual), u = h * weight (weight NULL: 1;
+ * one_plus_weight: 1 + weight), divided by sqrt(mean(h^2) + eps) with `norm`;
+ * scales[row] = max|u| / 127, codes = rint(127 u / max|u|).  x f32 or bf16
+ * (x_dtype), residual and hidden f32 (nullable); hidden receives h and may be
+ * residual (or x, in f32).  A row whose u is not finite, or whose sum of squares
+ * passes f32, gets scale NaN and codes 0.  1 <= cols <= 49152
+ * (KL_EUNSUPPORTED above). */
+KL_API kl_status kl_norm_q8(kl_ctx_t ctx, const void* x, int x_dtype, int64_t ldx, const float* residual, int64_t ldr,
+                            const float* weight, int rows, int cols, float eps, int norm, int one_plus_weight,
+                            float* hidden, int64_t ldh, int8_t* codes, int64_t ldc, float* scales);
+/* A projection's weights in 8 bits: codes [out_dim][ld] and scales [out_dim]
+ * (device, copied), bias (device, nullable, copied).  in_dim <= 131071, so that
+ * no sum passes 32 bits. */
+KL_API kl_status kl_q8_linear_create(kl_ctx_t ctx, int in_dim, int out_dim, const int8_t* codes, int64_t ld,
+                                     const float* scales, const float* bias, kl_q8_linear_t* out);
+KL_API kl_status kl_q8_linear_destroy(kl_q8_linear_t lin);
+/* out[r][c] = (sum_k a[r][k] w[c][k]) * a_scales[r] * w_scales[c] (+ bias[c]),
+ * added to out with accumulate (f32 only).  a [rows][lda]: base and lda multiples
+ * of 16 bytes.  out f32 or bf16 (out_dtype) [rows][ldo]. */
+KL_API kl_status kl_q8_linear_forward(kl_q8_linear_t lin, const int8_t* a, int64_t lda, const float* a_scales,
+                                      int rows, void* out, int out_dtype, int64_t ldo, int accumulate);
+
+/* ------------------------------------------------------------------------ */
 /* Datasets: LibSVM / XML files and shuffled CSR batches (host memory).      */
 /* These calls take no context; on failure kl_last_error(NULL) returns the   */
 /* message (parse errors name the 1-based line, as the reference does).      */

@@ -71,6 +71,16 @@ class RebuildPolicyC(C.Structure):
 REBUILD_SCHEDULE, REBUILD_ADAPTIVE = 0, 1
 
 
+class SeqBatchC(C.Structure):
+    _fields_ = [("cu_q", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+                ("table_width", C.c_int32), ("num_seqs", C.c_int32), ("num_tokens", C.c_int32), ("max_q", C.c_int32),
+                ("max_kv", C.c_int32)]
+
+
+class HeadRowsC(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
 class LayerStatsC(C.Structure):
     _fields_ = [("active_sum", C.c_uint64), ("touched_rows", C.c_uint64), ("input_nnz", C.c_uint64),
                 ("examples", C.c_uint64), ("steps", C.c_uint64), ("rebuilds", C.c_uint64)]
@@ -163,6 +173,19 @@ _PROTOS = {
     "kl_ffn_stack_create": (_S, [_H, C.c_int, _P, _P, _P, C.c_float, C.c_int, C.POINTER(_H)]),
     "kl_ffn_stack_destroy": (_S, [_H]),
     "kl_ffn_stack_decode": (_S, [_H, _P, C.c_int, C.c_float]),
+    "kl_rope_create": (_S, [_H, C.c_int, C.c_int64, _P, C.c_float, C.c_int, C.POINTER(_H)]),
+    "kl_rope_destroy": (_S, [_H]),
+    "kl_kv4_create": (_S, [_H, C.c_int64, C.c_int, C.c_int, C.c_int, C.POINTER(_H)]),
+    "kl_kv4_destroy": (_S, [_H]),
+    "kl_kv4_append": (_S, [_H, _H, _P, _P, C.c_int, _P, _P, _P, _P]),
+    "kl_kv4_read": (_S, [_H, _P, _P, _P]),
+    "kl_kv4_attend_workspace": (_S, [_H, _P, C.c_int, C.c_int, _P]),
+    "kl_kv4_attend": (_S, [_H, _P, C.c_int, _P, _P, C.c_float, C.c_int, _P, C.c_size_t]),
+    "kl_norm_q8": (_S, [_H, _P, C.c_int, C.c_int64, _P, C.c_int64, _P, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int,
+                        _P, C.c_int64, _P, C.c_int64, _P]),
+    "kl_q8_linear_create": (_S, [_H, C.c_int, C.c_int, _P, C.c_int64, _P, _P, C.POINTER(_H)]),
+    "kl_q8_linear_destroy": (_S, [_H]),
+    "kl_q8_linear_forward": (_S, [_H, _P, C.c_int64, _P, C.c_int, _P, C.c_int, C.c_int64, C.c_int]),
     "kl_libsvm_load": (_S, [C.c_char_p, C.c_int64, C.c_int64, C.c_int, C.POINTER(_H)]),
     "kl_libsvm_parse": (_S, [C.c_char_p, C.c_size_t, C.c_int64, C.c_int64, C.c_int, C.POINTER(_H)]),
     "kl_dataset_from_csr": (_S, [_P, _P, _P, _P, _P, C.c_int64, C.c_int64, C.c_int64, C.POINTER(_H)]),

@@ -10,6 +10,7 @@ Same names, argument meaning and error behaviour as the Rust reference:
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from dataclasses import dataclass
 
 import numpy as np
@@ -41,6 +42,7 @@ class Context:
         if not torch.cuda.is_available():
             raise RuntimeError("klearu_b200 needs a CUDA device (there is no CPU fallback)")
         self.device = device
+        self.launch_lock = threading.Lock()  # held by calls that follow torch's current stream
         self.stream = stream if stream is not None else torch.cuda.current_stream(device)
         h = C.c_void_p()
         check(self.lib.kl_ctx_create(device, C.c_void_p(self.stream.cuda_stream), C.byref(h)), None, "kl_ctx_create")

@@ -23,6 +23,7 @@
 #include <functional>
 
 #include "engine.h"
+#include "kv4.cuh"
 #include "watchdog.h"
 
 using namespace kl;
@@ -3670,5 +3671,256 @@ extern "C" kl_status kl_ffn_stack_decode(kl_ffn_stack_t s, float* hidden, int n_
   }
   ck(cudaGraphLaunch(s->gexec, st), "graph launch");
   count_launch((unsigned)(4 * s->nl));
+  KL_API_END
+}
+
+// ===========================================================================
+// The attention half of a decode step: rotary positions, the paged 4-bit
+// cache, attention over it, 8-bit rows and projections.
+// ===========================================================================
+struct kl_rope_s {
+  kl_ctx_t ctx;
+  int device = 0;
+  int rot = 0, interleaved = 0;
+  int64_t max_pos = 0;
+  DBuf table;  // float2 [max_pos][rot / 2]
+};
+struct kl_kv4_s {
+  kl_ctx_t ctx;
+  int device = 0, head_dim = 0;
+  Kv4View view{};
+  DBuf mem;
+};
+struct kl_q8_linear_s {
+  kl_ctx_t ctx;
+  int device = 0, in = 0, out = 0;
+  int64_t ldw = 0;
+  DBuf w, scale, bias;
+  bool has_bias = false;
+};
+
+namespace {
+// Does not touch the context, which a garbage collector may have destroyed
+// first; freeing device memory waits for the work that uses it.
+template <class H>
+kl_status destroy_handle(H* h) {
+  if (!h) return KL_EINVAL;
+  DeviceGuard guard(h->device);
+  delete h;
+  return KL_OK;
+}
+SeqView seq_view(const kl_seq_batch* s) {
+  require(s != nullptr, "seqs is required");
+  require(s->num_seqs >= 0 && s->num_tokens >= 0 && s->table_width >= 0 && s->table_stride >= s->table_width,
+          "seqs: num_seqs, num_tokens and table_width must be >= 0, table_stride >= table_width");
+  require(s->num_seqs == 0 || (s->cu_q && s->kv_len && (s->page_table || s->table_width == 0)),
+          "seqs: cu_q, kv_len and page_table are required");
+  return SeqView{s->cu_q, s->kv_len, s->page_table, s->table_stride, s->table_width, s->num_seqs, s->num_tokens};
+}
+HeadRows head_rows(const kl_head_rows* r, const char* what) {
+  require(r && r->data, std::string(what) + " is required");
+  require(r->token_stride >= 0 && r->head_stride >= 0, std::string(what) + ": strides must be >= 0");
+  require((reinterpret_cast<uintptr_t>(r->data) & 1) == 0, std::string(what) + ": misaligned bf16 data");
+  const bool vec = (reinterpret_cast<uintptr_t>(r->data) & 15) == 0 && r->token_stride % 8 == 0 && r->head_stride % 8 == 0;
+  return HeadRows{r->data, r->token_stride, r->head_stride, vec ? 1 : 0};
+}
+AttendShape attend_shape(kl_kv4_t c, const kl_seq_batch* s, int q_heads, int window) {
+  require(q_heads >= 1 && q_heads % c->view.kv_heads == 0, "kv4_attend: q_heads must be a multiple of the cache's kv_heads");
+  require(window >= 0, "kv4_attend: window must be >= 0");
+  const int64_t reach = std::min<int64_t>((int64_t)s->table_width * c->view.page_size, INT32_MAX);
+  AttendShape a{};
+  a.D = c->head_dim;
+  a.q_heads = q_heads;
+  a.kv_heads = c->view.kv_heads;
+  a.num_seqs = s->num_seqs;
+  a.num_tokens = s->num_tokens;
+  a.max_q = std::max(1, std::min(s->max_q, s->num_tokens));
+  a.max_kv = (int)std::max<int64_t>(1, std::min<int64_t>(s->max_kv, reach));
+  a.window = window;
+  return a;
+}
+}  // namespace
+
+extern "C" kl_status kl_rope_create(kl_ctx_t ctx, int rot_dim, int64_t max_positions, const double* inv_freq_host,
+                                    float attention_factor, int interleaved, kl_rope_t* out) {
+  if (!ctx || !out) return KL_EINVAL;
+  KL_API_BEGIN(ctx)
+  require(rot_dim >= 2 && rot_dim % 2 == 0, "rope: rot_dim must be even and >= 2");
+  require(max_positions >= 1 && max_positions <= INT32_MAX, "rope: max_positions must be in [1, 2^31)");
+  require(inv_freq_host != nullptr, "rope: inv_freq is required");
+  auto r = std::make_unique<kl_rope_s>();
+  r->ctx = ctx;
+  r->device = ctx->device;
+  r->rot = rot_dim;
+  r->interleaved = interleaved ? 1 : 0;
+  r->max_pos = max_positions;
+  r->table.alloc((size_t)max_positions * (rot_dim / 2) * sizeof(float2));
+  DBuf f;
+  f.alloc((size_t)(rot_dim / 2) * 8);
+  ck(cudaMemcpyAsync(f.p, inv_freq_host, (size_t)(rot_dim / 2) * 8, cudaMemcpyHostToDevice, ctx->stream), "upload");
+  launch_rope_table(f.as<double>(), rot_dim / 2, max_positions, attention_factor, r->table.as<float2>(), ctx->stream);
+  ck_launch("rope table");
+  ck(cudaStreamSynchronize(ctx->stream), "sync");
+  *out = r.release();
+  KL_API_END
+}
+extern "C" kl_status kl_rope_destroy(kl_rope_t r) { return destroy_handle(r); }
+
+extern "C" kl_status kl_kv4_create(kl_ctx_t ctx, int64_t num_pages, int page_size, int kv_heads, int head_dim,
+                                   kl_kv4_t* out) {
+  if (!ctx || !out) return KL_EINVAL;
+  KL_API_BEGIN(ctx)
+  require(num_pages >= 1 && num_pages <= INT32_MAX, "kv4: num_pages must be in [1, 2^31)");
+  require(page_size >= KV4_TILE && page_size % KV4_TILE == 0 && page_size <= (1 << 20),
+          "kv4: page_size must be a multiple of 16, at most 2^20");
+  require(kv_heads >= 1 && kv_heads <= 65535, "kv4: kv_heads must be in [1, 65535]");
+  support(head_dim == 64 || head_dim == 128, "kv4: head_dim must be 64 or 128");
+  const double bytes = (double)num_pages * kv_heads * (page_size / KV4_TILE) * kv4_tile_bytes(head_dim);
+  if (bytes > 1e15) raise(KL_ENOMEM, "kv4: the cache is too large");
+  auto c = std::make_unique<kl_kv4_s>();
+  c->ctx = ctx;
+  c->device = ctx->device;
+  c->head_dim = head_dim;
+  c->mem.alloc((size_t)num_pages * kv_heads * (page_size / KV4_TILE) * kv4_tile_bytes(head_dim));
+  // zero steps and minima: a token that was never written reads as zero
+  ck(cudaMemsetAsync(c->mem.p, 0, c->mem.bytes, ctx->stream), "memset");
+  c->view = Kv4View{c->mem.as<unsigned char>(), num_pages, page_size, kv_heads, page_size / KV4_TILE};
+  ck(cudaStreamSynchronize(ctx->stream), "sync");
+  *out = c.release();
+  KL_API_END
+}
+extern "C" kl_status kl_kv4_destroy(kl_kv4_t c) { return destroy_handle(c); }
+
+extern "C" kl_status kl_kv4_append(kl_kv4_t c, kl_rope_t rope, const kl_seq_batch* seqs_host, const int32_t* positions,
+                                   int q_heads, const kl_head_rows* q_host, const kl_head_rows* k_host,
+                                   const kl_head_rows* v_host, const kl_head_rows* q_out_host) {
+  if (!c) return KL_EINVAL;
+  KL_API_BEGIN(c->ctx)
+  const SeqView s = seq_view(seqs_host);
+  require(q_heads >= 0 && q_heads <= 65535, "kv4_append: q_heads must be in [0, 65535]");
+  require(!rope || rope->ctx == c->ctx, "kv4_append: the rope must share the cache's context");
+  require(!rope || rope->rot <= c->head_dim, "kv4_append: the rope's rot_dim exceeds head_dim");
+  if (s.num_seqs == 0 || s.num_tokens == 0) return KL_OK;
+  HeadRows q{}, qo{};
+  if (q_heads) {
+    q = head_rows(q_host, "kv4_append: q");
+    qo = head_rows(q_out_host, "kv4_append: q_out");
+  }
+  const HeadRows k = head_rows(k_host, "kv4_append: k"), v = head_rows(v_host, "kv4_append: v");
+  launch_kv4_append(c->view, c->head_dim, s, positions, rope ? rope->table.as<float2>() : nullptr, rope ? rope->rot : 0,
+                    rope ? rope->interleaved : 0, rope ? rope->max_pos : 0, q_heads, q, k, v, qo, ctx__->err.as<int>(),
+                    ctx__->stream);
+  ck_launch("kv4_append");
+  KL_API_END
+}
+
+extern "C" kl_status kl_kv4_read(kl_kv4_t c, const kl_seq_batch* seqs_host, const kl_head_rows* k_host,
+                                 const kl_head_rows* v_host) {
+  if (!c) return KL_EINVAL;
+  KL_API_BEGIN(c->ctx)
+  const SeqView s = seq_view(seqs_host);
+  if (s.num_seqs == 0 || s.num_tokens == 0) return KL_OK;
+  const HeadRows k = head_rows(k_host, "kv4_read: k"), v = head_rows(v_host, "kv4_read: v");
+  launch_kv4_read(c->view, c->head_dim, s, k, v, ctx__->err.as<int>(), ctx__->stream);
+  ck_launch("kv4_read");
+  KL_API_END
+}
+
+extern "C" kl_status kl_kv4_attend_workspace(kl_kv4_t c, const kl_seq_batch* seqs_host, int q_heads, int window,
+                                             size_t* bytes_host) {
+  if (!c) return KL_EINVAL;
+  KL_API_BEGIN(c->ctx)
+  require(bytes_host != nullptr, "kv4_attend_workspace: bytes_host is required");
+  const SeqView s = seq_view(seqs_host);
+  *bytes_host = s.num_seqs && s.num_tokens ? attend_workspace(attend_shape(c, seqs_host, q_heads, window)) : 0;
+  KL_API_END
+}
+
+extern "C" kl_status kl_kv4_attend(kl_kv4_t c, const kl_seq_batch* seqs_host, int q_heads, const kl_head_rows* q_host,
+                                   const kl_head_rows* out_host, float scale, int window, void* workspace,
+                                   size_t workspace_bytes) {
+  if (!c) return KL_EINVAL;
+  KL_API_BEGIN(c->ctx)
+  const SeqView s = seq_view(seqs_host);
+  const AttendShape shape = attend_shape(c, seqs_host, q_heads, window);
+  require(std::isfinite(scale), "kv4_attend: scale must be finite");
+  if (s.num_seqs == 0 || s.num_tokens == 0) return KL_OK;
+  const HeadRows q = head_rows(q_host, "kv4_attend: q"), o = head_rows(out_host, "kv4_attend: out");
+  const size_t need = attend_workspace(shape);
+  require(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+          "kv4_attend: the workspace is missing, too small or not 16-byte aligned");
+  const AttendArgs a{c->view, s, q_heads, q, o, scale, window, static_cast<float*>(workspace), ctx__->err.as<int>()};
+  launch_attend(a, shape, ctx__->stream);
+  ck_launch("kv4_attend");
+  KL_API_END
+}
+
+extern "C" kl_status kl_norm_q8(kl_ctx_t ctx, const void* x, int x_dtype, int64_t ldx, const float* residual,
+                                int64_t ldr, const float* weight, int rows, int cols, float eps, int norm,
+                                int one_plus_weight, float* hidden, int64_t ldh, int8_t* codes, int64_t ldc,
+                                float* scales) {
+  if (!ctx) return KL_EINVAL;
+  KL_API_BEGIN(ctx)
+  require(rows >= 0 && cols >= 1, "norm_q8: rows must be >= 0, cols >= 1");
+  require(x_dtype == KL_DTYPE_F32 || x_dtype == KL_DTYPE_BF16, "norm_q8: x must be f32 or bf16");
+  support(cols <= NORM_Q8_MAX_COLS, "norm_q8: more than 49152 columns are not supported");
+  require(eps >= 0.f, "norm_q8: eps must be >= 0");
+  if (rows == 0) return KL_OK;
+  require(x && codes && scales, "norm_q8: x, codes and scales are required");
+  require(ldx >= cols && ldc >= cols && (!residual || ldr >= cols) && (!hidden || ldh >= cols),
+          "norm_q8: a row stride is below cols");
+  const NormQ8Args a{x, residual, weight, hidden, codes, scales, ldx, ldr, ldh, ldc, cols, eps,
+                     one_plus_weight ? 1 : 0, norm ? 1 : 0, x_dtype == KL_DTYPE_BF16 ? 1 : 0};
+  launch_norm_q8(a, rows, ctx__->stream);
+  ck_launch("norm_q8");
+  KL_API_END
+}
+
+extern "C" kl_status kl_q8_linear_create(kl_ctx_t ctx, int in_dim, int out_dim, const int8_t* codes, int64_t ld,
+                                         const float* scales, const float* bias, kl_q8_linear_t* out) {
+  if (!ctx || !out) return KL_EINVAL;
+  KL_API_BEGIN(ctx)
+  require(in_dim >= 1 && out_dim >= 1, "q8_linear: dimensions must be >= 1");
+  support(in_dim <= 131071, "q8_linear: in_dim above 131071 (sums would pass 32 bits)");
+  require(codes && scales && ld >= in_dim, "q8_linear: codes and scales are required, ld >= in_dim");
+  auto l = std::make_unique<kl_q8_linear_s>();
+  l->ctx = ctx;
+  l->device = ctx->device;
+  l->in = in_dim;
+  l->out = out_dim;
+  l->ldw = round_up(in_dim, 128);
+  l->w.alloc((size_t)l->ldw * out_dim);
+  l->scale.alloc((size_t)out_dim * 4);
+  launch_q8_pack(codes, ld, out_dim, in_dim, l->w.as<int8_t>(), l->ldw, ctx->stream);
+  ck_launch("q8_linear pack");
+  ck(cudaMemcpyAsync(l->scale.p, scales, (size_t)out_dim * 4, cudaMemcpyDeviceToDevice, ctx->stream), "copy");
+  l->has_bias = bias != nullptr;
+  if (bias) {
+    l->bias.alloc((size_t)out_dim * 4);
+    ck(cudaMemcpyAsync(l->bias.p, bias, (size_t)out_dim * 4, cudaMemcpyDeviceToDevice, ctx->stream), "copy");
+  }
+  ck(cudaStreamSynchronize(ctx->stream), "sync");
+  *out = l.release();
+  KL_API_END
+}
+extern "C" kl_status kl_q8_linear_destroy(kl_q8_linear_t l) { return destroy_handle(l); }
+
+extern "C" kl_status kl_q8_linear_forward(kl_q8_linear_t l, const int8_t* a, int64_t lda, const float* a_scales,
+                                          int rows, void* out, int out_dtype, int64_t ldo, int accumulate) {
+  if (!l) return KL_EINVAL;
+  KL_API_BEGIN(l->ctx)
+  require(rows >= 0, "q8_linear_forward: rows must be >= 0");
+  require(out_dtype == KL_DTYPE_F32 || out_dtype == KL_DTYPE_BF16, "q8_linear_forward: out must be f32 or bf16");
+  require(!accumulate || out_dtype == KL_DTYPE_F32, "q8_linear_forward: accumulate needs an f32 out");
+  if (rows == 0) return KL_OK;
+  require(a && a_scales && out, "q8_linear_forward: a, a_scales and out are required");
+  require((reinterpret_cast<uintptr_t>(a) & 15) == 0 && lda % 16 == 0 && lda >= l->in,
+          "q8_linear_forward: a's rows must start on 16 bytes, lda >= in_dim");
+  require(ldo >= l->out, "q8_linear_forward: ldo is below out_dim");
+  const Q8Args q{a, l->w.as<int8_t>(), a_scales, l->scale.as<float>(), l->has_bias ? l->bias.as<float>() : nullptr,
+                 out, lda, l->ldw, ldo, rows, l->out, l->in, out_dtype == KL_DTYPE_BF16 ? 1 : 0, accumulate ? 1 : 0,
+                 ctx__->err.as<int>()};
+  launch_q8_matmul(q, ctx__->stream);
+  ck_launch("q8_linear_forward");
   KL_API_END
 }

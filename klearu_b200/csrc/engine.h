@@ -397,4 +397,50 @@ void launch_residual_add(float* h, const float* d, int64_t n, cudaStream_t st);
 
 void launch_set_opt(OptStep* dst, const OptStep& v, cudaStream_t st);
 
+// ---- rotary positions and the paged 4-bit key/value cache (kv4.cu, attend.cu) ----
+struct Kv4View;
+struct SeqView;
+struct HeadRows;
+struct AttendArgs;
+struct AttendShape;
+void launch_rope_table(const double* inv_freq, int pairs, int64_t n, float factor, float2* table, cudaStream_t st);
+void launch_kv4_append(const Kv4View& cache, int D, const SeqView& seq, const int32_t* positions, const float2* table,
+                       int rot, int interleaved, int64_t max_pos, int q_heads, const HeadRows& q, const HeadRows& k,
+                       const HeadRows& v, const HeadRows& q_out, int* err, cudaStream_t st);
+void launch_kv4_read(const Kv4View& cache, int D, const SeqView& seq, const HeadRows& k, const HeadRows& v, int* err,
+                     cudaStream_t st);
+size_t attend_workspace(const AttendShape& s);
+void launch_attend(const AttendArgs& a, const AttendShape& s, cudaStream_t st);
+
+// ---- 8-bit rows and products (q8.cu) ----
+constexpr int NORM_Q8_MAX_COLS = 49152;  // a row of f32 in shared memory
+struct NormQ8Args {
+  const void* x;
+  const float* residual;  // nullable
+  const float* weight;    // nullable: ones
+  float* hidden;          // nullable; may be residual, or x where x is f32
+  int8_t* codes;
+  float* scales;
+  int64_t ldx, ldr, ldh, ldc;
+  int cols;
+  float eps;
+  int one_plus, norm, x_bf16;
+};
+void launch_norm_q8(const NormQ8Args& a, int rows, cudaStream_t st);
+// A [m][lda] (rows on 16 bytes), W [n][ldw] zero from k to ldw, ldw a multiple of 128.
+struct Q8Args {
+  const int8_t* a;
+  const int8_t* w;
+  const float* a_scale;
+  const float* w_scale;
+  const float* bias;  // nullable
+  void* out;
+  int64_t lda, ldw, ldo;
+  int m, n, k;
+  int out_bf16, accumulate;
+  int* err;
+};
+void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, int64_t ldw, cudaStream_t st);
+void launch_q8_matmul(const Q8Args& a, cudaStream_t st);
+
 }  // namespace kl
