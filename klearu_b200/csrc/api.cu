@@ -3920,7 +3920,7 @@ extern "C" kl_status kl_q8_linear_forward(kl_q8_linear_t l, const int8_t* a, int
   const Q8Args q{a, l->w.as<int8_t>(), a_scales, l->scale.as<float>(), l->has_bias ? l->bias.as<float>() : nullptr,
                  out, lda, l->ldw, ldo, rows, l->out, l->in, out_dtype == KL_DTYPE_BF16 ? 1 : 0, accumulate ? 1 : 0,
                  ctx__->err.as<int>()};
-  launch_q8_matmul(q, ctx__->stream);
+  if (!launch_q8_matmul(q, ctx__->stream)) raise(KL_ECUDA, "q8_linear_forward: a TMA tensor map could not be encoded");
   ck_launch("q8_linear_forward");
   KL_API_END
 }

@@ -441,6 +441,7 @@ struct Q8Args {
   int* err;
 };
 void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, int64_t ldw, cudaStream_t st);
-void launch_q8_matmul(const Q8Args& a, cudaStream_t st);
+// False when a tensor map could not be encoded (nothing launched).
+bool launch_q8_matmul(const Q8Args& a, cudaStream_t st);
 
 }  // namespace kl

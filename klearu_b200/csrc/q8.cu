@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "engine.h"
+#include "tcgen05.cuh"
 
 namespace kl {
 namespace {
@@ -88,9 +89,27 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
   }
 }
 
-__device__ __forceinline__ void q8_store(const Q8Args& a, int64_t r, int64_t c, int acc) {
-  float v = (float)acc * a.a_scale[r] * a.w_scale[c];
-  if (a.bias) v += a.bias[c];
+// ---- the product ----
+// out^T in tiles: 128 output channels (rows of W: the MMA's M) by nt rows of A
+// (its N), so that the weights, the larger operand of a decode step, fill the
+// 128 lanes whatever the number of rows, and a warp's stores of one row of out
+// are 32 neighbouring channels.  Both operands arrive by TMA in boxes of 128
+// bytes of K (128-byte swizzle), four MMAs of K = 32 each; rows and K beyond
+// the matrices arrive as zeros.
+constexpr int Q8_KB = 128;               // bytes of K per stage
+constexpr int Q8_WTILE = 128 * Q8_KB;    // weight bytes of a stage
+
+struct Q8Tile {
+  int nt;      // rows of A per tile, a multiple of 16
+  int stages;
+  int kc;      // K chunks of 128
+  uint32_t tmem_cols;
+};
+
+__device__ __forceinline__ float q8_value(const Q8Args& a, int acc, float sa, float sw, float bias) {
+  return fmaf((float)acc * sa, sw, bias);
+}
+__device__ __forceinline__ void q8_store(const Q8Args& a, int64_t r, int64_t c, float v) {
   if (a.out_bf16) {
     static_cast<__nv_bfloat16*>(a.out)[r * a.ldo + c] = __float2bfloat16_rn(v);
   } else {
@@ -99,17 +118,236 @@ __device__ __forceinline__ void q8_store(const Q8Args& a, int64_t r, int64_t c, 
   }
 }
 
-// One thread per output, four products an instruction.
-__global__ void q8_simple_kernel(Q8Args a) {
-  const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, r = blockIdx.y;
-  if (c >= a.n) return;
-  const int8_t* x = a.a + r * a.lda;
-  const int8_t* w = a.w + c * a.ldw;
-  int acc = 0, k = 0;
-  for (; k + 4 <= a.k; k += 4)
-    acc = __dp4a(*reinterpret_cast<const int*>(x + k), *reinterpret_cast<const int*>(w + k), acc);
-  for (; k < a.k; ++k) acc += (int)x[k] * (int)w[k];
-  q8_store(a, r, c, acc);
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ int ld_cluster(uint32_t saddr, uint32_t rank) {
+  uint32_t p;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(p) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(p) : "memory");
+  return v;
+}
+
+// The TMA side of a tile: K chunks [c0, c1) through the ring; q counts chunks
+// since the kernel began.  False when a wait gave up.
+__device__ __forceinline__ bool q8_load(const CUtensorMap* wm, const CUtensorMap* am, const Q8Tile& t, unsigned char* sm,
+                                        uint64_t* full, uint64_t* empty, int ch, int row, int c0, int c1, uint32_t& q,
+                                        volatile int* fail) {
+  const int stage = Q8_WTILE + t.nt * Q8_KB;
+  for (int c = c0; c < c1; ++c, ++q) {
+    const int s = (int)(q % t.stages);
+    const uint32_t round = q / t.stages;
+    if (*fail || (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1u))) return false;
+    mbar_arrive_expect_tx(&full[s], (uint32_t)stage);
+    tma_load_2d(sm + s * stage, wm, c * Q8_KB, ch, &full[s]);
+    tma_load_2d(sm + s * stage + Q8_WTILE, am, c * Q8_KB, row, &full[s]);
+  }
+  return true;
+}
+__device__ __forceinline__ bool q8_mma(const Q8Tile& t, unsigned char* sm, uint64_t* full, uint64_t* empty, uint32_t tmem,
+                                       int chunks, uint32_t& q, volatile int* fail) {
+  const int stage = Q8_WTILE + t.nt * Q8_KB;
+  const uint32_t idesc = i8_idesc(128, t.nt);
+  for (int c = 0; c < chunks; ++c, ++q) {
+    const int s = (int)(q % t.stages);
+    if (*fail || !mbar_wait(&full[s], (q / t.stages) & 1u)) return false;
+    tc5_fence_after();
+    const uint64_t dw = sw128_desc(smem_u32(sm + s * stage)), da = sw128_desc(smem_u32(sm + s * stage + Q8_WTILE));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) tc5_mma_i8(tmem, dw + 2 * k, da + 2 * k, idesc, (c | k) != 0);
+    tc5_commit(&empty[s]);
+  }
+  return true;
+}
+// no copy may be in flight when the block ends
+__device__ __forceinline__ void q8_drain(const Q8Tile& t, uint64_t* full, uint32_t q) {
+  for (uint32_t r = q > (uint32_t)t.stages ? q - t.stages : 0; r < q; ++r)
+    mbar_wait(&full[r % t.stages], (r / t.stages) & 1u);
+}
+
+// Few tiles: one tile per cluster, its K split over the cluster's blocks; the
+// 32-bit sums of the others are read over distributed shared memory (whole
+// numbers: any order gives the same sum), each block finishing its share of
+// the tile's rows.  One launch, no workspace.
+__global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ CUtensorMap wm,
+                                                       const __grid_constant__ CUtensorMap am, Q8Args a, Q8Tile t,
+                                                       int splits) {
+  extern __shared__ unsigned char q8_dyn[];
+  __shared__ uint64_t full[12], empty[12], done;
+  __shared__ uint32_t tmem_s;
+  __shared__ int fail;
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(q8_dyn) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = splits > 1 ? (int)cluster_rank() : 0;
+  const int ch = (blockIdx.x / splits) * 128, row = blockIdx.y * t.nt;
+  const int c0 = (int)((int64_t)t.kc * rank / splits), c1 = (int)((int64_t)t.kc * (rank + 1) / splits);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < t.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&done, 1);
+    fail = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tc5_alloc(&tmem_s, t.tmem_cols);
+  tc5_fence_before();
+  __syncthreads();
+  tc5_fence_after();
+  const uint32_t tmem = tmem_s;
+  if (warp == 0 && lane == 0) {
+    uint32_t q = 0;
+    if (!q8_load(&wm, &am, t, sm, full, empty, ch, row, c0, c1, q, &fail)) atomicExch(&fail, 1);
+    q8_drain(t, full, q);
+  } else if (warp == 1 && lane == 0) {
+    uint32_t q = 0;
+    if (!q8_mma(t, sm, full, empty, tmem, c1 - c0, q, &fail)) atomicExch(&fail, 1);
+    tc5_commit(&done);
+    if (!mbar_wait(&done, 0)) atomicExch(&fail, 1);
+  }
+  __syncthreads();
+  tc5_fence_after();
+  const int c = ch + threadIdx.x;
+  const float sw = c < a.n ? a.w_scale[c] : 0.f, bias = a.bias && c < a.n ? a.bias[c] : 0.f;
+  const uint32_t mine = tmem + ((uint32_t)warp << 21);  // lane 32 * warp
+  const int rows = min(t.nt, a.m - row);
+  if (splits == 1) {
+    for (int j = 0; j < rows; j += 16) {
+      uint32_t v[16];
+      tc5_ld16_async(mine + j, v);
+      tc5_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c < a.n && j + i < rows) q8_store(a, row + j + i, c, q8_value(a, (int)v[i], a.a_scale[row + j + i], sw, bias));
+    }
+  } else {
+    int* part = reinterpret_cast<int*>(sm);  // [row][channel]; the ring has no copy in flight and no MMA reads it
+    for (int j = 0; j < rows; j += 16) {
+      uint32_t v[16];
+      tc5_ld16_async(mine + j, v);
+      tc5_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part[(j + i) * 128 + threadIdx.x] = c0 < c1 ? (int)v[i] : 0;
+    }
+    __syncwarp();
+    cluster_sync();
+    for (int j = rank; j < rows; j += splits) {
+      int acc = 0;
+      const uint32_t at = smem_u32(part + j * 128 + threadIdx.x);
+      for (int r = 0; r < splits; ++r) acc += ld_cluster(at, (uint32_t)r);
+      if (c < a.n) q8_store(a, row + j, c, q8_value(a, acc, a.a_scale[row + j], sw, bias));
+    }
+    __syncwarp();
+    cluster_sync();  // the other blocks may still read this one's sums
+  }
+  tc5_fence_before();
+  __syncthreads();
+  if (fail && threadIdx.x == 0) atomicOr(a.err, DERR_TIMEOUT);
+  if (warp == 1) tc5_dealloc(tmem, t.tmem_cols);
+}
+
+// Many tiles: one block per SM takes tiles in turn, two accumulators in tensor
+// memory so that the tile before is written while the next one multiplies.
+constexpr int Q8_PN = 256;
+constexpr int Q8_PNT = 192;
+__global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_constant__ CUtensorMap wm,
+                                                                  const __grid_constant__ CUtensorMap am, Q8Args a,
+                                                                  Q8Tile t, int ch_tiles, int tiles) {
+  extern __shared__ unsigned char q8_dyn[];
+  __shared__ uint64_t full[12], empty[12], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_s;
+  __shared__ int fail;
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(q8_dyn) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < t.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+    }
+    fail = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tc5_alloc(&tmem_s, 512);
+  tc5_fence_before();
+  __syncthreads();
+  tc5_fence_after();
+  const uint32_t tmem = tmem_s;
+  volatile int* vf = &fail;
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t q = 0;
+      for (int i = blockIdx.x; i < tiles; i += gridDim.x)
+        if (!q8_load(&wm, &am, t, sm, full, empty, i % ch_tiles * 128, i / ch_tiles * Q8_PN, 0, t.kc, q, vf)) {
+          atomicExch(&fail, 1);
+          break;
+        }
+      q8_drain(t, full, q);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      uint32_t q = 0;
+      int n = 0;
+      for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
+        const int b = n & 1;
+        if ((n >= 2 && !mbar_wait(&acc_empty[b], (uint32_t)(n / 2 - 1) & 1u)) ||
+            (tc5_fence_after(), !q8_mma(t, sm, full, empty, tmem + b * Q8_PN, t.kc, q, vf))) {
+          atomicExch(&fail, 1);
+          break;
+        }
+        tc5_commit(&acc_full[b]);
+      }
+    }
+  } else {
+    const int quad = warp & 3;  // the tensor-memory lanes that this warp may read
+    int n = 0;
+    for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
+      const int b = n & 1;
+      const int c = i % ch_tiles * 128 + quad * 32 + lane, row = i / ch_tiles * Q8_PN;
+      const int rows = min(Q8_PN, a.m - row);
+      const float sw = c < a.n ? a.w_scale[c] : 0.f, bias = a.bias && c < a.n ? a.bias[c] : 0.f;
+      if (*vf || !mbar_wait(&acc_full[b], (uint32_t)(n / 2) & 1u)) {
+        atomicExch(&fail, 1);
+        break;
+      }
+      tc5_fence_after();
+      for (int j = 0; j < rows; j += 16) {
+        uint32_t v[16];
+        tc5_ld16_async(tmem + ((uint32_t)quad << 21) + b * Q8_PN + j, v);
+        tc5_ld_wait();
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+          if (c < a.n && j + u < rows)
+            q8_store(a, row + j + u, c, q8_value(a, (int)v[u], a.a_scale[row + j + u], sw, bias));
+      }
+      tc5_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[b]);
+    }
+  }
+  tc5_fence_before();
+  __syncthreads();
+  if (fail && threadIdx.x == 0) atomicOr(a.err, DERR_TIMEOUT);
+  if (warp == 1) tc5_dealloc(tmem, 512);
+}
+
+int q8_sms() {
+  static int n = [] {
+    int dev = 0, v = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+    return v;
+  }();
+  return n;
 }
 
 __global__ void q8_pack_kernel(const int8_t* src, int64_t ld, int k, int8_t* dst, int64_t ldw) {
@@ -139,15 +377,75 @@ void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, in
         src + r * ld, ld, k, dst + r * ldw, ldw), count_launch();
 }
 
-void launch_q8_matmul(const Q8Args& a, cudaStream_t st) {
-  for (int r = 0; r < a.m; r += 65535) {
-    Q8Args b = a;
-    b.a += r * a.lda;
-    b.a_scale += r;
-    b.out = static_cast<char*>(a.out) + r * a.ldo * (a.out_bf16 ? 2 : 4);
-    q8_simple_kernel<<<dim3((unsigned)ceil_div(a.n, 128), std::min(65535, a.m - r)), 128, 0, st>>>(b);
-    count_launch();
+// Rows per tile and splits of K for few tiles.  A block streams its share of
+// the weights at the memory's rate and pays about as much again as 64 KB of
+// them for filling its ring and joining; two blocks fit an SM up to 64 rows.
+struct Q8Plan {
+  bool persistent;
+  int nt, splits;
+};
+static Q8Plan q8_plan(const Q8Args& a) {
+  const int sms = q8_sms();
+  const int ch = (int)ceil_div(a.n, 128), kc = (int)ceil_div(a.k, Q8_KB);
+  int nt = 16;
+  while (nt < 256 && nt < a.m) nt *= 2;
+  const int64_t tiles = ceil_div(a.m, nt) * ch;
+  if (nt == 256 && tiles >= 2 * sms) return {true, 256, 1};
+  Q8Plan best{false, nt, 1};
+  double least = 1e30;
+  const int resident = sms * (nt <= 64 ? 2 : 1);
+  for (int s = 1; s <= 8 && s <= std::max(1, kc); s *= 2) {
+    const double bytes = (double)ceil_div(kc, s) * (Q8_WTILE + nt * Q8_KB);
+    const double cost = (double)ceil_div(tiles * s, resident) * (bytes + (s > 1 ? 96.0 : 64.0) * 1024);
+    if (cost < least) {
+      least = cost;
+      best.splits = s;
+    }
   }
+  return best;
+}
+
+bool launch_q8_matmul(const Q8Args& a, cudaStream_t st) {
+  static OncePerDevice once;
+  once([] {
+    cudaFuncSetAttribute(q8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    cudaFuncSetAttribute(q8_persistent_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+  });
+  const Q8Plan p = q8_plan(a);
+  const int kc = (int)ceil_div(a.k, Q8_KB), stage = Q8_WTILE + p.nt * Q8_KB;
+  CUtensorMap wm, am;
+  if (!tma_map_u8(&wm, a.w, a.n, a.ldw, a.ldw, Q8_KB, 128) || !tma_map_u8(&am, a.a, a.m, a.k, a.lda, Q8_KB, p.nt)) {
+    return false;
+  }
+  Q8Tile t{p.nt, 0, kc, 32};
+  while ((int)t.tmem_cols < p.nt) t.tmem_cols *= 2;
+  const int ch = (int)ceil_div(a.n, 128);
+  const int64_t row_tiles = ceil_div(a.m, p.nt);
+  if (p.persistent) {
+    t.stages = 4;
+    const int64_t tiles = row_tiles * ch;
+    q8_persistent_kernel<<<(unsigned)std::min<int64_t>(tiles, q8_sms()), Q8_PNT, t.stages * stage + 1024, st>>>(
+        wm, am, a, t, ch, (int)tiles);
+    count_launch();
+    return true;
+  }
+  // the ring: up to 104 KB where two blocks share an SM, else up to 200 KB; it also holds the sums to join
+  t.stages = std::min(12, (p.nt <= 64 ? 104 : 200) * 1024 / stage);
+  size_t bytes = (size_t)t.stages * stage;
+  if (p.splits > 1) bytes = std::max(bytes, (size_t)p.nt * 128 * 4);
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = 128;
+  cfg.dynamicSmemBytes = bytes + 1024;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim = {(unsigned)p.splits, 1, 1};
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)(ch * p.splits), (unsigned)row_tiles, 1);
+  cudaLaunchKernelEx(&cfg, q8_split_kernel, wm, am, a, t, p.splits);
+  count_launch();
+  return true;
 }
 
 }  // namespace kl

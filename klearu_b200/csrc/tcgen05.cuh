@@ -36,6 +36,19 @@ __device__ __forceinline__ void tc5_mma(uint32_t tmem, uint64_t da, uint64_t db,
       "l"(da), "l"(db), "r"(idesc), "r"(acc)
       : "memory");
 }
+// kind::i8 instruction descriptor: signed 8-bit A and B, both K-major, 32-bit
+// integer accumulator, M = 128, N = n (a multiple of 16 up to 256); K = 32 per
+// MMA, 32 bytes further inside the swizzle atom.
+__host__ __device__ constexpr uint32_t i8_idesc(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void tc5_mma_i8(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc)
+      : "memory");
+}
 // arrives on `bar` when every MMA this thread issued before it has completed
 __device__ __forceinline__ void tc5_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar))
@@ -81,5 +94,7 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 // refuses the arguments (base or pitch not 16-byte aligned, box too large).
 bool tma_map_bf16(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_cols,
                   int box_rows);
+// The same for a matrix of bytes.
+bool tma_map_u8(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows);
 
 }  // namespace kl
