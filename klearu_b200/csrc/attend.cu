@@ -3,81 +3,500 @@
 // K = ks c + km, V = vs c + vm.  Token i of a sequence (0-based over its whole
 // length) sees tokens j <= i, and with a window w only i - w < j.  A token
 // that sees nothing gets zeros.
+//
+// The steps stay out of the codes: with one step and minimum per head vector,
+//   q . K_j = ks_j (q . c_j) + km_j sum(q),
+//   sum_j p_j V_j = sum_j (p_j vs_j) c_j + sum_j p_j vm_j,
+// so the tensor cores multiply bare codes 0..15, and steps and minima touch
+// one score and one probability per key, not D values.
+#include "attend.cuh"
 #include "engine.h"
-#include "kv4.cuh"
+#include "tcgen05.cuh"
 
 namespace kl {
 namespace {
 
-// One warp per (token, query head), a running maximum and sum in 32 bits.
+constexpr int AT_W = 4;       // warps per block
+constexpr int AT_STAGES = 4;  // tiles in flight per warp
+
+struct SplitPlan {
+  int chunk;      // tokens per block, a multiple of 16 AT_W
+  int chunks;     // blocks along a sequence
+  int row_tiles;  // blocks along a sequence's rows
+};
+
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the 8 x 8 matrix of 16-bit values whose row g, columns 2t, 2t + 1 lane (g, t) holds, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Codes in nibbles 0 and 4 of w, less 8, as two bf16 whole numbers: 0x4300 | c is 128 + c, less 136 exactly.
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
+  const uint32_t v = (w & 0x000f000fu) | 0x43004300u;
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(v), "r"(0x43084308u));
+  return r;
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// Few rows: decode steps and drafts.  One block takes a chunk of a sequence for
+// up to 8 NR rows (token, query head of one key head); its warps take the
+// chunk's 16-token tiles in turn, each through a ring of its own filled by
+// bulk copies, and join at the end; chunks of a sequence are joined by
+// attend_join_kernel.
+//
+// S^T = K . Q^T and O^T = V^T . P^T, so keys fill the 16 rows of a matrix
+// fragment and query rows its 8 columns.  A K code is used as it stands: its
+// nibble in an f16 register is the number c 2^-24 (or 16 c 2^-24 for the
+// second nibble of a byte, q there divided by 16), exact in the product; q is
+// scaled by a power of two into f16's range, which loses what is below 2^-37
+// of the row's largest.  V codes become bf16, as P has to be, whose range a
+// step may need; they are taken less 8, about the middle of their vector, so
+// that rounding a probability times its step to bf16 (half a step, 2^-8) errs
+// on about what a bf16 P would on V itself.  Sums, maxima and O are f32.
+//
+// Bound by memory, D + 8 bytes a token and key head; per 16 tokens a warp
+// spends about 100 logic instructions on the nibbles, half the rate at which
+// the memory delivers them.
+template <int D, int NR>
+__global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kernel(AttendArgs a, SplitPlan p) {
+  constexpr int TB = kv4_tile_bytes(D), CODES = kv4_codes(D);
+  constexpr int KW = D / 32;  // words of K per lane and token
+  constexpr int MT = D / 16;  // O^T fragments
+  constexpr int RING = AT_W * AT_STAGES * TB, JOIN = AT_W * 8 * NR * D * 4;
+  __shared__ __align__(128) unsigned char ring[RING > JOIN ? RING : JOIN];
+  __shared__ uint64_t full[AT_W][AT_STAGES];
+  __shared__ int tile_ok[AT_W][AT_STAGES];
+  __shared__ float2 ml[AT_W][8 * NR];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int kvh = blockIdx.y, group = a.q_heads / a.cache.kv_heads, ps = a.cache.page_size;
+  const int chunk_id = blockIdx.x / p.row_tiles;
+  unsigned char* mine = ring + warp * AT_STAGES * TB;
+  if (lane < AT_STAGES) mbar_init(&full[warp][lane], 1);
+  fence_mbar_init();
+  __syncthreads();
+  uint32_t used = 0;  // tiles that this warp has put through its ring
+  const float log2e = 1.4426950408889634f;
+
+  for (int b = blockIdx.z; b < a.seq.num_seqs; b += gridDim.z) {
+    bool bad = false;
+    const SeqSpan s = seq_span(a.seq, b, ps, &bad);
+    if (bad && threadIdx.x == 0) atomicOr(a.err, DERR_BOUNDS);
+    const int rows = s.q_len * group, first = s.kv_len - s.q_len;  // row r is token first + r / group
+    for (int r0 = (blockIdx.x % p.row_tiles) * 8 * NR; r0 < rows; r0 += p.row_tiles * 8 * NR) {
+      // tokens that some row of this tile sees: [lo, hi), this block's share [k0, k1)
+      const int pos0 = first + r0 / group, hi = first + (min(r0 + 8 * NR, rows) - 1) / group + 1;
+      const int lo = (a.window > 0 ? max(0, pos0 - a.window + 1) : 0) & ~15;
+      const int span = max(0, hi - lo);
+      const int chunk = max(p.chunk, (int)round_up(ceil_div(span, p.chunks), 16 * AT_W));
+      const int k0 = min(hi, lo + chunk_id * chunk), k1 = max(k0, min(hi, k0 + chunk));
+      const int t0 = k0 >> 4, tiles = (k1 - k0 + 15) >> 4;  // k0 is a multiple of 16 wherever tiles > 0
+      const int n = tiles > warp ? (tiles - warp + AT_W - 1) / AT_W : 0;  // this warp's tiles: warp, warp + AT_W, ...
+
+      // ---- the ring's first fills: lane i takes the warp's tile i ----
+      const int32_t* table = a.seq.table + b * a.seq.table_ld;
+      const int tpp = a.cache.tiles_per_page;
+      auto issue = [&](int i, int32_t page) {  // by one lane
+        const uint32_t st = (used + i) % AT_STAGES;
+        const int tile = t0 + warp + i * AT_W;
+        const bool ok = page >= 0 && page < a.cache.num_pages;
+        tile_ok[warp][st] = ok;
+        if (ok) {
+          mbar_arrive_expect_tx(&full[warp][st], TB);
+          bulk_load(mine + st * TB, kv4_tile(a.cache, TB, page, kvh, tile % tpp), TB, &full[warp][st]);
+        } else {
+          atomicOr(a.err, DERR_BOUNDS);
+          mbar_arrive(&full[warp][st]);
+        }
+      };
+      if (lane < AT_STAGES && lane < n) issue(lane, table[(t0 + warp + lane * AT_W) / tpp]);
+
+      // ---- q: row g's dims [t D/4, (t+1) D/4), scaled by a power of two ----
+      uint32_t qf[NR][2 * KW][2];
+      float f[NR][2], qs[NR][2];  // of rows 2t, 2t + 1: what a product of codes is worth, and sum(q), in units of log2
+      int pos[NR][2];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const int row = r0 + 8 * r + g;
+        float x[D / 4], top = 0.f, sum = 0.f;
+        bool fin = true;
+        if (row < rows) {
+          const __nv_bfloat16* qp = static_cast<const __nv_bfloat16*>(a.q.p) + (s.row + row / group) * a.q.token +
+                                    (kvh * group + row % group) * a.q.head + t * (D / 4);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) load8_bf16(qp + 8 * i, a.q.vec, x + 8 * i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) {
+          top = fmaxf(top, fabsf(x[i]));
+          sum += x[i];
+          fin = fin && finite_f(x[i]);
+        }
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+        sum += __shfl_xor_sync(FULL, sum, 1);
+        sum += __shfl_xor_sync(FULL, sum, 2);
+        const unsigned bads = __ballot_sync(FULL, !fin);
+        fin = ((bads >> (4 * g)) & 15u) == 0;
+        const int e = fin ? max(-100, min(126, 13 - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
+        const float up = __uint_as_float((uint32_t)(e + 127) << 23), up16 = up * 0.0625f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* y = x + 8 * w + 4 * h;
+            qf[r][2 * w + h][0] = fin ? pack_f16(y[0] * up, y[1] * up) : 0u;
+            qf[r][2 * w + h][1] = fin ? pack_f16(y[2] * up16, y[3] * up16) : 0u;
+          }
+        const float worth = __uint_as_float((uint32_t)(24 - e + 127) << 23) * (a.scale * log2e);
+        const float total = fin ? sum * (a.scale * log2e) : __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f[r][i] = __shfl_sync(FULL, worth, 4 * (2 * t + i));
+          qs[r][i] = __shfl_sync(FULL, total, 4 * (2 * t + i));
+          pos[r][i] = first + (r0 + 8 * r + 2 * t + i) / group;
+        }
+      }
+      const int see_all_to = pos0;  // every row of the tile sees tokens up to here ..
+      const int see_all_from = a.window > 0 ? hi - a.window : 0;  // .. from here
+
+      float o[MT][NR][4], l[NR][2], vb[NR][2], ref[NR][2], lift[NR][2];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[m][r][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          l[r][i] = vb[r][i] = ref[r][i] = 0.f;
+          lift[r][i] = -INFINITY;  // a score above this moves the row's reference
+        }
+      }
+      int32_t next_page = n > AT_STAGES ? table[(t0 + warp + AT_STAGES * AT_W) / tpp] : 0;
+
+      for (int i = 0; i < n; ++i) {
+        const uint32_t st = (used + i) % AT_STAGES;
+        if (!mbar_wait(&full[warp][st], ((used + i) / AT_STAGES) & 1u)) {
+          atomicOr(a.err, DERR_TIMEOUT);
+          // no copy may land where the warps are about to join
+          for (int k = i; k < min(n, i + AT_STAGES); ++k)
+            mbar_wait(&full[warp][(used + k) % AT_STAGES], ((used + k) / AT_STAGES) & 1u);
+          break;
+        }
+        const unsigned char* tile = mine + st * TB;
+        uint32_t kw[2][KW], ve[2][KW / 2], vo[2][KW / 2];
+        if (D == 128) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 k = *reinterpret_cast<const uint4*>(tile + h * 512 + lane * 16);
+            const uint4 v = *reinterpret_cast<const uint4*>(tile + CODES + h * 512 + lane * 16);
+            kw[h][0] = k.x; kw[h][1] = k.y; kw[h][KW - 2] = k.z; kw[h][KW - 1] = k.w;
+            ve[h][0] = v.x; ve[h][KW / 2 - 1] = v.y; vo[h][0] = v.z; vo[h][KW / 2 - 1] = v.w;
+          }
+        } else {
+          const uint4 k = *reinterpret_cast<const uint4*>(tile + lane * 16);
+          const uint4 v = *reinterpret_cast<const uint4*>(tile + CODES + lane * 16);
+          kw[0][0] = k.x; kw[0][1] = k.y; kw[1][0] = k.z; kw[1][1] = k.w;
+          ve[0][0] = v.x; vo[0][0] = v.y; ve[1][0] = v.z; vo[1][0] = v.w;
+        }
+        const uint2 pr[2] = {*reinterpret_cast<const uint2*>(tile + 2 * CODES + g * 8),
+                             *reinterpret_cast<const uint2*>(tile + 2 * CODES + (g + 8) * 8)};
+        const bool ok = tile_ok[warp][st];
+        __syncwarp();  // the stage has been read
+        if (lane == 0 && i + AT_STAGES < n) {
+          issue(i + AT_STAGES, next_page);
+          if (i + AT_STAGES + 1 < n) next_page = table[(t0 + warp + (i + AT_STAGES + 1) * AT_W) / tpp];
+        }
+        if (!ok) continue;
+
+        float x[NR][4];
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) x[r][u] = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t u0 = kw[0][w] >> (8 * h), u1 = kw[1][w] >> (8 * h);
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+              mma_f16(x[r], u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qf[r][2 * w + h][0],
+                      qf[r][2 * w + h][1]);
+          }
+        // x[r][2 k + i]: key g + 8 k, row 2t + i
+        float vs[2], vm[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float ks = __uint_as_float(pr[k].x << 16), km = __uint_as_float(pr[k].x & 0xffff0000u);
+          vs[k] = __uint_as_float(pr[k].y << 16);
+          vm[k] = fmaf(8.f, vs[k], __uint_as_float(pr[k].y & 0xffff0000u));  // what goes with codes less 8
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) x[r][2 * k + u] = fmaf(x[r][2 * k + u] * ks, f[r][u], km * qs[r][u]);
+        }
+        const int j0 = (t0 + warp + i * AT_W) * 16;
+        const bool partial = j0 + 15 > see_all_to || j0 < see_all_from;
+        uint32_t unseen = 0;
+        if (partial) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int j = j0 + g + 8 * (u >> 1), q = pos[r][u & 1];
+              if (j > q || (a.window > 0 && j <= q - a.window)) {
+                x[r][u] = -INFINITY;
+                unseen |= 1u << (4 * r + u);
+              }
+            }
+        }
+        bool up = false;
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) up = up || x[r][u] > lift[r][u] || x[r][2 + u] > lift[r][u];
+        if (__any_sync(FULL, up)) {
+          // move the references to the maxima seen so far (a probability is at most 2^8 until the next move)
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float top = fmaxf(x[r][u], x[r][2 + u]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
+              if (top > lift[r][u] - 8.f || lift[r][u] == -INFINITY) {
+                const bool none = lift[r][u] == -INFINITY;
+                const float now = none ? top : fmaxf(top, ref[r][u]);
+                if (now != -INFINITY) {
+                  const float keep = none ? 0.f : exp2f(ref[r][u] - now);
+                  // sums taken with no finite score so far are NaN or zero: both stay what they are
+                  l[r][u] *= none ? 1.f : keep;
+                  vb[r][u] *= none ? 1.f : keep;
+#pragma unroll
+                  for (int m = 0; m < MT; ++m) {
+                    o[m][r][u] *= none ? 1.f : keep;
+                    o[m][r][2 + u] *= none ? 1.f : keep;
+                  }
+                  ref[r][u] = now;
+                  lift[r][u] = now + 8.f;
+                }
+              }
+            }
+        }
+        uint32_t pb[NR][2];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float w[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float y = exp2_fast(x[r][2 * k + u] - ref[r][u]);
+              l[r][u] += y;
+              w[u] = y * vs[k];
+              if (!partial || !(unseen >> (4 * r + 2 * k + u) & 1u)) vb[r][u] = fmaf(y, vm[k], vb[r][u]);
+            }
+            pb[r][k] = transpose8(pack_bf16(w[0], w[1]));
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < KW / 2; ++w) {
+          uint32_t lo2[2], hi2[2];  // dims 0 2 4 6 and 1 3 5 7 of the word, tokens 2t and 2t + 1 side by side
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            lo2[h] = __byte_perm(ve[h][w], vo[h][w], 0x5410);
+            hi2[h] = __byte_perm(ve[h][w], vo[h][w], 0x7632);
+          }
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const uint32_t a0 = codes_bf16(lo2[0] >> (4 * d)), a1 = codes_bf16(hi2[0] >> (4 * d));
+            const uint32_t a2 = codes_bf16(lo2[1] >> (4 * d)), a3 = codes_bf16(hi2[1] >> (4 * d));
+#pragma unroll
+            for (int r = 0; r < NR; ++r) mma_bf16(o[4 * w + d][r], a0, a1, a2, a3, pb[r][0], pb[r][1]);
+          }
+        }
+      }
+      used += n;
+
+      // ---- join the warps: every warp's rows [8 NR][D] and (reference, sum) in shared memory ----
+      __syncthreads();
+      float* part = reinterpret_cast<float*>(ring);
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            l[r][u] += __shfl_xor_sync(FULL, l[r][u], d);
+            vb[r][u] += __shfl_xor_sync(FULL, vb[r][u], d);
+          }
+          const int row = 8 * r + 2 * t + u;
+          float* at = part + (warp * 8 * NR + row) * D + g * (D / 8);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            *reinterpret_cast<float2*>(at + 2 * m) = make_float2(o[m][r][u] + vb[r][u], o[m][r][2 + u] + vb[r][u]);
+          if (g == 0) ml[warp][row] = make_float2(lift[r][u] == -INFINITY ? -INFINITY : ref[r][u], l[r][u]);
+        }
+      __syncthreads();
+      for (int e = threadIdx.x; e < 8 * NR * (D / 4); e += AT_W * 32) {
+        const int row = e / (D / 4), d = e % (D / 4) * 4;
+        if (r0 + row >= rows) continue;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < AT_W; ++w) top = fmaxf(top, ml[w][row].x);
+        const float rf = top == -INFINITY ? 0.f : top;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < AT_W; ++w) {
+          const float2 v = ml[w][row];
+          const float keep = exp2f(v.x - rf);
+          const float4 y = *reinterpret_cast<const float4*>(part + (w * 8 * NR + row) * D + d);
+          sum = fmaf(keep, v.y, sum);
+          acc[0] = fmaf(keep, y.x, acc[0]);
+          acc[1] = fmaf(keep, y.y, acc[1]);
+          acc[2] = fmaf(keep, y.z, acc[2]);
+          acc[3] = fmaf(keep, y.w, acc[3]);
+        }
+        const int64_t tok = s.row + (r0 + row) / group;
+        const int head = kvh * group + (r0 + row) % group;
+        if (p.chunks == 1) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          attend_store4(a.out, tok, head, d, acc, inv);
+        } else {
+          const int64_t at = ((int64_t)chunk_id * a.seq.num_tokens + tok) * a.q_heads + head;
+          if (sum != 0.f)
+            *reinterpret_cast<float4*>(join_rows(a, p.chunks) + at * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          if (d == 0) reinterpret_cast<float2*>(a.scratch)[at] = make_float2(top, sum);
+        }
+      }
+      fence_proxy_async_smem();  // the ring, written here by threads, is next written by copies
+      __syncthreads();
+    }
+  }
+}
+
+// One warp per (token, query head): the chunks' rows, brought to one reference
+// and summed in the chunks' order.
 template <int D>
-__global__ void attend_simple_kernel(AttendArgs a) {
-  constexpr int E = D / 32;  // dims per lane
+__global__ void __launch_bounds__(128) attend_join_kernel(AttendArgs a, int chunks) {
+  constexpr int E = D / 32;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  const int head = blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int t = blockIdx.y + blockIdx.z * 65535;
-  if (t >= a.seq.num_tokens) return;
-  const int b = find_seq(a.seq.cu_q, a.seq.num_seqs, t);
-  if (b >= a.seq.num_seqs || head >= a.q_heads) return;
-  bool bad = false;
-  const int ps = a.cache.page_size, kvh = head / (a.q_heads / a.cache.kv_heads);
-  const SeqSpan s = seq_span(a.seq, b, ps, &bad);
-  const int index = s.kv_len - s.q_len + (t - s.row);
-  const __nv_bfloat16* qp = static_cast<const __nv_bfloat16*>(a.q.p) + t * a.q.token + head * a.q.head;
-  float q[E], o[E], m = -INFINITY, l = 0.f;
+  if (i >= (int64_t)a.seq.num_tokens * a.q_heads) return;
+  const int64_t tok = i / a.q_heads;
+  const int head = (int)(i % a.q_heads);
+  if (tok < a.seq.cu_q[0] || tok >= a.seq.cu_q[a.seq.num_seqs]) return;  // a row of no sequence
+  const int64_t step = (int64_t)a.seq.num_tokens * a.q_heads;
+  const float2* ml = reinterpret_cast<const float2*>(a.scratch) + i;
+  const float* rows = join_rows(a, chunks) + i * D + lane * E;
+  float top = -INFINITY;
+  for (int c = lane; c < chunks; c += 32) top = fmaxf(top, ml[c * step].x);
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    q[i] = to_f(qp[lane * E + i]) * a.scale;
-    o[i] = 0.f;
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
+  const float rf = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, acc[E] = {};
+  for (int c = 0; c < chunks; ++c) {
+    const float2 v = ml[c * step];
+    if (v.y == 0.f) continue;  // saw nothing
+    const float keep = exp2f(v.x - rf);
+    sum = fmaf(keep, v.y, sum);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(keep, rows[c * step * D + e], acc[e]);
   }
-  const int first = a.window > 0 ? max(0, index - a.window + 1) : 0;
-  for (int j = first; j <= index; ++j) {
-    const int64_t page = a.seq.table[b * a.seq.table_ld + j / ps];
-    if (page < 0 || page >= a.cache.num_pages) {
-      bad = true;
-      continue;
-    }
-    const int off = j % ps, tok = off & 15;
-    const unsigned char* tile = kv4_tile(a.cache, kv4_tile_bytes(D), page, kvh, off >> 4);
-    const uint2 pr = *reinterpret_cast<const uint2*>(tile + 2 * kv4_codes(D) + tok * 8);
-    const int w = lane * E / 8;
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(tile + kv4_k_off<D>(tok, w));
-    const uint32_t vw = *reinterpret_cast<const uint32_t*>(tile + kv4_codes(D) + kv4_v_off<D>(tok, w));
-    const float ks = __uint_as_float(pr.x << 16), km = __uint_as_float(pr.x & 0xffff0000u);
-    const float vs = __uint_as_float(pr.y << 16), vm = __uint_as_float(pr.y & 0xffff0000u);
-    float x = 0.f;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.p) + tok * a.out.token + head * a.out.head + lane * E;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int e = (lane * E + i) & 7;
-      x = fmaf(q[i], fmaf((float)((kw >> (4 * kv4_nibble(e))) & 15u), ks, km), x);
-    }
-    x = warp_sum_f(x);
-    const float mn = fmaxf(m, x), ref = mn == -INFINITY ? 0.f : mn;
-    const float keep = expf(m - ref), p = expf(x - ref);
-    m = mn;
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int e = (lane * E + i) & 7;
-      o[i] = fmaf(p, fmaf((float)((vw >> (4 * kv4_nibble(e))) & 15u), vs, vm), o[i] * keep);
-    }
-  }
-  if (bad && lane == 0) atomicOr(a.err, DERR_BOUNDS);
-  __nv_bfloat16* op = static_cast<__nv_bfloat16*>(a.out.p) + t * a.out.token + head * a.out.head;
-#pragma unroll
-  for (int i = 0; i < E; ++i) op[lane * E + i] = __float2bfloat16_rn(l == 0.f ? 0.f : o[i] / l);
+  for (int e = 0; e < E; ++e) out[e] = __float2bfloat16_rn(acc[e] * inv);
+}
+
+SplitPlan split_plan(const AttendShape& s) {
+  const int group = s.q_heads / s.kv_heads;
+  const int64_t rows = (int64_t)s.max_q * group;
+  const int nr = rows <= 8 ? 1 : 2;
+  SplitPlan p{};
+  p.row_tiles = (int)std::min<int64_t>(ceil_div(rows, 8 * nr), 64);
+  // the longest stretch of keys that a tile of rows may see
+  int64_t span = s.max_kv;
+  if (s.window > 0) span = std::min<int64_t>(span, (int64_t)s.window + ceil_div(8 * nr, group) + 16);
+  const int64_t items = (int64_t)s.num_seqs * s.kv_heads * p.row_tiles;
+  const int64_t resident = 148 * (nr == 1 ? 4 : 3);
+  // a batch's sequences are ragged: eight turns even them out; a few long ones are cut for one
+  const int64_t want = items >= 148 ? 8 * resident : resident;
+  int64_t chunks = std::max<int64_t>(1, want / items);
+  int64_t chunk = round_up(std::max<int64_t>(ceil_div(span, chunks), 16 * AT_W), 16 * AT_W);
+  chunk = std::max<int64_t>(chunk, std::min<int64_t>(round_up(span, 16 * AT_W), 256));
+  p.chunk = (int)chunk;
+  p.chunks = (int)std::max<int64_t>(1, ceil_div(span, chunk));
+  return p;
+}
+
+template <int D, int NR>
+void launch_split(const AttendArgs& a, const SplitPlan& p, cudaStream_t st) {
+  const dim3 grid((unsigned)(p.chunks * p.row_tiles), (unsigned)a.cache.kv_heads,
+                  (unsigned)std::min(a.seq.num_seqs, 65535));
+  attend_split_kernel<D, NR><<<grid, AT_W * 32, 0, st>>>(a, p);
+  count_launch();
+  if (p.chunks == 1) return;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ceil_div((int64_t)a.seq.num_tokens * a.q_heads, 4));
+  cfg.blockDim = 128;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, a, p.chunks);
+  count_launch();
 }
 
 }  // namespace
 
-size_t attend_workspace(const AttendShape&) { return 0; }
+size_t attend_workspace(const AttendShape& s) {
+  const SplitPlan p = split_plan(s);
+  if (p.chunks == 1) return 0;
+  const int64_t rows = (int64_t)p.chunks * s.num_tokens * s.q_heads;
+  return (size_t)(round_up(rows * 2, 4) + rows * s.D) * 4;
+}
 
 void launch_attend(const AttendArgs& a, const AttendShape& s, cudaStream_t st) {
-  const dim3 grid((unsigned)ceil_div(a.q_heads, 4), (unsigned)std::min(a.seq.num_tokens, 65535),
-                  (unsigned)ceil_div(a.seq.num_tokens, 65535));
-  if (s.D == 128) attend_simple_kernel<128><<<grid, 128, 0, st>>>(a);
-  else attend_simple_kernel<64><<<grid, 128, 0, st>>>(a);
-  count_launch();
+  const SplitPlan p = split_plan(s);
+  const bool one = (int64_t)s.max_q * (s.q_heads / s.kv_heads) <= 8;
+  if (s.D == 128) one ? launch_split<128, 1>(a, p, st) : launch_split<128, 2>(a, p, st);
+  else one ? launch_split<64, 1>(a, p, st) : launch_split<64, 2>(a, p, st);
 }
 
 }  // namespace kl

@@ -39,8 +39,11 @@ def rotate(x, pos, inv_freq, interleaved, factor=1.0):
 def attend(q, k, v, first, window, scale):
     """One sequence: q [rows][heads][dim], row r is token first + r; k, v [tokens][kv_heads][dim] (values held).
     Returns the output and how far a kernel that rounds probabilities, keys and values to bf16 may be off:
-    half a step of the output, of each probability and value (both scale sum p |v|), and of each key, which moves
-    a score by at most HALF * |scale| * sum |q| |k| and the output by twice that times sum p |v|."""
+    half a step of the output, of each value (sum p |v|), of each probability, and of each key, which moves
+    a score by at most HALF * |scale| * sum |q| |k| and the output by twice that times sum p |v|.
+    A probability may be rounded times its step s, on the code less 8: that errs on s |c - 8| =
+    |v - (m + 8 s)| <= |v| + |mid| + s, mid the middle of the vector (codes reach 0 and at least 14, so mid is
+    within s of m + 8 s, and s <= (max - min) / 14)."""
     rows, heads, _ = q.shape
     q = q.double()
     group = heads // k.shape[1]
@@ -62,7 +65,9 @@ def attend(q, k, v, first, window, scale):
         p = torch.where(seen.any(-1, keepdim=True), p / total, 0.0)
         o = p @ torch.nan_to_num(vv)
         a = p @ torch.nan_to_num(vv).abs()
+        lo, hi = torch.nan_to_num(vv).amin(-1), torch.nan_to_num(vv).amax(-1)
+        b = a + (p @ ((lo + hi).abs() / 2 + (hi - lo) / 14))[:, None]
         sway = abs(scale) * (q[:, h].abs() @ torch.nan_to_num(kk).abs().T).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
         out[:, h] = o
-        tol[:, h] = HALF * (o.abs() + 2 * a + 2 * sway * a) + 1e-5 * a + 1e-30
+        tol[:, h] = HALF * (o.abs() + a + b + 2 * sway * a) + 1e-5 * a + 1e-30
     return out, tol
