@@ -22,8 +22,8 @@ PKG = ROOT / "klearu_b200"
 CSRC = PKG / "csrc"
 BUILD = ROOT / "_build" / "gpu"
 LIB = PKG / "libklearu_gpu.so"
-SOURCES = ["hash.cu", "hash_tc.cu", "index.cu", "layer.cu", "shard.cu", "dejavu.cu", "kv4.cu", "attend.cu", "q8.cu", "data.cu",
-           "api.cu"]
+SOURCES = ["hash.cu", "hash_tc.cu", "index.cu", "layer.cu", "shard.cu", "dejavu.cu", "kv4.cu", "attend.cu",
+           "attend_tc.cu", "q8.cu", "data.cu", "api.cu"]
 
 def _nccl_dirs() -> tuple[str, str]:
     """NCCL headers and library: the copy PyTorch itself loads (nvidia-nccl

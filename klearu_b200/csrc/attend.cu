@@ -485,7 +485,12 @@ void launch_split(const AttendArgs& a, const SplitPlan& p, cudaStream_t st) {
 
 }  // namespace
 
+// Above 48 rows of one key head and sequence the tensor-core kernel's 256-row
+// blocks, below it 16-row tiles that read the keys again for each.
+static bool many_rows(const AttendShape& s) { return (int64_t)s.max_q * (s.q_heads / s.kv_heads) > 48; }
+
 size_t attend_workspace(const AttendShape& s) {
+  if (many_rows(s)) return 0;
   const SplitPlan p = split_plan(s);
   if (p.chunks == 1) return 0;
   const int64_t rows = (int64_t)p.chunks * s.num_tokens * s.q_heads;
@@ -493,6 +498,7 @@ size_t attend_workspace(const AttendShape& s) {
 }
 
 void launch_attend(const AttendArgs& a, const AttendShape& s, cudaStream_t st) {
+  if (many_rows(s)) return launch_attend_tc(a, s, st);
   const SplitPlan p = split_plan(s);
   const bool one = (int64_t)s.max_q * (s.q_heads / s.kv_heads) <= 8;
   if (s.D == 128) one ? launch_split<128, 1>(a, p, st) : launch_split<128, 2>(a, p, st);
