@@ -33,14 +33,6 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
-      "%3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // the 8 x 8 matrix of 16-bit values whose row g, columns 2t, 2t + 1 lane (g, t) holds, transposed
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
@@ -50,13 +42,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// Codes in nibbles 0 and 4 of w, less 8, as two bf16 whole numbers: 0x4300 | c is 128 + c, less 136 exactly.
-__device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
-  const uint32_t v = (w & 0x000f000fu) | 0x43004300u;
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(v), "r"(0x43084308u));
   return r;
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -73,17 +58,17 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // attend_join_kernel.
 //
 // S^T = K . Q^T and O^T = V^T . P^T, so keys fill the 16 rows of a matrix
-// fragment and query rows its 8 columns.  A K code is used as it stands: its
-// nibble in an f16 register is the number c 2^-24 (or 16 c 2^-24 for the
-// second nibble of a byte, q there divided by 16), exact in the product; q is
-// scaled by a power of two into f16's range, which loses what is below 2^-37
-// of the row's largest.  V codes become bf16, as P has to be, whose range a
-// step may need; they are taken less 8, about the middle of their vector, so
-// that rounding a probability times its step to bf16 (half a step, 2^-8) errs
-// on about what a bf16 P would on V itself.  Sums, maxima and O are f32.
+// fragment and query rows its 8 columns.  A code is used as it stands: its
+// nibble in an f16 register is the number c 2^-24, the second nibble of a byte
+// 16 c 2^-24 (q, or that dim of O, divided by 16), exact in the product, so a
+// word of 8 codes costs five logic instructions.  q is scaled by a power of two
+// into f16's range, which loses what is below 2^-37 of the row's largest;
+// probabilities go in times their value's step and a power of two 2^-E that
+// keeps the largest so far within f16, rounded to 11 bits (2^-12), and what is
+// 2^-25 below the largest to none.  Sums, maxima and O are f32.
 //
 // Bound by memory, D + 8 bytes a token and key head; per 16 tokens a warp
-// spends about 100 logic instructions on the nibbles, half the rate at which
+// spends about 90 logic instructions on the nibbles, half the rate at which
 // the memory delivers them.
 template <int D, int NR>
 __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kernel(AttendArgs a, SplitPlan p) {
@@ -203,6 +188,14 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
           lift[r][i] = -INFINITY;  // a score above this moves the row's reference
         }
       }
+      float down[NR][2], most[NR][2];  // 2^-E, and the largest weight that it keeps within f16's range
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          down[r][u] = 1.f;
+          most[r][u] = 0.f;
+        }
       int32_t next_page = n > AT_STAGES ? table[(t0 + warp + AT_STAGES * AT_W) / tpp] : 0;
 
       for (int i = 0; i < n; ++i) {
@@ -261,7 +254,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
         for (int k = 0; k < 2; ++k) {
           const float ks = __uint_as_float(pr[k].x << 16), km = __uint_as_float(pr[k].x & 0xffff0000u);
           vs[k] = __uint_as_float(pr[k].y << 16);
-          vm[k] = fmaf(8.f, vs[k], __uint_as_float(pr[k].y & 0xffff0000u));  // what goes with codes less 8
+          vm[k] = __uint_as_float(pr[k].y & 0xffff0000u);
 #pragma unroll
           for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -315,22 +308,46 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
               }
             }
         }
-        uint32_t pb[NR][2];
+        float w[NR][4];
+        bool heavy = false;
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float w[2];
+          for (int u = 0; u < 4; ++u) {
+            const float y = exp2_fast(x[r][u] - ref[r][u & 1]);
+            l[r][u & 1] += y;
+            w[r][u] = y * vs[u >> 1];
+            heavy = heavy || w[r][u] > most[r][u & 1];
+            if (!partial || !(unseen >> (4 * r + u) & 1u)) vb[r][u & 1] = fmaf(y, vm[u >> 1], vb[r][u & 1]);
+          }
+        if (__any_sync(FULL, heavy)) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const float y = exp2_fast(x[r][2 * k + u] - ref[r][u]);
-              l[r][u] += y;
-              w[u] = y * vs[k];
-              if (!partial || !(unseen >> (4 * r + 2 * k + u) & 1u)) vb[r][u] = fmaf(y, vm[k], vb[r][u]);
+              float top = fmaxf(w[r][u], w[r][2 + u]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
+              if (top > most[r][u]) {  // E: this weight at 2^8; later ones may pass it by 2^7
+                const int e = max(-126, min(127, 8 - ((int)(__float_as_uint(top) >> 23) - 127)));
+                const float now = __uint_as_float((uint32_t)(e + 127) << 23);
+                const float keep = most[r][u] == 0.f ? 1.f : now / down[r][u];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                  o[m][r][u] *= keep;
+                  o[m][r][2 + u] *= keep;
+                }
+                down[r][u] = now;
+                most[r][u] = 32768.f / now;
+              }
             }
-            pb[r][k] = transpose8(pack_bf16(w[0], w[1]));
-          }
         }
+        uint32_t pb[NR][2];
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            pb[r][k] = transpose8(pack_f16(w[r][2 * k] * down[r][0], w[r][2 * k + 1] * down[r][1]));
 #pragma unroll
         for (int w = 0; w < KW / 2; ++w) {
           uint32_t lo2[2], hi2[2];  // dims 0 2 4 6 and 1 3 5 7 of the word, tokens 2t and 2t + 1 side by side
@@ -341,10 +358,12 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
           }
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
-            const uint32_t a0 = codes_bf16(lo2[0] >> (4 * d)), a1 = codes_bf16(hi2[0] >> (4 * d));
-            const uint32_t a2 = codes_bf16(lo2[1] >> (4 * d)), a3 = codes_bf16(hi2[1] >> (4 * d));
+            const uint32_t mask = d & 1 ? 0x00f000f0u : 0x000f000fu;
+            const int s = d & 2 ? 8 : 0;
 #pragma unroll
-            for (int r = 0; r < NR; ++r) mma_bf16(o[4 * w + d][r], a0, a1, a2, a3, pb[r][0], pb[r][1]);
+            for (int r = 0; r < NR; ++r)
+              mma_f16(o[4 * w + d][r], lo2[0] >> s & mask, hi2[0] >> s & mask, lo2[1] >> s & mask, hi2[1] >> s & mask,
+                      pb[r][0], pb[r][1]);
           }
         }
       }
@@ -364,9 +383,13 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
           }
           const int row = 8 * r + 2 * t + u;
           float* at = part + (warp * 8 * NR + row) * D + g * (D / 8);
+          const float up = 1.f / down[r][u];
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
-            *reinterpret_cast<float2*>(at + 2 * m) = make_float2(o[m][r][u] + vb[r][u], o[m][r][2 + u] + vb[r][u]);
+          for (int m = 0; m < MT; ++m) {
+            const float f = m & 1 ? 1048576.f : 16777216.f;  // a code is worth 2^-24, or 2^-20
+            *reinterpret_cast<float2*>(at + 2 * m) =
+                make_float2(fmaf(o[m][r][u] * f, up, vb[r][u]), fmaf(o[m][r][2 + u] * f, up, vb[r][u]));
+          }
           if (g == 0) ml[warp][row] = make_float2(lift[r][u] == -INFINITY ? -INFINITY : ref[r][u], l[r][u]);
         }
       __syncthreads();

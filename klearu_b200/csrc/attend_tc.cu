@@ -3,21 +3,28 @@
 //
 // One block takes 256 rows (token, query head) of one key head as two tiles of
 // 128, so that one tile multiplies while the other takes its softmax:
-//  * warps 0-3 and 4-7: softmax of tile 0 and 1, one row per thread, straight
-//    from tensor memory; P goes back there as bf16, over the scores that it
-//    came from; O is rescaled in place only when a row's maximum has risen by
-//    more than 2^8;
+//  * warps 0-3 and 4-7: softmax of tile 0 and 1, one row per thread, its 128
+//    scores in registers; P goes back to tensor memory as f16, over the scores
+//    that it came from; O is rescaled in place only when a row's maximum has
+//    risen by more than 2^8;
 //  * warps 8-11: the next 128 keys and values, codes read from global memory
-//    one tile ahead, turned into bf16 (s c + m in one rounding) and written to
+//    one step ahead, turned into f16 (s c + m in one rounding) and written to
 //    shared memory in the tensor core's swizzled layouts, K with D contiguous,
 //    V as it stands (its tokens are the product's K, "MN-major");
-//  * warp 12: issues S_i = Q_i . K^T and O_i += P_i . V in the order
+//  * a thread of warp 12: issues S_i = Q_i . K^T and O_i += P_i . V in the order
 //    PV_0, S_0, PV_1, S_1 of each step, so the scores' completion also says
 //    that O_i may be rescaled.
+// f16, not bf16, for its 11 bits: with keys, values and probabilities at 2^-12
+// the output is as exact as its own bf16 rounding.  Its range is made up for by
+// powers of two: of each row of Q, of each step's K (both into the score's
+// factor) and V (the step's probabilities are taken times 2^(ev - ev of the
+// first step), which the running reference follows and the row sum takes out).
 // Tensor memory: S_0, S_1 (128 columns each), O_0, O_1 (D columns each).
 //
 // Per 128 keys and 256 rows at D = 128 the tensor cores need 2048 cycles and
 // the 32768 exponentials as many of the special function units.
+#include <cstddef>
+
 #include "attend.cuh"
 #include "engine.h"
 #include "tcgen05.cuh"
@@ -27,7 +34,7 @@ namespace {
 
 constexpr int TC_KV = 128;   // keys per step
 constexpr int TC_ROWS = 256;  // rows per block
-constexpr int TC_NT = 416;   // 13 warps
+constexpr int TC_NT = 512;    // 4 warpgroups
 
 // MN-major operand, 128-byte swizzle: 64 values of N in 128 bytes, 8 of K in
 // 1024; the next 64 of N are lbo bytes on, the next 8 of K 1024.
@@ -35,7 +42,7 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lbo) 
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          (1ull << 46) | (2ull << 61);
 }
-// A from tensor memory (bf16, two values of K per column)
+// A from tensor memory (f16, two values of K per column)
 __device__ __forceinline__ void tc5_mma_ta(uint32_t tmem, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -66,412 +73,534 @@ __device__ __forceinline__ void tc5_st16(uint32_t taddr, const uint32_t* v) {
 }
 __device__ __forceinline__ void tc5_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
-// codes in nibbles 0 and 4 of w as bf16 s c + m, one rounding
+// codes in nibbles 0 and 4 of w as f16 s c + m, one rounding
 __device__ __forceinline__ uint32_t value2(uint32_t w, uint32_t s2, uint32_t m2) {
-  const uint32_t v = (w & 0x000f000fu) | 0x43004300u;  // 128 + c, exact
+  const uint32_t v = (w & 0x000f000fu) | 0x64006400u;  // 1024 + c, exact
   uint32_t c, r;
-  asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(c) : "r"(v), "r"(0x43004300u));
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;\n" : "=r"(r) : "r"(c), "r"(s2), "r"(m2));
+  asm("sub.rn.f16x2 %0, %1, %2;\n" : "=r"(c) : "r"(v), "r"(0x64006400u));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(r) : "r"(c), "r"(s2), "r"(m2));
   return r;
 }
 // the 8 dims of a word as 16 bytes
 __device__ __forceinline__ uint4 values8(uint32_t w, uint32_t s2, uint32_t m2) {
   return make_uint4(value2(w, s2, m2), value2(w >> 4, s2, m2), value2(w >> 8, s2, m2), value2(w >> 12, s2, m2));
 }
-__device__ __forceinline__ bool nan_low(uint32_t pr) { return (pr & 0x7fff0000u) > 0x7f800000u; }  // the minimum is NaN
+__device__ __forceinline__ uint32_t twice_f16(float x) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %1;\n" : "=r"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float bf_low(uint32_t pr) { return __uint_as_float(pr << 16); }           // a step
+__device__ __forceinline__ float bf_high(uint32_t pr) { return __uint_as_float(pr & 0xffff0000u); }  // a minimum
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+// what a vector's values do not pass; zero where its minimum is NaN
+__device__ __forceinline__ uint32_t reach(uint32_t pr) {
+  const float s = bf_low(pr), m = bf_high(pr);
+  return m == m ? __float_as_uint(fmaxf(fabsf(m), fabsf(fmaf(15.f, s, m)))) : 0u;
+}
+// two f32 operations an instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 template <int D>
 struct TcSmem {
-  static constexpr int Q = 128 * D * 2;   // one tile
+  static constexpr int Q = 128 * D * 2;     // one tile
   static constexpr int KV = TC_KV * D * 2;  // one stage of K or V
   static constexpr int BYTES = 2 * Q + 4 * KV + 1024;
 };
 
-struct TcBars {
-  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], done;
+// A step's powers of two and missing pages.
+struct TcStep {
+  unsigned char hole[8];  // 16-token tiles whose page does not exist
+  int ek, ev;             // K is held times 2^-ek, V times 2^-ev
 };
+struct TcShared {
+  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], done;
+  uint32_t tmem;
+  int fail;
+  alignas(16) uint32_t reach[2][2][4];  // by step & 1: largest |K|, |V| of each decoding warp
+  // by step & 3: a step's is written again when the step two on has its scores, after this one's softmax
+  alignas(16) TcStep step[4];
+};
+static_assert(offsetof(TcShared, reach) % 16 == 0 && offsetof(TcShared, step) % 16 == 0 && sizeof(TcStep) == 16,
+              "read as 16- and 8-byte vectors");
 // every lane's answer, so that a warp gives up as one
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(FULL, mbar_wait(bar, parity));
 }
 
+// the decoding warps' barrier, and whether all of their threads said yes
+__device__ __forceinline__ bool all_of_128(bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred.aligned q, 1, 128, p;\n"
+      " selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)yes)
+      : "memory");
+  return r != 0;
+}
+
 // One pair of row tiles of one sequence.
 struct TcWork {
   SeqSpan s;
-  int rows, r0, first;  // row r is token first + r / group
-  int lo, steps;        // keys [lo, lo + 128 steps) cover what the rows see; lo a multiple of 16
-  int hi;               // no row sees hi or later
+  int b, rows, r0, first;  // row r is token first + r / group
+  int lo, steps;           // keys [lo, lo + 128 steps) cover what the rows see; lo a multiple of 16
+  int hi;                  // no row sees hi or later
 };
-__device__ __forceinline__ TcWork tc_work(const AttendArgs& a, int b, int group, bool* bad) {
+
+// Calls f(work) for each of this block's pairs of tiles until it returns false.
+// The last rows of a sequence see most: they go first.
+template <class F>
+__device__ __forceinline__ void tc_each(const AttendArgs& a, TcShared& sh, bool* bad, F f) {
+  const int group = a.q_heads / a.cache.kv_heads;
   TcWork w;
-  w.s = seq_span(a.seq, b, a.cache.page_size, bad);
-  w.rows = w.s.q_len * group;
-  w.first = w.s.kv_len - w.s.q_len;
-  return w;
+  for (w.b = blockIdx.z; w.b < a.seq.num_seqs; w.b += gridDim.z) {
+    w.s = seq_span(a.seq, w.b, a.cache.page_size, bad);
+    w.rows = w.s.q_len * group;
+    w.first = w.s.kv_len - w.s.q_len;
+    const int tiles = (w.rows + TC_ROWS - 1) / TC_ROWS;
+    for (int rt = (int)gridDim.x - 1 - (int)blockIdx.x; rt < tiles; rt += gridDim.x) {
+      w.r0 = rt * TC_ROWS;
+      const int pos0 = w.first + w.r0 / group;
+      w.hi = w.first + (min(w.r0 + TC_ROWS, w.rows) - 1) / group + 1;
+      w.lo = (a.window > 0 ? max(0, pos0 - a.window + 1) : 0) & ~15;
+      w.steps = w.hi > w.lo ? (w.hi - w.lo + TC_KV - 1) / TC_KV : 0;
+      if (!f(w)) {  // a wait gave up
+        sh.fail = 1;
+        return;
+      }
+    }
+  }
 }
-__device__ __forceinline__ void tc_range(TcWork& w, int r0, int group, int window) {
-  w.r0 = r0;
-  const int pos0 = w.first + r0 / group;
-  w.hi = w.first + (min(r0 + TC_ROWS, w.rows) - 1) / group + 1;
-  w.lo = (window > 0 ? max(0, pos0 - window + 1) : 0) & ~15;
-  w.steps = w.hi > w.lo ? (w.hi - w.lo + TC_KV - 1) / TC_KV : 0;
+
+// ---- warps 0-7: one row per thread ----
+template <int D>
+__device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, unsigned char* sQ, bool* bad) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 2, r = threadIdx.x & 127;
+  const int kvh = blockIdx.y, group = a.q_heads / a.cache.kv_heads;
+  const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
+  const uint32_t tS = sh.tmem + i * 128 + lane_off, tO = sh.tmem + 256 + i * D + lane_off;
+  unsigned char* to_q = sQ + i * TcSmem<D>::Q + r * 128;
+  uint32_t kq = 0, items = 0;
+  tc_each(a, sh, bad, [&](const TcWork& w) {
+    const int row = w.r0 + i * 128 + r;
+    const bool live = row < w.rows;
+    const int64_t tok = w.s.row + row / group;
+    const int head = kvh * group + row % group;
+    float scl = 0.f;  // what a score is worth in units of log2, but for the keys' power of two
+    int eq = 0;
+    if (w.steps > 0) {
+      // the row of Q as f16, its largest value in [2^13, 2^14), K-major with the 128-byte swizzle
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q.p) + tok * a.q.token + head * a.q.head;
+      float top = 0.f;
+      bool fin = true;
+      if (live) {
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          float x[8];
+          load8_bf16(q + 8 * c, a.q.vec, x);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            top = fmaxf(top, fabsf(x[u]));
+            fin = fin && finite_f(x[u]);
+          }
+        }
+      }
+      eq = max(-126, min(126, 13 - ((int)(__float_as_uint(top) >> 23) - 127)));
+      const float up = fin ? pow2(eq) : 0.f;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        float x[8] = {};
+        if (live) load8_bf16(q + 8 * c, a.q.vec, x);
+        uint32_t v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          v[u] = fin ? pack_f16(x[2 * u] * up, x[2 * u + 1] * up) : 0x7fff7fffu;  // a row that is not finite is NaN
+        *reinterpret_cast<uint4*>(to_q + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) =
+            make_uint4(v[0], v[1], v[2], v[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full);
+      scl = a.scale * 1.4426950408889634f;
+    }
+    const int pos = w.first + row / group;
+    const int pos_first = w.first + (w.r0 + i * 128) / group;  // of this tile's rows
+    const int pos_last = w.first + (min(w.r0 + i * 128 + 128, w.rows) - 1) / group;
+    float ref = 0.f, lift = -INFINITY, l = 0.f;
+    int ev0 = 0;
+    for (int j = 0; j < w.steps; ++j) {
+      if (!warp_wait(&sh.s_full[i], (kq + j) & 1u)) return false;
+      tc5_fence_after();
+      float s[TC_KV];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc5_ld32(tS + 32 * c, reinterpret_cast<uint32_t*>(s) + 32 * c);
+      const TcStep& st = sh.step[(kq + j) & 3u];
+      const uint2 holes = *reinterpret_cast<const uint2*>(st.hole);
+      if (j == 0) ev0 = st.ev;
+      const int ev = st.ev - ev0;
+      float f = scl * exp2f((float)(st.ek - eq));
+      const int k0 = w.lo + j * TC_KV;
+      const bool partial =
+          k0 + TC_KV - 1 > pos_first || (a.window > 0 && k0 <= pos_last - a.window) || (holes.x | holes.y) != 0;
+      tc5_ld_wait();
+      if (partial) {
+        const int from = a.window > 0 ? pos - a.window + 1 - k0 : 0, to = pos - k0;  // columns [from, to] are seen
+        const float none = f < 0.f ? INFINITY : -INFINITY;
+#pragma unroll
+        for (int u = 0; u < TC_KV; ++u)
+          if (u > to || u < from || (((u < 64 ? holes.x : holes.y) >> (8 * ((u >> 4) & 3))) & 1u)) s[u] = none;
+      }
+      if (f == 0.f) {  // a scale of zero: not to the unseen, where it would be 0 * inf
+        f = 1.f;
+#pragma unroll
+        for (int u = 0; u < TC_KV; ++u) s[u] = s[u] == -INFINITY ? s[u] : s[u] * 0.f;
+      }
+      float top = -INFINITY;
+      if (f >= 0.f) {
+#pragma unroll
+        for (int u = 0; u < TC_KV; u += 2) top = fmaxf(top, fmaxf(s[u], s[u + 1]));
+        top = top == -INFINITY ? top : fmaf(top, f, (float)ev);
+      } else {
+        float low = INFINITY;
+#pragma unroll
+        for (int u = 0; u < TC_KV; u += 2) low = fminf(low, fminf(s[u], s[u + 1]));
+        top = low == INFINITY ? top : fmaf(low, f, (float)ev);
+      }
+      if (__any_sync(FULL, top > lift)) {
+        const bool first = lift == -INFINITY;
+        const float now = top > lift - 8.f || first ? top : ref;
+        float keep = 1.f;
+        if (now != -INFINITY) {
+          keep = first ? 1.f : exp2_fast(ref - now);
+          ref = now;
+          lift = now + 8.f;
+        }
+        l *= keep;
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t v[16];
+            tc5_ld16_async(tO + 16 * c, v);
+            tc5_ld_wait();
+#pragma unroll
+            for (int u = 0; u < 16; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * keep);
+            tc5_st16(tO + 16 * c, v);
+          }
+        }
+      }
+      const uint64_t f2 = pair(f, f), less2 = pair((float)ev - ref, (float)ev - ref);
+      uint64_t sum2 = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          float x, y;
+          unpair(fma2(pair(s[32 * c + 2 * u], s[32 * c + 2 * u + 1]), f2, less2), x, y);
+          x = exp2_fast(x);
+          y = exp2_fast(y);
+          sum2 = add2(sum2, pair(x, y));
+          pk[u] = pack_f16(x, y);
+        }
+        tc5_st16(tS + 16 * c, pk);
+      }
+      float x, y;
+      unpair(sum2, x, y);
+      l = fmaf(x + y, exp2f((float)-ev), l);
+      tc5_st_wait();
+      tc5_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[i]);
+    }
+    if (w.steps > 0) {
+      if (!warp_wait(&sh.o_full[i], items & 1u)) return false;
+      tc5_fence_after();
+      ++items;
+    }
+    kq += (uint32_t)w.steps;
+    const float inv = l == 0.f ? 0.f : 1.f / l, up = exp2f((float)ev0);
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.p) + tok * a.out.token + head * a.out.head;
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t v[32];
+      if (w.steps > 0) {
+        tc5_ld32(tO + 32 * c, v);
+        tc5_ld_wait();
+      }
+      if (live) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : __uint_as_float(v[8 * u + e]) * inv * up;
+          store8_bf16(out + 32 * c + 8 * u, a.out.vec, y);
+        }
+      }
+    }
+    tc5_fence_before();  // the next rows' first product overwrites O
+    return true;
+  });
 }
+
+// ---- warps 8-11: keys and values ----
+template <int D>
+__device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, unsigned char* sK, unsigned char* sV,
+                                          bool* bad) {
+  constexpr int TB = kv4_tile_bytes(D), CODES = kv4_codes(D), KVB = TcSmem<D>::KV;
+  const int lane = threadIdx.x & 31, tid = threadIdx.x - 256, sub = tid & 15;
+  const int kvh = blockIdx.y;
+  const int ps = a.cache.page_size, tpp = a.cache.tiles_per_page;
+  uint32_t kq = 0;
+  int ev_before = 0;
+  bool alive = true;
+  tc_each(a, sh, bad, [&](const TcWork& w) {
+    const int32_t* table = a.seq.table + w.b * a.seq.table_ld;
+    uint4 kc[D / 32], vc[D / 32], vp[2];
+    uint2 kp;
+    bool hole;
+    auto page_of = [&](int j) {
+      const int n = w.lo + j * TC_KV + (tid & ~15);
+      return j < w.steps && n < w.hi ? table[n / ps] : -1;
+    };
+    auto fetch = [&](int j, int32_t page) {
+      const int n = w.lo + j * TC_KV + (tid & ~15);
+      hole = j < w.steps && n < w.hi && (page < 0 || page >= a.cache.num_pages);
+      if (hole) *bad = true;
+      if (hole || page < 0) {
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
+        vp[0] = vp[1] = make_uint4(0, 0, 0, 0);
+        kp = make_uint2(0, 0);
+        return;
+      }
+      const unsigned char* tile = kv4_tile(a.cache, TB, page, kvh, (n >> 4) % tpp);
+      const unsigned char* codes = tile + CODES;
+      const unsigned char* pr = tile + 2 * CODES;
+#pragma unroll
+      for (int u = 0; u < D / 32; ++u) {
+        if (D == 128) {
+          kc[u] = *reinterpret_cast<const uint4*>(tile + sub * 64 + u * 16);
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(tile + (sub & 7) * 64 + 2 * u * 16 + (sub >> 3) * 8);
+          const uint2 y = *reinterpret_cast<const uint2*>(tile + (sub & 7) * 64 + (2 * u + 1) * 16 + (sub >> 3) * 8);
+          kc[u] = make_uint4(x.x, x.y, y.x, y.y);
+        }
+        vc[u] = *reinterpret_cast<const uint4*>(codes + (sub + 16 * u) * 16);
+      }
+      kp = *reinterpret_cast<const uint2*>(pr + sub * 8);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) vp[h] = *reinterpret_cast<const uint4*>(pr + (8 * h + 2 * (sub & 3)) * 8);
+    };
+    int32_t next = page_of(1);
+    fetch(0, page_of(0));
+    for (int j = 0; j < w.steps; ++j) {
+      const uint32_t q = kq + j, st = q & 1u;
+      // ---- the step's powers of two: the largest |K| and |V| to [2^13, 2^14) ----
+      const uint32_t rk = __reduce_max_sync(FULL, reach(kp.x)), rv = __reduce_max_sync(FULL, reach(kp.y));
+      if (lane == 0) {
+        sh.reach[st][0][tid >> 5] = rk;
+        sh.reach[st][1][tid >> 5] = rv;
+      }
+      // one wait says that the ring's K stage and the step's slot are free; the four warps give up as one
+      if (q >= 2 && alive) alive = warp_wait(&sh.k_empty[st], (q / 2 - 1) & 1u);
+      if (alive && sub == 0) sh.step[q & 3u].hole[tid >> 4] = hole;
+      if (!all_of_128(alive)) return false;
+      const uint4 mk = *reinterpret_cast<const uint4*>(sh.reach[st][0]);
+      const uint4 mv = *reinterpret_cast<const uint4*>(sh.reach[st][1]);
+      const uint32_t tk = max(max(mk.x, mk.y), max(mk.z, mk.w)), tv = max(max(mv.x, mv.y), max(mv.z, mv.w));
+      const int ek = tk ? max(-126, (int)(tk >> 23) - 127 - 13) : 0;
+      const int ev = tv ? max(-126, (int)(tv >> 23) - 127 - 13) : ev_before;  // nothing but zeros: as it was
+      ev_before = ev;
+      if (tid == 0) {
+        sh.step[q & 3u].ek = ek;
+        sh.step[q & 3u].ev = ev;
+      }
+      const float fk = pow2(-ek), fv = pow2(-ev);
+      {  // ---- K: this thread's token, D contiguous ----
+        // a vector that is not finite: the key becomes NaN for whoever sees it, the value zero, since a
+        // product with it reaches rows that do not
+        const bool nan = bf_high(kp.x) != bf_high(kp.x) || bf_high(kp.y) != bf_high(kp.y);
+        const uint32_t s2 = nan ? 0u : twice_f16(bf_low(kp.x) * fk);
+        const uint32_t m2 = nan ? 0x7fff7fffu : twice_f16(bf_high(kp.x) * fk);
+        unsigned char* to = sK + st * KVB + tid * 128;
+#pragma unroll
+        for (int u = 0; u < D / 8; ++u) {
+          const uint4& k = kc[u >> 2];
+          const uint32_t word = (u & 3) == 0 ? k.x : (u & 3) == 1 ? k.y : (u & 3) == 2 ? k.z : k.w;
+          *reinterpret_cast<uint4*>(to + (u >> 3) * 16384 + (((u & 7) ^ (tid & 7)) << 4)) = values8(word, s2, m2);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.k_full[st]);
+      // ---- V: 16-byte chunks of the codes; two tokens each ----
+      if (q >= 2 && !warp_wait(&sh.v_empty[st], (q / 2 - 1) & 1u)) {
+        alive = false;
+        continue;
+      }
+      uint32_t s2[2][2], m2[2][2];  // of tokens 2t + o of half h
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const uint32_t k = o ? vp[h].z : vp[h].x, v = o ? vp[h].w : vp[h].y;
+          const bool nan = bf_high(k) != bf_high(k) || bf_high(v) != bf_high(v);
+          s2[h][o] = nan ? 0u : twice_f16(bf_low(v) * fv);
+          m2[h][o] = nan ? 0u : twice_f16(bf_high(v) * fv);
+        }
+#pragma unroll
+      for (int u = 0; u < D / 32; ++u) {
+        const int chunk = sub + 16 * u, t = chunk & 3;
+        const uint32_t words[4] = {vc[u].x, vc[u].y, vc[u].z, vc[u].w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          // D = 128: chunk (h, g, t) = [even w0, even w1, odd w0, odd w1]; D = 64: (g, t) = [h0 even, h0 odd, h1 even, h1 odd]
+          const int h = D == 128 ? u >> 1 : x >> 1, o = D == 128 ? x >> 1 : x & 1;
+          const int g = D == 128 ? (chunk >> 2) & 7 : chunk >> 2;
+          const int d8 = D == 128 ? 2 * g + (x & 1) : g;  // which 8 dims
+          const int tok = (tid & ~15) + 8 * h + 2 * t + o;
+          *reinterpret_cast<uint4*>(sV + st * KVB + (d8 >> 3) * 16384 + tok * 128 + (((d8 & 7) ^ (tok & 7)) << 4)) =
+              values8(words[x], s2[h][o], m2[h][o]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.v_full[st]);
+      fetch(j + 1, next);
+      next = page_of(j + 2);
+    }
+    kq += (uint32_t)w.steps;
+    return true;
+  });
+}
+
+// ---- one thread: the products ----
+template <int D>
+__device__ __forceinline__ void tc_products(const AttendArgs& a, TcShared& sh, unsigned char* sQ, unsigned char* sK,
+                                            unsigned char* sV, bool* bad) {
+  constexpr int QB = TcSmem<D>::Q, KVB = TcSmem<D>::KV;
+  constexpr uint32_t bf16_ab = (1u << 7) | (1u << 10);
+  const uint32_t tmem = sh.tmem, id_s = f16_idesc(128, TC_KV) & ~bf16_ab, id_o = (f16_idesc(128, D) & ~bf16_ab) | (1u << 16);
+  uint32_t kq = 0, items = 0;
+  auto scores = [&](int i, uint32_t st) {
+    const uint64_t dq = sw128_desc(smem_u32(sQ + i * QB)), dk = sw128_desc(smem_u32(sK + st * KVB));
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      const uint64_t off = (uint64_t)((k >> 2) * 1024 + (k & 3) * 2);
+      tc5_mma(tmem + i * 128, dq + off, dk + off, id_s, k != 0);
+    }
+    tc5_commit(&sh.s_full[i]);
+  };
+  tc_each(a, sh, bad, [&](const TcWork& w) {
+    if (w.steps == 0) return true;
+    if (!mbar_wait(&sh.q_full, items & 1u) || !mbar_wait(&sh.k_full[kq & 1u], (kq / 2) & 1u)) return false;
+    tc5_fence_after();
+    scores(0, kq & 1u);
+    scores(1, kq & 1u);
+    tc5_commit(&sh.k_empty[kq & 1u]);
+    for (int j = 0; j < w.steps; ++j) {
+      const uint32_t q = kq + j, st = q & 1u, nx = st ^ 1u;
+      if (!mbar_wait(&sh.v_full[st], (q / 2) & 1u)) return false;
+      const uint64_t dv = sw128_mn_desc(smem_u32(sV + st * KVB), 16384);
+      for (int i = 0; i < 2; ++i) {
+        if (!mbar_wait(&sh.p_full[i], q & 1u)) return false;
+        tc5_fence_after();
+#pragma unroll
+        for (int k = 0; k < TC_KV / 16; ++k)
+          tc5_mma_ta(tmem + 256 + i * D, tmem + i * 128 + 8 * k, dv + (uint64_t)(k * 128), id_o, (j | k) != 0);
+        if (i == 1) tc5_commit(&sh.v_empty[st]);
+        if (j + 1 < w.steps) {
+          if (i == 0 && !mbar_wait(&sh.k_full[nx], ((q + 1) / 2) & 1u)) return false;
+          tc5_fence_after();
+          scores(i, nx);
+          if (i == 1) tc5_commit(&sh.k_empty[nx]);
+        } else {
+          tc5_commit(&sh.o_full[i]);
+        }
+      }
+    }
+    kq += (uint32_t)w.steps;
+    ++items;
+    return true;
+  });
+  // nothing of the tensor core's may be pending when its memory is freed
+  tc5_commit(&sh.done);
+  mbar_wait(&sh.done, 0);
+}
+
+// Registers: 512 threads start with 128 each; 128 (2 x 184 + 96 + 48) = 512 x 128.
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void less_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
 
 template <int D>
 __global__ void __launch_bounds__(TC_NT, 1) attend_tc_kernel(AttendArgs a) {
   extern __shared__ unsigned char tc_dyn[];
-  __shared__ TcBars bars;
-  __shared__ uint32_t tmem_s;
-  __shared__ int fail;
-  __shared__ __align__(8) unsigned char no_page[4][8];  // by step & 3: the 16-token tiles whose page does not exist
-  constexpr int TB = kv4_tile_bytes(D), CODES = kv4_codes(D);
-  constexpr int QB = TcSmem<D>::Q, KVB = TcSmem<D>::KV;
+  __shared__ __align__(16) TcShared sh;
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tc_dyn) + 1023) & ~uintptr_t(1023));
   unsigned char* sQ = sm;
-  unsigned char* sK = sm + 2 * QB;
-  unsigned char* sV = sK + 2 * KVB;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = blockIdx.y, group = a.q_heads / a.cache.kv_heads;
+  unsigned char* sK = sm + 2 * TcSmem<D>::Q;
+  unsigned char* sV = sK + 2 * TcSmem<D>::KV;
+  const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
-    mbar_init(&bars.q_full, 8);
+    mbar_init(&sh.q_full, 8);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars.k_full[i], 4);
-      mbar_init(&bars.v_full[i], 4);
-      mbar_init(&bars.k_empty[i], 1);
-      mbar_init(&bars.v_empty[i], 1);
-      mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 4);
-      mbar_init(&bars.o_full[i], 1);
+      mbar_init(&sh.k_full[i], 4);
+      mbar_init(&sh.v_full[i], 4);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.o_full[i], 1);
     }
-    mbar_init(&bars.done, 1);
-    fail = 0;
+    mbar_init(&sh.done, 1);
+    sh.fail = 0;
     fence_mbar_init();
   }
-  if (warp == 12) tc5_alloc(&tmem_s, 512);
+  if (warp == 12) tc5_alloc(&sh.tmem, 512);
   tc5_fence_before();
   __syncthreads();
   tc5_fence_after();
-  const uint32_t tmem = tmem_s;
-  bool bad = false, lost = false;  // lost: a wait gave up, this role ends
-  uint32_t kq = 0, items = 0;      // steps and pairs of tiles done
-
-  for (int b = blockIdx.z; b < a.seq.num_seqs && !lost; b += gridDim.z) {
-    TcWork w = tc_work(a, b, group, &bad);
-    const int tiles = (w.rows + TC_ROWS - 1) / TC_ROWS;
-    // the last rows see most: they go first
-    for (int rt = (int)gridDim.x - 1 - (int)blockIdx.x; rt < tiles && !lost; rt += gridDim.x) {
-      tc_range(w, rt * TC_ROWS, group, a.window);
-
-      if (warp < 8) {
-        // ------------------------------------------------ softmax: one row per thread
-        const int i = warp >> 2, r = threadIdx.x & 127, row = w.r0 + i * 128 + r;
-        const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
-        const uint32_t tS = tmem + i * 128 + lane_off, tO = tmem + 256 + i * D + lane_off;
-        const bool live = row < w.rows;
-        const int64_t tok = w.s.row + row / group;
-        const int head = kvh * group + row % group;
-        if (w.steps > 0) {  // the row of Q, K-major with the 128-byte swizzle; a negative scale goes into its sign
-          const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-          const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q.p) + tok * a.q.token + head * a.q.head;
-          unsigned char* to = sQ + i * QB + r * 128;
-#pragma unroll 4
-          for (int c = 0; c < D / 8; ++c) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (live) {
-              if (a.q.vec) {
-                v = reinterpret_cast<const uint4*>(q)[c];
-              } else {
-                const unsigned short* u = reinterpret_cast<const unsigned short*>(q) + 8 * c;
-                v = make_uint4(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16,
-                               u[6] | (uint32_t)u[7] << 16);
-              }
-              v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-            }
-            *reinterpret_cast<uint4*>(to + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) = v;
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.q_full);
-        }
-        const float scl = fabsf(a.scale) * 1.4426950408889634f;
-        const int pos = w.first + row / group;
-        const int pos_first = w.first + (w.r0 + i * 128) / group;                         // of this tile's rows
-        const int pos_last = w.first + (min(w.r0 + i * 128 + 128, max(w.rows, 1)) - 1) / group;
-        float ref = 0.f, lift = -INFINITY, l0 = 0.f, l1 = 0.f;
-        for (int j = 0; j < w.steps; ++j) {
-          if (!warp_wait(&bars.s_full[i], (kq + j) & 1u)) {
-            lost = true;
-            break;
-          }
-          tc5_fence_after();
-          const int k0 = w.lo + j * TC_KV;
-          const int from = a.window > 0 ? pos - a.window + 1 - k0 : 0, to = pos - k0;  // columns [from, to] are seen
-          const uint2 none2 = *reinterpret_cast<const uint2*>(no_page[(kq + j) & 3u]);
-          const bool holes = (none2.x | none2.y) != 0;
-          const bool partial = k0 + TC_KV - 1 > pos_first || (a.window > 0 && k0 <= pos_last - a.window) || holes;
-          auto unseen = [&](int col) {
-            return col > to || col < from || (holes && no_page[(kq + j) & 3u][col >> 4]);
-          };
-          float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tc5_ld32(tS + 32 * c, v);
-            tc5_ld_wait();
-            if (partial) {
-#pragma unroll
-              for (int u = 0; u < 32; ++u)
-                if (unseen(32 * c + u)) v[u] = 0xff800000u;
-            }
-#pragma unroll
-            for (int u = 0; u < 32; ++u) top = fmaxf(top, __uint_as_float(v[u]));
-          }
-          const float x = top == -INFINITY ? -INFINITY : top * scl;
-          if (__any_sync(FULL, x > lift)) {
-            const bool none = lift == -INFINITY;
-            const float now = x > lift - 8.f || none ? x : ref;
-            float keep = 1.f;
-            if (now != -INFINITY) {
-              keep = none ? 1.f : exp2_fast(ref - now);
-              ref = now;
-              lift = now + 8.f;
-            }
-            l0 *= keep;
-            l1 *= keep;
-            if (j > 0) {
-#pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t v[32];
-                tc5_ld32(tO + 32 * c, v);
-                tc5_ld_wait();
-#pragma unroll
-                for (int u = 0; u < 32; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * keep);
-                tc5_st16(tO + 32 * c, v);
-                tc5_st16(tO + 32 * c + 16, v + 16);
-              }
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32], pk[16];
-            tc5_ld32(tS + 32 * c, v);
-            tc5_ld_wait();
-            if (partial) {
-#pragma unroll
-              for (int u = 0; u < 32; ++u)
-                if (unseen(32 * c + u)) v[u] = 0xff800000u;
-            }
-#pragma unroll
-            for (int u = 0; u < 16; ++u) {
-              const float y0 = exp2_fast(fmaf(__uint_as_float(v[2 * u]), scl, -ref));
-              const float y1 = exp2_fast(fmaf(__uint_as_float(v[2 * u + 1]), scl, -ref));
-              l0 += y0;
-              l1 += y1;
-              pk[u] = pack_bf16(y0, y1);
-            }
-            tc5_st16(tS + 16 * c, pk);
-          }
-          tc5_st_wait();
-          tc5_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.p_full[i]);
-        }
-        if (!lost && w.steps > 0) {
-          if (warp_wait(&bars.o_full[i], items & 1u)) tc5_fence_after();
-          else lost = true;
-        }
-        if (!lost) {
-          const float l = l0 + l1, inv = l == 0.f ? 0.f : 1.f / l;
-          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.p) + tok * a.out.token + head * a.out.head;
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t v[32];
-            if (w.steps > 0) {
-              tc5_ld32(tO + 32 * c, v);
-              tc5_ld_wait();
-            } else {
-#pragma unroll
-              for (int u = 0; u < 32; ++u) v[u] = 0u;
-            }
-            if (live) {
-              float y[32];
-#pragma unroll
-              for (int u = 0; u < 32; ++u) y[u] = l == 0.f ? 0.f : __uint_as_float(v[u]) * inv;
-#pragma unroll
-              for (int u = 0; u < 4; ++u) store8_bf16(out + 32 * c + 8 * u, a.out.vec, y + 8 * u);
-            }
-          }
-          tc5_fence_before();  // the next rows' first product overwrites O
-        }
-      } else if (warp < 12) {
-        // ------------------------------------------------ keys and values
-        const int tid = threadIdx.x - 256, sub = tid & 15;
-        const int32_t* table = a.seq.table + b * a.seq.table_ld;
-        const int ps = a.cache.page_size, tpp = a.cache.tiles_per_page;
-        uint4 kc[4], vc[4], vp[2];
-        uint2 kp;
-        bool hole = false;
-        auto page_of = [&](int j) {
-          const int n = w.lo + j * TC_KV + (tid & ~15);
-          return j < w.steps && n < w.hi ? table[n / ps] : -1;
-        };
-        auto fetch = [&](int j, int32_t page) {
-          const int n = w.lo + j * TC_KV + (tid & ~15);
-          if (j < w.steps && n < w.hi && (page < 0 || page >= a.cache.num_pages)) {
-            bad = true;
-            page = -1;
-          }
-          if (page < 0) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
-            vp[0] = vp[1] = make_uint4(0, 0, 0, 0);
-            kp = make_uint2(0, 0);
-            hole = j < w.steps && n < w.hi;
-            return;
-          }
-          hole = false;
-          const unsigned char* tile = kv4_tile(a.cache, TB, page, kvh, (n >> 4) % tpp);
-          const unsigned char* codes = tile + CODES;
-          const unsigned char* pr = tile + 2 * CODES;
-          if (D == 128) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              kc[u] = *reinterpret_cast<const uint4*>(tile + sub * 64 + u * 16);
-              vc[u] = *reinterpret_cast<const uint4*>(codes + (sub + 16 * u) * 16);
-            }
-          } else {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const uint2 x = *reinterpret_cast<const uint2*>(tile + (sub & 7) * 64 + u * 16 + (sub >> 3) * 8);
-              kc[u] = make_uint4(x.x, x.y, 0, 0);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) vc[u] = *reinterpret_cast<const uint4*>(codes + (sub + 16 * u) * 16);
-          }
-          kp = *reinterpret_cast<const uint2*>(pr + sub * 8);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) vp[h] = *reinterpret_cast<const uint4*>(pr + (8 * h + 2 * (sub & 3)) * 8);
-        };
-        int32_t next = page_of(1);
-        fetch(0, page_of(0));
-        for (int j = 0; j < w.steps; ++j) {
-          const uint32_t q = kq + j, st = q & 1u;
-          // ---- K: this thread's token, D contiguous ----
-          if (q >= 2 && !warp_wait(&bars.k_empty[st], (q / 2 - 1) & 1u)) {
-            lost = true;
-            break;
-          }
-          // four slots: a step's is written again when the step three on has its scores, after this one's softmax
-          if (sub == 0) no_page[q & 3u][tid >> 4] = hole;
-          {
-            // a value that is not finite: the key becomes NaN for whoever sees it, the value zero, since a
-            // product with it reaches rows that do not
-            const bool nan = nan_low(kp.x) || nan_low(kp.y);
-            const uint32_t s = nan ? 0u : kp.x & 0xffffu, m = nan ? 0x7fffu : kp.x >> 16;
-            const uint32_t s2 = s | s << 16, m2 = m | m << 16;
-            unsigned char* to = sK + st * KVB + tid * 128;
-#pragma unroll
-            for (int u = 0; u < D / 8; ++u) {
-              const uint32_t word = D == 128 ? (&kc[u >> 2].x)[u & 3] : (&kc[u >> 1].x)[u & 1];
-              *reinterpret_cast<uint4*>(to + (u >> 3) * 16384 + (((u & 7) ^ (tid & 7)) << 4)) = values8(word, s2, m2);
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.k_full[st]);
-          // ---- V: 16-byte chunks of the codes; two tokens each ----
-          if (q >= 2 && !warp_wait(&bars.v_empty[st], (q / 2 - 1) & 1u)) {
-            lost = true;
-            break;
-          }
-#pragma unroll
-          for (int u = 0; u < D / 32; ++u) {
-            const int chunk = sub + 16 * u, t = chunk & 3;
-            const uint32_t words[4] = {vc[u].x, vc[u].y, vc[u].z, vc[u].w};
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              // D = 128: chunk (h, g, t) = [even w0, even w1, odd w0, odd w1]; D = 64: (g, t) = [h0 e, h0 o, h1 e, h1 o]
-              const int h = D == 128 ? u >> 1 : x >> 1, o = D == 128 ? x >> 1 : x & 1;
-              const int g = D == 128 ? (chunk >> 2) & 7 : chunk >> 2;
-              const int d8 = D == 128 ? 2 * g + (x & 1) : g;  // which 8 dims
-              const uint32_t k2 = o ? vp[h].z : vp[h].x, v2 = o ? vp[h].w : vp[h].y;
-              const bool nan = nan_low(k2) || nan_low(v2);
-              const uint32_t s = nan ? 0u : v2 & 0xffffu, m = nan ? 0u : v2 >> 16;
-              const int tok = (tid & ~15) + 8 * h + 2 * t + o;
-              *reinterpret_cast<uint4*>(sV + st * KVB + (d8 >> 3) * 16384 + tok * 128 + (((d8 & 7) ^ (tok & 7)) << 4)) =
-                  values8(words[x], s | s << 16, m | m << 16);
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.v_full[st]);
-          fetch(j + 1, next);
-          next = page_of(j + 2);
-        }
-      } else if (lane == 0 && w.steps > 0) {
-        // ------------------------------------------------ the products
-        const uint32_t id_s = f16_idesc(128, TC_KV), id_o = f16_idesc(128, D) | (1u << 16);
-        auto scores = [&](int i, uint32_t st) {
-          const uint64_t dq = sw128_desc(smem_u32(sQ + i * QB)), dk = sw128_desc(smem_u32(sK + st * KVB));
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = (uint64_t)((k >> 2) * 1024 + (k & 3) * 2);
-            tc5_mma(tmem + i * 128, dq + off, dk + off, id_s, k != 0);
-          }
-          tc5_commit(&bars.s_full[i]);
-        };
-        lost = !mbar_wait(&bars.q_full, items & 1u) || !mbar_wait(&bars.k_full[kq & 1u], (kq / 2) & 1u);
-        if (!lost) {
-          tc5_fence_after();
-          scores(0, kq & 1u);
-          scores(1, kq & 1u);
-          tc5_commit(&bars.k_empty[kq & 1u]);
-        }
-        for (int j = 0; j < w.steps && !lost; ++j) {
-          const uint32_t q = kq + j, st = q & 1u, nx = st ^ 1u;
-          if (!mbar_wait(&bars.v_full[st], (q / 2) & 1u)) {
-            lost = true;
-            break;
-          }
-          for (int i = 0; i < 2; ++i) {
-            if (!mbar_wait(&bars.p_full[i], q & 1u)) {
-              lost = true;
-              break;
-            }
-            tc5_fence_after();
-            const uint64_t dv = sw128_mn_desc(smem_u32(sV + st * KVB), 16384);
-#pragma unroll
-            for (int k = 0; k < TC_KV / 16; ++k)
-              tc5_mma_ta(tmem + 256 + i * D, tmem + i * 128 + 8 * k, dv + (uint64_t)(k * 128), id_o, (j | k) != 0);
-            if (i == 1) tc5_commit(&bars.v_empty[st]);
-            if (j + 1 < w.steps) {
-              if (i == 0 && !mbar_wait(&bars.k_full[nx], ((q + 1) / 2) & 1u)) {
-                lost = true;
-                break;
-              }
-              tc5_fence_after();
-              scores(i, nx);
-              if (i == 1) tc5_commit(&bars.k_empty[nx]);
-            } else {
-              tc5_commit(&bars.o_full[i]);
-            }
-          }
-        }
-      }
-      if (lost) atomicExch(&fail, 1);
-      kq += (uint32_t)w.steps;
-      if (w.steps > 0) ++items;
-    }
+  bool bad = false;
+  if (warp < 8) {
+    more_registers<184>();
+    tc_softmax<D>(a, sh, sQ, &bad);
+  } else if (warp < 12) {
+    less_registers<96>();
+    tc_decode<D>(a, sh, sK, sV, &bad);
+  } else {
+    less_registers<48>();
+    if (threadIdx.x == 12 * 32) tc_products<D>(a, sh, sQ, sK, sV, &bad);
   }
-  if (warp == 12 && lane == 0) {  // nothing of the tensor core's may be pending when its memory is freed
-    tc5_commit(&bars.done);
-    mbar_wait(&bars.done, 0);
-  }
+  if (bad) atomicOr(a.err, DERR_BOUNDS);
   tc5_fence_before();
   __syncthreads();
-  if (fail && threadIdx.x == 0) atomicOr(a.err, DERR_TIMEOUT);
-  if (bad) atomicOr(a.err, DERR_BOUNDS);
-  if (warp == 12) tc5_dealloc(tmem, 512);
+  if (sh.fail && threadIdx.x == 0) atomicOr(a.err, DERR_TIMEOUT);
+  if (warp == 12) tc5_dealloc(sh.tmem, 512);
 }
 
 }  // namespace
