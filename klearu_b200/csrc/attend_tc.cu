@@ -3,8 +3,8 @@
 //
 // One block takes 256 rows (token, query head) of one key head as two tiles of
 // 128, so that one tile multiplies while the other takes its softmax:
-//  * warps 0-3 and 4-7: softmax of tile 0 and 1, one row per thread, its 128
-//    scores in registers; P goes back to tensor memory as f16, over the scores
+//  * warps 0-3 and 4-7: softmax of tile 0 and 1, one row per thread, 64
+//    scores in registers at a time; P goes back to tensor memory as f16, over the scores
 //    that it came from; O is rescaled in place only when a row's maximum has
 //    risen by more than 2^8;
 //  * warps 8-11: the next 128 keys and values, codes read from global memory
@@ -23,6 +23,8 @@
 //
 // Per 128 keys and 256 rows at D = 128 the tensor cores need 2048 cycles and
 // the 32768 exponentials as many of the special function units.
+#include <cuda_fp16.h>
+
 #include <cstddef>
 
 #include "attend.cuh"
@@ -115,6 +117,11 @@ __device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
@@ -229,7 +236,8 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
         }
       }
       eq = max(-126, min(126, 13 - ((int)(__float_as_uint(top) >> 23) - 127)));
-      const float up = fin ? pow2(eq) : 0.f;
+      // the scale's sign goes into q, and a scale of zero makes it zero, so that a score's factor is positive
+      const float up = a.scale == 0.f ? 0.f : a.scale < 0.f ? -pow2(eq) : pow2(eq);
 #pragma unroll 4
       for (int c = 0; c < D / 8; ++c) {
         float x[8] = {};
@@ -244,7 +252,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
-      scl = a.scale * 1.4426950408889634f;
+      scl = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
     }
     const int pos = w.first + row / group;
     const int pos_first = w.first + (w.r0 + i * 128) / group;  // of this tile's rows
@@ -254,82 +262,94 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
     for (int j = 0; j < w.steps; ++j) {
       if (!warp_wait(&sh.s_full[i], (kq + j) & 1u)) return false;
       tc5_fence_after();
-      float s[TC_KV];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tc5_ld32(tS + 32 * c, reinterpret_cast<uint32_t*>(s) + 32 * c);
       const TcStep& st = sh.step[(kq + j) & 3u];
       const uint2 holes = *reinterpret_cast<const uint2*>(st.hole);
       if (j == 0) ev0 = st.ev;
-      const int ev = st.ev - ev0;
-      float f = scl * exp2f((float)(st.ek - eq));
+      const float ev = (float)(st.ev - ev0);
+      const float f = fmaxf(scl * exp2f((float)(st.ek - eq)), 1.2e-38f);  // never 0, which an unseen score's -inf would make NaN
       const int k0 = w.lo + j * TC_KV;
-      const bool partial =
-          k0 + TC_KV - 1 > pos_first || (a.window > 0 && k0 <= pos_last - a.window) || (holes.x | holes.y) != 0;
-      tc5_ld_wait();
-      if (partial) {
-        const int from = a.window > 0 ? pos - a.window + 1 - k0 : 0, to = pos - k0;  // columns [from, to] are seen
-        const float none = f < 0.f ? INFINITY : -INFINITY;
-#pragma unroll
-        for (int u = 0; u < TC_KV; ++u)
-          if (u > to || u < from || (((u < 64 ? holes.x : holes.y) >> (8 * ((u >> 4) & 3))) & 1u)) s[u] = none;
-      }
-      if (f == 0.f) {  // a scale of zero: not to the unseen, where it would be 0 * inf
-        f = 1.f;
-#pragma unroll
-        for (int u = 0; u < TC_KV; ++u) s[u] = s[u] == -INFINITY ? s[u] : s[u] * 0.f;
-      }
-      float top = -INFINITY;
-      if (f >= 0.f) {
-#pragma unroll
-        for (int u = 0; u < TC_KV; u += 2) top = fmaxf(top, fmaxf(s[u], s[u + 1]));
-        top = top == -INFINITY ? top : fmaf(top, f, (float)ev);
-      } else {
-        float low = INFINITY;
-#pragma unroll
-        for (int u = 0; u < TC_KV; u += 2) low = fminf(low, fminf(s[u], s[u + 1]));
-        top = low == INFINITY ? top : fmaf(low, f, (float)ev);
-      }
-      if (__any_sync(FULL, top > lift)) {
-        const bool first = lift == -INFINITY;
-        const float now = top > lift - 8.f || first ? top : ref;
-        float keep = 1.f;
-        if (now != -INFINITY) {
-          keep = first ? 1.f : exp2_fast(ref - now);
-          ref = now;
-          lift = now + 8.f;
-        }
-        l *= keep;
-        if (j > 0) {
+      const bool partial = k0 + TC_KV - 1 > pos_first || (a.window > 0 && k0 <= pos_last - a.window);
+      uint64_t sum2 = 0;
 #pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
-            uint32_t v[16];
-            tc5_ld16_async(tO + 16 * c, v);
-            tc5_ld_wait();
+      for (int h = 0; h < 2; ++h) {  // 64 scores at a time, which fit the registers
+        float s[64];
+        tc5_ld32(tS + 64 * h, reinterpret_cast<uint32_t*>(s));
+        tc5_ld32(tS + 64 * h + 32, reinterpret_cast<uint32_t*>(s) + 32);
+        tc5_ld_wait();
+        if (partial) {
+          const int to = pos - k0, from = a.window > 0 ? max(0, to - a.window + 1) : 0;  // columns [from, to] are seen
+          const unsigned span = to >= from ? (unsigned)(to - from) : 0u, at = to >= from ? (unsigned)from : 0x40000000u;
 #pragma unroll
-            for (int u = 0; u < 16; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * keep);
-            tc5_st16(tO + 16 * c, v);
+          for (int u = 0; u < 64; ++u)
+            if ((unsigned)(64 * h + u) - at > span) s[u] = -INFINITY;
+        }
+        const uint32_t hole4 = h ? holes.y : holes.x;
+        if (hole4) {
+#pragma unroll
+          for (int u = 0; u < 64; ++u)
+            if (hole4 >> (8 * (u >> 4)) & 1u) s[u] = -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 64; u += 2) top = fmaxf(top, fmaxf(s[u], s[u + 1]));
+        if (top != -INFINITY) top = fmaf(top, f, ev);
+        if (__any_sync(FULL, top > lift)) {
+          const bool first = lift == -INFINITY;
+          const float now = top > lift - 8.f || first ? top : ref;
+          float keep = 1.f;
+          if (now != -INFINITY) {
+            keep = first ? 1.f : exp2_fast(ref - now);
+            ref = now;
+            lift = now + 8.f;
+          }
+          l *= keep;
+          sum2 = mul2(sum2, pair(keep, keep));
+          if (h == 1) {  // the step's first probabilities
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+              uint32_t v[16];
+              tc5_ld16_async(tS + 16 * c, v);
+              tc5_ld_wait();
+#pragma unroll
+              for (int u = 0; u < 16; ++u) {
+                const __half2 p = *reinterpret_cast<__half2*>(&v[u]);
+                v[u] = pack_f16(__low2float(p) * keep, __high2float(p) * keep);
+              }
+              tc5_st16(tS + 16 * c, v);
+            }
+          }
+          if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t v[16];
+              tc5_ld16_async(tO + 16 * c, v);
+              tc5_ld_wait();
+#pragma unroll
+              for (int u = 0; u < 16; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * keep);
+              tc5_st16(tO + 16 * c, v);
+            }
           }
         }
-      }
-      const uint64_t f2 = pair(f, f), less2 = pair((float)ev - ref, (float)ev - ref);
-      uint64_t sum2 = 0;
+        const uint64_t f2 = pair(f, f), less2 = pair(ev - ref, ev - ref);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-        for (int u = 0; u < 16; ++u) {
-          float x, y;
-          unpair(fma2(pair(s[32 * c + 2 * u], s[32 * c + 2 * u + 1]), f2, less2), x, y);
-          x = exp2_fast(x);
-          y = exp2_fast(y);
-          sum2 = add2(sum2, pair(x, y));
-          pk[u] = pack_f16(x, y);
+          for (int u = 0; u < 16; ++u) {
+            float x, y;
+            unpair(fma2(pair(s[32 * c + 2 * u], s[32 * c + 2 * u + 1]), f2, less2), x, y);
+            x = exp2_fast(x);
+            y = exp2_fast(y);
+            sum2 = add2(sum2, pair(x, y));
+            pk[u] = pack_f16(x, y);
+          }
+          tc5_st16(tS + 32 * h + 16 * c, pk);
         }
-        tc5_st16(tS + 16 * c, pk);
+        if (h == 0) tc5_st_wait();  // the second half may read them back
       }
       float x, y;
       unpair(sum2, x, y);
-      l = fmaf(x + y, exp2f((float)-ev), l);
+      l = fmaf(x + y, exp2f(-ev), l);
       tc5_st_wait();
       tc5_fence_before();
       __syncwarp();
@@ -380,25 +400,26 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
     const int32_t* table = a.seq.table + w.b * a.seq.table_ld;
     uint4 kc[D / 32], vc[D / 32], vp[2];
     uint2 kp;
-    bool hole;
     auto page_of = [&](int j) {
       const int n = w.lo + j * TC_KV + (tid & ~15);
       return j < w.steps && n < w.hi ? table[n / ps] : -1;
     };
-    auto fetch = [&](int j, int32_t page) {
+    auto is_hole = [&](int j, int32_t page) {
+      return j < w.steps && w.lo + j * TC_KV + (tid & ~15) < w.hi && (page < 0 || page >= a.cache.num_pages);
+    };
+    // this thread's 16-token tile of step j, null where there is none
+    auto tile_of = [&](int j, int32_t page) -> const unsigned char* {
       const int n = w.lo + j * TC_KV + (tid & ~15);
-      hole = j < w.steps && n < w.hi && (page < 0 || page >= a.cache.num_pages);
-      if (hole) *bad = true;
-      if (hole || page < 0) {
+      return page < 0 || page >= a.cache.num_pages ? nullptr : kv4_tile(a.cache, TB, page, kvh, (n >> 4) % tpp);
+    };
+    auto fetch_k = [&](const unsigned char* tile) {
+      kp = make_uint2(0, 0);
+      if (!tile) {
 #pragma unroll
-        for (int u = 0; u < D / 32; ++u) kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
-        vp[0] = vp[1] = make_uint4(0, 0, 0, 0);
-        kp = make_uint2(0, 0);
+        for (int u = 0; u < D / 32; ++u) kc[u] = make_uint4(0, 0, 0, 0);
         return;
       }
-      const unsigned char* tile = kv4_tile(a.cache, TB, page, kvh, (n >> 4) % tpp);
-      const unsigned char* codes = tile + CODES;
-      const unsigned char* pr = tile + 2 * CODES;
+      kp = *reinterpret_cast<const uint2*>(tile + 2 * CODES + sub * 8);
 #pragma unroll
       for (int u = 0; u < D / 32; ++u) {
         if (D == 128) {
@@ -408,14 +429,25 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
           const uint2 y = *reinterpret_cast<const uint2*>(tile + (sub & 7) * 64 + (2 * u + 1) * 16 + (sub >> 3) * 8);
           kc[u] = make_uint4(x.x, x.y, y.x, y.y);
         }
-        vc[u] = *reinterpret_cast<const uint4*>(codes + (sub + 16 * u) * 16);
       }
-      kp = *reinterpret_cast<const uint2*>(pr + sub * 8);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) vp[h] = *reinterpret_cast<const uint4*>(pr + (8 * h + 2 * (sub & 3)) * 8);
     };
-    int32_t next = page_of(1);
-    fetch(0, page_of(0));
+    auto fetch_v = [&](const unsigned char* tile) {
+      if (!tile) {
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) vc[u] = make_uint4(0, 0, 0, 0);
+        vp[0] = vp[1] = make_uint4(0, 0, 0, 0);
+        return;
+      }
+#pragma unroll
+      for (int u = 0; u < D / 32; ++u) vc[u] = *reinterpret_cast<const uint4*>(tile + CODES + (sub + 16 * u) * 16);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        vp[h] = *reinterpret_cast<const uint4*>(tile + 2 * CODES + (8 * h + 2 * (sub & 3)) * 8);
+    };
+    int32_t page = page_of(0), next = page_of(1);
+    const unsigned char* tile = tile_of(0, page);
+    fetch_k(tile);
+    fetch_v(tile);
     for (int j = 0; j < w.steps; ++j) {
       const uint32_t q = kq + j, st = q & 1u;
       // ---- the step's powers of two: the largest |K| and |V| to [2^13, 2^14) ----
@@ -426,6 +458,8 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
       }
       // one wait says that the ring's K stage and the step's slot are free; the four warps give up as one
       if (q >= 2 && alive) alive = warp_wait(&sh.k_empty[st], (q / 2 - 1) & 1u);
+      const bool hole = is_hole(j, page);
+      if (hole) *bad = true;
       if (alive && sub == 0) sh.step[q & 3u].hole[tid >> 4] = hole;
       if (!all_of_128(alive)) return false;
       const uint4 mk = *reinterpret_cast<const uint4*>(sh.reach[st][0]);
@@ -456,6 +490,11 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.k_full[st]);
+      // the next step's loads go out as soon as their registers are free
+      page = next;
+      tile = tile_of(j + 1, page);
+      fetch_k(tile);
+      next = page_of(j + 2);
       // ---- V: 16-byte chunks of the codes; two tokens each ----
       if (q >= 2 && !warp_wait(&sh.v_empty[st], (q / 2 - 1) & 1u)) {
         alive = false;
@@ -489,8 +528,7 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.v_full[st]);
-      fetch(j + 1, next);
-      next = page_of(j + 2);
+      fetch_v(tile);
     }
     kq += (uint32_t)w.steps;
     return true;
@@ -505,35 +543,41 @@ __device__ __forceinline__ void tc_products(const AttendArgs& a, TcShared& sh, u
   constexpr uint32_t bf16_ab = (1u << 7) | (1u << 10);
   const uint32_t tmem = sh.tmem, id_s = f16_idesc(128, TC_KV) & ~bf16_ab, id_o = (f16_idesc(128, D) & ~bf16_ab) | (1u << 16);
   uint32_t kq = 0, items = 0;
+  const uint64_t dq = sw128_desc(smem_u32(sQ)), dk = sw128_desc(smem_u32(sK));
+  const uint64_t dv = sw128_mn_desc(smem_u32(sV), 16384);
   auto scores = [&](int i, uint32_t st) {
-    const uint64_t dq = sw128_desc(smem_u32(sQ + i * QB)), dk = sw128_desc(smem_u32(sK + st * KVB));
+    const uint64_t q = dq + (uint64_t)(i * (QB >> 4)), k = dk + (uint64_t)(st * (KVB >> 4));
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      const uint64_t off = (uint64_t)((k >> 2) * 1024 + (k & 3) * 2);
-      tc5_mma(tmem + i * 128, dq + off, dk + off, id_s, k != 0);
-    }
+    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        tc5_mma(tmem + i * 128, q + (uint64_t)(h * 1024 + u * 2), k + (uint64_t)(h * 1024 + u * 2), id_s, (h | u) != 0);
     tc5_commit(&sh.s_full[i]);
   };
   tc_each(a, sh, bad, [&](const TcWork& w) {
-    if (w.steps == 0) return true;
+    const int steps = w.steps;
+    if (steps == 0) return true;
     if (!mbar_wait(&sh.q_full, items & 1u) || !mbar_wait(&sh.k_full[kq & 1u], (kq / 2) & 1u)) return false;
+    ++items;
     tc5_fence_after();
-    scores(0, kq & 1u);
-    scores(1, kq & 1u);
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) scores(i, kq & 1u);
     tc5_commit(&sh.k_empty[kq & 1u]);
-    for (int j = 0; j < w.steps; ++j) {
-      const uint32_t q = kq + j, st = q & 1u, nx = st ^ 1u;
-      if (!mbar_wait(&sh.v_full[st], (q / 2) & 1u)) return false;
-      const uint64_t dv = sw128_mn_desc(smem_u32(sV + st * KVB), 16384);
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j, ++kq) {
+      const uint32_t st = kq & 1u, nx = st ^ 1u;
+      if (!mbar_wait(&sh.v_full[st], (kq / 2) & 1u)) return false;
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
-        if (!mbar_wait(&sh.p_full[i], q & 1u)) return false;
+        if (!mbar_wait(&sh.p_full[i], kq & 1u)) return false;
         tc5_fence_after();
+        const uint64_t v = dv + (uint64_t)(st * (KVB >> 4));
 #pragma unroll
         for (int k = 0; k < TC_KV / 16; ++k)
-          tc5_mma_ta(tmem + 256 + i * D, tmem + i * 128 + 8 * k, dv + (uint64_t)(k * 128), id_o, (j | k) != 0);
+          tc5_mma_ta(tmem + 256 + i * D, tmem + i * 128 + 8 * k, v + (uint64_t)(k * 128), id_o, (j | k) != 0);
         if (i == 1) tc5_commit(&sh.v_empty[st]);
-        if (j + 1 < w.steps) {
-          if (i == 0 && !mbar_wait(&sh.k_full[nx], ((q + 1) / 2) & 1u)) return false;
+        if (j + 1 < steps) {
+          if (i == 0 && !mbar_wait(&sh.k_full[nx], ((kq + 1) / 2) & 1u)) return false;
           tc5_fence_after();
           scores(i, nx);
           if (i == 1) tc5_commit(&sh.k_empty[nx]);
@@ -542,8 +586,6 @@ __device__ __forceinline__ void tc_products(const AttendArgs& a, TcShared& sh, u
         }
       }
     }
-    kq += (uint32_t)w.steps;
-    ++items;
     return true;
   });
   // nothing of the tensor core's may be pending when its memory is freed
@@ -551,7 +593,7 @@ __device__ __forceinline__ void tc_products(const AttendArgs& a, TcShared& sh, u
   mbar_wait(&sh.done, 0);
 }
 
-// Registers: 512 threads start with 128 each; 128 (2 x 184 + 96 + 48) = 512 x 128.
+// Registers: 512 threads start with 128 each; 128 (2 x 168 + 96 + 80) = 512 x 128.
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
 template <int N>
@@ -587,13 +629,13 @@ __global__ void __launch_bounds__(TC_NT, 1) attend_tc_kernel(AttendArgs a) {
   tc5_fence_after();
   bool bad = false;
   if (warp < 8) {
-    more_registers<184>();
+    more_registers<168>();
     tc_softmax<D>(a, sh, sQ, &bad);
   } else if (warp < 12) {
     less_registers<96>();
     tc_decode<D>(a, sh, sK, sV, &bad);
   } else {
-    less_registers<48>();
+    less_registers<80>();
     if (threadIdx.x == 12 * 32) tc_products<D>(a, sh, sQ, sK, sV, &bad);
   }
   if (bad) atomicOr(a.err, DERR_BOUNDS);
