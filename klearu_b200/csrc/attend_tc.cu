@@ -221,31 +221,27 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
     if (w.steps > 0) {
       // the row of Q as f16, its largest value in [2^13, 2^14), K-major with the 128-byte swizzle
       const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q.p) + tok * a.q.token + head * a.q.head;
-      float top = 0.f;
-      bool fin = true;
-      if (live) {
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          float x[8];
-          load8_bf16(q + 8 * c, a.q.vec, x);
+      uint4 raw[D / 8];  // all of the row's loads at once: nothing else runs until the first scores
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            top = fmaxf(top, fabsf(x[u]));
-            fin = fin && finite_f(x[u]);
-          }
-        }
+      for (int c = 0; c < D / 8; ++c) raw[c] = live ? load8_raw(q + 8 * c, a.q.vec) : make_uint4(0, 0, 0, 0);
+      uint32_t top = 0;  // the largest |x|, as bf16 bits
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) top = __vmaxu2(top, v[u] & 0x7fff7fffu);
       }
-      eq = max(-126, min(126, 13 - ((int)(__float_as_uint(top) >> 23) - 127)));
+      top = max(top & 0xffffu, top >> 16);
+      const bool fin = top < 0x7f80u;
+      eq = max(-126, min(126, 13 - ((int)(top >> 7) - 127)));
       // the scale's sign goes into q, and a scale of zero makes it zero, so that a score's factor is positive
       const float up = a.scale == 0.f ? 0.f : a.scale < 0.f ? -pow2(eq) : pow2(eq);
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
-        float x[8] = {};
-        if (live) load8_bf16(q + 8 * c, a.q.vec, x);
-        uint32_t v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          v[u] = fin ? pack_f16(x[2 * u] * up, x[2 * u + 1] * up) : 0x7fff7fffu;  // a row that is not finite is NaN
+      for (int c = 0; c < D / 8; ++c) {
+        uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)  // a row that is not finite is NaN
+          v[u] = fin ? pack_f16(__uint_as_float(v[u] << 16) * up, __uint_as_float(v[u] & 0xffff0000u) * up) : 0x7fff7fffu;
         *reinterpret_cast<uint4*>(to_q + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) =
             make_uint4(v[0], v[1], v[2], v[3]);
       }
@@ -269,7 +265,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
       const float f = fmaxf(scl * exp2f((float)(st.ek - eq)), 1.2e-38f);  // never 0, which an unseen score's -inf would make NaN
       const int k0 = w.lo + j * TC_KV;
       const bool partial = k0 + TC_KV - 1 > pos_first || (a.window > 0 && k0 <= pos_last - a.window);
-      uint64_t sum2 = 0;
+      uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {  // 64 scores at a time, which fit the registers
         float s[64];
@@ -289,9 +285,15 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
           for (int u = 0; u < 64; ++u)
             if (hole4 >> (8 * (u >> 4)) & 1u) s[u] = -INFINITY;
         }
-        float top = -INFINITY;
+        // maxima and sums in four chains: a warp has its scheduler almost to itself, so latency counts
+        float tops[4];
 #pragma unroll
-        for (int u = 0; u < 64; u += 2) top = fmaxf(top, fmaxf(s[u], s[u + 1]));
+        for (int u = 0; u < 4; ++u) tops[u] = fmaxf(s[u], s[u + 4]);
+#pragma unroll
+        for (int u = 8; u < 64; u += 8)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tops[c] = fmaxf(tops[c], fmaxf(s[u + c], s[u + c + 4]));
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         if (top != -INFINITY) top = fmaf(top, f, ev);
         if (__any_sync(FULL, top > lift)) {
           const bool first = lift == -INFINITY;
@@ -303,7 +305,8 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
             lift = now + 8.f;
           }
           l *= keep;
-          sum2 = mul2(sum2, pair(keep, keep));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum2[c] = mul2(sum2[c], pair(keep, keep));
           if (h == 1) {  // the step's first probabilities
 #pragma unroll 1
             for (int c = 0; c < 2; ++c) {
@@ -340,7 +343,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
             unpair(fma2(pair(s[32 * c + 2 * u], s[32 * c + 2 * u + 1]), f2, less2), x, y);
             x = exp2_fast(x);
             y = exp2_fast(y);
-            sum2 = add2(sum2, pair(x, y));
+            sum2[u & 3] = add2(sum2[u & 3], pair(x, y));
             pk[u] = pack_f16(x, y);
           }
           tc5_st16(tS + 32 * h + 16 * c, pk);
@@ -348,7 +351,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
         if (h == 0) tc5_st_wait();  // the second half may read them back
       }
       float x, y;
-      unpair(sum2, x, y);
+      unpair(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), x, y);
       l = fmaf(x + y, exp2f(-ev), l);
       tc5_st_wait();
       tc5_fence_before();

@@ -124,17 +124,17 @@ __device__ __forceinline__ SeqSpan seq_span(const SeqView& s, int b, int page_si
 
 __device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// 8 bf16 of a row as f32; vec: 16-byte aligned
+// 8 bf16 of a row; vec: 16-byte aligned
+__device__ __forceinline__ uint4 load8_raw(const __nv_bfloat16* p, bool vec) {
+  if (vec) return *reinterpret_cast<const uint4*>(p);
+  const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+  return make_uint4((uint32_t)s[0] | (uint32_t)s[1] << 16, (uint32_t)s[2] | (uint32_t)s[3] << 16,
+                    (uint32_t)s[4] | (uint32_t)s[5] << 16, (uint32_t)s[6] | (uint32_t)s[7] << 16);
+}
+// as f32
 __device__ __forceinline__ void load8_bf16(const __nv_bfloat16* p, bool vec, float* x) {
-  uint32_t w[4];
-  if (vec) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-  } else {
-    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)s[2 * i] | ((uint32_t)s[2 * i + 1] << 16);
-  }
+  const uint4 r = load8_raw(p, vec);
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     x[2 * i] = __uint_as_float(w[i] << 16);
