@@ -3,17 +3,18 @@
 //
 // One block takes 256 rows (token, query head) of one key head as two tiles of
 // 128, so that one tile multiplies while the other takes its softmax:
-//  * warps 0-3 and 4-7: softmax of tile 0 and 1, one row per thread, 64
-//    scores in registers at a time; P goes back to tensor memory as f16, over the scores
-//    that it came from; O is rescaled in place only when a row's maximum has
-//    risen by more than 2^8;
+//  * warps 0-3 and 4-7: softmax of tile 0 and 1, one row per thread, 64 scores
+//    in registers at a time; P goes back to tensor memory as f16, over the
+//    scores that it came from; O is rescaled in place only when a row's maximum
+//    has risen by more than 2^8;
 //  * warps 8-11: the next 128 keys and values, codes read from global memory
 //    one step ahead, turned into f16 (s c + m in one rounding) and written to
 //    shared memory in the tensor core's swizzled layouts, K with D contiguous,
 //    V as it stands (its tokens are the product's K, "MN-major");
-//  * a thread of warp 12: issues S_i = Q_i . K^T and O_i += P_i . V in the order
-//    PV_0, S_0, PV_1, S_1 of each step, so the scores' completion also says
-//    that O_i may be rescaled.
+//  * a thread of warp 12: the products, O_i += P_i . V and then S_i = Q_i . K^T
+//    of the next step, the tiles in turn, which keeps their softmaxes apart.
+//    Few barriers (a commit each) and rolled loops: the four roles share the
+//    instruction caches, and unrolling this one over the tiles cost 14%.
 // f16, not bf16, for its 11 bits: with keys, values and probabilities at 2^-12
 // the output is as exact as its own bf16 rounding.  Its range is made up for by
 // powers of two: of each row of Q, of each step's K (both into the score's
@@ -22,7 +23,12 @@
 // Tensor memory: S_0, S_1 (128 columns each), O_0, O_1 (D columns each).
 //
 // Per 128 keys and 256 rows at D = 128 the tensor cores need 2048 cycles and
-// the 32768 exponentials as many of the special function units.
+// the 32768 exponentials as many of the special function units; a step takes
+// about 5000.  What is left bounds it: each scheduler has two softmax warps and
+// one decoding warp, about 2600 instructions a step at one in four cycles each.
+// Tried without gain: two threads to a row (twice the softmax warps), half of
+// the exponentials as polynomials, scores of 64 keys (a product reads all of Q
+// whatever its width), P and its product in halves.
 #include <cuda_fp16.h>
 
 #include <cstddef>
@@ -140,10 +146,11 @@ struct TcSmem {
 // A step's powers of two and missing pages.
 struct TcStep {
   unsigned char hole[8];  // 16-token tiles whose page does not exist
-  int ek, ev;             // K is held times 2^-ek, V times 2^-ev
+  float ek2, ev;          // K is held times 1 / ek2, V times 2^-ev
 };
 struct TcShared {
-  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], done;
+  uint64_t q_full, k_full[2], v_full[2], done;
+  uint64_t s_full[2], p_full[2], o_full[2];  // by tile, one phase a step: scores there; P there; O has taken P
   uint32_t tmem;
   int fail;
   alignas(16) uint32_t reach[2][2][4];  // by step & 1: largest |K|, |V| of each decoding warp
@@ -205,66 +212,75 @@ __device__ __forceinline__ void tc_each(const AttendArgs& a, TcShared& sh, bool*
 // ---- warps 0-7: one row per thread ----
 template <int D>
 __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, unsigned char* sQ, bool* bad) {
+  constexpr int LPR = D / 8, RPI = 32 / LPR;  // a row's lanes where a warp moves rows, 16 bytes each; rows at a time
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 2, r = threadIdx.x & 127;
   const int kvh = blockIdx.y, group = a.q_heads / a.cache.kv_heads;
   const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
   const uint32_t tS = sh.tmem + i * 128 + lane_off, tO = sh.tmem + 256 + i * D + lane_off;
-  unsigned char* to_q = sQ + i * TcSmem<D>::Q + r * 128;
-  uint32_t kq = 0, items = 0;
+  // row x, chunk c of 16 bytes of this tile's share of shared memory: the 128-byte swizzle
+  unsigned char* tile = sQ + i * TcSmem<D>::Q;
+  auto place = [&](int x, int c) {
+    return reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + x * 128 + (((c & 7) ^ (x & 7)) << 4));
+  };
+  const int sub = lane / LPR, chunk = lane % LPR, warp_row = r & ~31;
+  uint32_t kq = 0;
   tc_each(a, sh, bad, [&](const TcWork& w) {
     const int row = w.r0 + i * 128 + r;
-    const bool live = row < w.rows;
-    const int64_t tok = w.s.row + row / group;
-    const int head = kvh * group + row % group;
-    float scl = 0.f;  // what a score is worth in units of log2, but for the keys' power of two
-    int eq = 0;
+    const int rows_here = w.rows - (w.r0 + i * 128 + warp_row);  // of this warp's 32, how many there are
+    float worth = 0.f;  // of a score, in units of log2, but for the keys' power of two
     if (w.steps > 0) {
-      // the row of Q as f16, its largest value in [2^13, 2^14), K-major with the 128-byte swizzle
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q.p) + tok * a.q.token + head * a.q.head;
-      uint4 raw[D / 8];  // all of the row's loads at once: nothing else runs until the first scores
+      // the rows of Q as f16, each with its largest value in [2^13, 2^14), K-major; a row by LPR lanes
+      const int64_t mine = (w.s.row + row / group) * a.q.token + (kvh * group + row % group) * a.q.head;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q.p) + 8 * chunk;
+      const float factor = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) raw[c] = live ? load8_raw(q + 8 * c, a.q.vec) : make_uint4(0, 0, 0, 0);
-      uint32_t top = 0;  // the largest |x|, as bf16 bits
+      for (int h = 0; h < 2; ++h) {
+        uint4 raw[LPR / 2];  // their loads at once: nothing else runs until the first scores
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        const uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+        for (int u = 0; u < LPR / 2; ++u) {
+          const int x = (h * (LPR / 2) + u) * RPI + sub;
+          const int64_t at = __shfl_sync(FULL, mine, x);
+          raw[u] = x < rows_here ? load8_raw(q + at, a.q.vec) : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) top = __vmaxu2(top, v[u] & 0x7fff7fffu);
-      }
-      top = max(top & 0xffffu, top >> 16);
-      const bool fin = top < 0x7f80u;
-      eq = max(-126, min(126, 13 - ((int)(top >> 7) - 127)));
-      // the scale's sign goes into q, and a scale of zero makes it zero, so that a score's factor is positive
-      const float up = a.scale == 0.f ? 0.f : a.scale < 0.f ? -pow2(eq) : pow2(eq);
+        for (int u = 0; u < LPR / 2; ++u) {
+          const int x = (h * (LPR / 2) + u) * RPI + sub;
+          uint32_t v[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w}, top = 0;  // the largest |x|, as bf16 bits
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+          for (int e = 0; e < 4; ++e) top = __vmaxu2(top, v[e] & 0x7fff7fffu);
+          top = max(top & 0xffffu, top >> 16);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)  // a row that is not finite is NaN
-          v[u] = fin ? pack_f16(__uint_as_float(v[u] << 16) * up, __uint_as_float(v[u] & 0xffff0000u) * up) : 0x7fff7fffu;
-        *reinterpret_cast<uint4*>(to_q + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) =
-            make_uint4(v[0], v[1], v[2], v[3]);
+          for (int d = 1; d < LPR; d <<= 1) top = max(top, __shfl_xor_sync(FULL, top, d));
+          const int eq = max(-115, min(100, 13 - ((int)(top >> 7) - 127)));
+          // the scale's sign goes into q, and a scale of zero makes it zero, so that a score's factor is positive
+          const float up = a.scale == 0.f ? 0.f : a.scale < 0.f ? -pow2(eq) : pow2(eq);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)  // a row that is not finite is NaN
+            v[e] = top < 0x7f80u ? pack_f16(__uint_as_float(v[e] << 16) * up, __uint_as_float(v[e] & 0xffff0000u) * up)
+                                 : 0x7fff7fffu;
+          *place(warp_row + x, chunk) = make_uint4(v[0], v[1], v[2], v[3]);
+          const float its = __shfl_sync(FULL, factor * pow2(-eq), (lane % RPI) * LPR);
+          if (lane / RPI == h * (LPR / 2) + u) worth = its;
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
-      scl = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
     }
-    const int pos = w.first + row / group;
-    const int pos_first = w.first + (w.r0 + i * 128) / group;  // of this tile's rows
-    const int pos_last = w.first + (min(w.r0 + i * 128 + 128, w.rows) - 1) / group;
-    float ref = 0.f, lift = -INFINITY, l = 0.f;
-    int ev0 = 0;
+    const int seen = w.first + row / group - w.lo;  // the row sees keys up to its own, counted from w.lo
+    // every row of the tile sees all of the steps in (jlo, jhi)
+    const int jhi = (w.first + (w.r0 + i * 128) / group - w.lo + 1) / TC_KV;
+    const int jlo = a.window > 0 ? (w.first + (min(w.r0 + i * 128 + 128, w.rows) - 1) / group - a.window - w.lo + TC_KV) / TC_KV - 1
+                                 : -1;
+    float ref = 0.f, lift = -INFINITY, l = 0.f, ev0 = 0.f;
     for (int j = 0; j < w.steps; ++j) {
       if (!warp_wait(&sh.s_full[i], (kq + j) & 1u)) return false;
       tc5_fence_after();
       const TcStep& st = sh.step[(kq + j) & 3u];
       const uint2 holes = *reinterpret_cast<const uint2*>(st.hole);
       if (j == 0) ev0 = st.ev;
-      const float ev = (float)(st.ev - ev0);
-      const float f = fmaxf(scl * exp2f((float)(st.ek - eq)), 1.2e-38f);  // never 0, which an unseen score's -inf would make NaN
-      const int k0 = w.lo + j * TC_KV;
-      const bool partial = k0 + TC_KV - 1 > pos_first || (a.window > 0 && k0 <= pos_last - a.window);
+      const float ev = st.ev - ev0;
+      const float f = fmaxf(worth * st.ek2, 1.2e-38f);  // never 0, which an unseen score's -inf would make NaN
       uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {  // 64 scores at a time, which fit the registers
@@ -272,14 +288,14 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
         tc5_ld32(tS + 64 * h, reinterpret_cast<uint32_t*>(s));
         tc5_ld32(tS + 64 * h + 32, reinterpret_cast<uint32_t*>(s) + 32);
         tc5_ld_wait();
-        if (partial) {
-          const int to = pos - k0, from = a.window > 0 ? max(0, to - a.window + 1) : 0;  // columns [from, to] are seen
+        const uint32_t hole4 = h ? holes.y : holes.x;
+        if (j >= jhi || j <= jlo) {
+          const int to = seen - TC_KV * j - 64 * h, from = a.window > 0 ? max(0, to - a.window + 1) : 0;  // columns seen
           const unsigned span = to >= from ? (unsigned)(to - from) : 0u, at = to >= from ? (unsigned)from : 0x40000000u;
 #pragma unroll
           for (int u = 0; u < 64; ++u)
-            if ((unsigned)(64 * h + u) - at > span) s[u] = -INFINITY;
+            if ((unsigned)u - at > span) s[u] = -INFINITY;
         }
-        const uint32_t hole4 = h ? holes.y : holes.x;
         if (hole4) {
 #pragma unroll
           for (int u = 0; u < 64; ++u)
@@ -321,7 +337,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
               tc5_st16(tS + 16 * c, v);
             }
           }
-          if (j > 0) {
+          if (j > 0) {  // O: these scores were not begun before it had taken the step before
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t v[16];
@@ -339,8 +355,9 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
           uint32_t pk[16];
 #pragma unroll
           for (int u = 0; u < 16; ++u) {
+            uint64_t v = fma2(pair(s[32 * c + 2 * u], s[32 * c + 2 * u + 1]), f2, less2);
             float x, y;
-            unpair(fma2(pair(s[32 * c + 2 * u], s[32 * c + 2 * u + 1]), f2, less2), x, y);
+            unpair(v, x, y);
             x = exp2_fast(x);
             y = exp2_fast(y);
             sum2[u & 3] = add2(sum2[u & 3], pair(x, y));
@@ -352,38 +369,48 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, TcShared& sh, un
       }
       float x, y;
       unpair(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), x, y);
-      l = fmaf(x + y, exp2f(-ev), l);
+      l = ev == 0.f ? l + (x + y) : fmaf(x + y, exp2f(-ev), l);
       tc5_st_wait();
       tc5_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.p_full[i]);
     }
+    // O through the rows' place in shared memory, whose queries are done with, so that a row is stored by LPR lanes
     if (w.steps > 0) {
-      if (!warp_wait(&sh.o_full[i], items & 1u)) return false;
+      kq += (uint32_t)w.steps;
+      if (!warp_wait(&sh.o_full[i], (kq - 1) & 1u)) return false;
       tc5_fence_after();
-      ++items;
-    }
-    kq += (uint32_t)w.steps;
-    const float inv = l == 0.f ? 0.f : 1.f / l, up = exp2f((float)ev0);
-    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.p) + tok * a.out.token + head * a.out.head;
+      const float inv = l == 0.f ? 0.f : 1.f / l, up = exp2f(ev0);
 #pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      uint32_t v[32];
-      if (w.steps > 0) {
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t v[32];
         tc5_ld32(tO + 32 * c, v);
         tc5_ld_wait();
-      }
-      if (live) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          float y[8];
+          uint32_t y[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : __uint_as_float(v[8 * u + e]) * inv * up;
-          store8_bf16(out + 32 * c + 8 * u, a.out.vec, y);
+          for (int e = 0; e < 4; ++e)
+            y[e] = l == 0.f ? 0u
+                            : pack_bf16(__uint_as_float(v[8 * u + 2 * e]) * inv * up,
+                                        __uint_as_float(v[8 * u + 2 * e + 1]) * inv * up);
+          *place(r, 4 * c + u) = make_uint4(y[0], y[1], y[2], y[3]);
         }
       }
+      tc5_fence_before();  // the next rows' first product overwrites O
+    } else {
+      for (int c = 0; c < LPR; ++c) *place(r, c) = make_uint4(0, 0, 0, 0);
     }
-    tc5_fence_before();  // the next rows' first product overwrites O
+    __syncwarp();
+    const int64_t mine = (w.s.row + row / group) * a.out.token + (kvh * group + row % group) * a.out.head;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.p) + 8 * chunk;
+#pragma unroll 4
+    for (int u = 0; u < LPR; ++u) {
+      const int x = u * RPI + sub;
+      const int64_t at = __shfl_sync(FULL, mine, x);
+      if (x < rows_here) store8_raw(out + at, a.out.vec, *place(warp_row + x, chunk));
+    }
+    __syncwarp();
     return true;
   });
 }
@@ -459,8 +486,9 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
         sh.reach[st][0][tid >> 5] = rk;
         sh.reach[st][1][tid >> 5] = rv;
       }
-      // one wait says that the ring's K stage and the step's slot are free; the four warps give up as one
-      if (q >= 2 && alive) alive = warp_wait(&sh.k_empty[st], (q / 2 - 1) & 1u);
+      // tile 1's scores of the step before are there: K's and V's stages of two steps before are free (its O had
+      // taken P before them), and so is the step's slot.  The four warps give up as one.
+      if (q >= 1 && alive) alive = warp_wait(&sh.s_full[1], (q - 1) & 1u);
       const bool hole = is_hole(j, page);
       if (hole) *bad = true;
       if (alive && sub == 0) sh.step[q & 3u].hole[tid >> 4] = hole;
@@ -472,8 +500,8 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
       const int ev = tv ? max(-126, (int)(tv >> 23) - 127 - 13) : ev_before;  // nothing but zeros: as it was
       ev_before = ev;
       if (tid == 0) {
-        sh.step[q & 3u].ek = ek;
-        sh.step[q & 3u].ev = ev;
+        sh.step[q & 3u].ek2 = pow2(ek);
+        sh.step[q & 3u].ev = (float)ev;
       }
       const float fk = pow2(-ek), fv = pow2(-ev);
       {  // ---- K: this thread's token, D contiguous ----
@@ -499,10 +527,6 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
       fetch_k(tile);
       next = page_of(j + 2);
       // ---- V: 16-byte chunks of the codes; two tokens each ----
-      if (q >= 2 && !warp_wait(&sh.v_empty[st], (q / 2 - 1) & 1u)) {
-        alive = false;
-        continue;
-      }
       uint32_t s2[2][2], m2[2][2];  // of tokens 2t + o of half h
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -538,54 +562,53 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
   });
 }
 
-// ---- one thread: the products ----
+// ---- one thread: the products, the tiles in turn, so that one's softmax runs while the other multiplies ----
 template <int D>
 __device__ __forceinline__ void tc_products(const AttendArgs& a, TcShared& sh, unsigned char* sQ, unsigned char* sK,
                                             unsigned char* sV, bool* bad) {
   constexpr int QB = TcSmem<D>::Q, KVB = TcSmem<D>::KV;
   constexpr uint32_t bf16_ab = (1u << 7) | (1u << 10);
-  const uint32_t tmem = sh.tmem, id_s = f16_idesc(128, TC_KV) & ~bf16_ab, id_o = (f16_idesc(128, D) & ~bf16_ab) | (1u << 16);
-  uint32_t kq = 0, items = 0;
+  constexpr uint32_t id_s = f16_idesc(128, TC_KV) & ~bf16_ab, id_o = (f16_idesc(128, D) & ~bf16_ab) | (1u << 16);
+  const uint32_t tmem = sh.tmem;
   const uint64_t dq = sw128_desc(smem_u32(sQ)), dk = sw128_desc(smem_u32(sK));
   const uint64_t dv = sw128_mn_desc(smem_u32(sV), 16384);
+  uint32_t q = 0, items = 0;  // steps so far
   auto scores = [&](int i, uint32_t st) {
-    const uint64_t q = dq + (uint64_t)(i * (QB >> 4)), k = dk + (uint64_t)(st * (KVB >> 4));
+    const uint64_t x = dq + (uint64_t)(i * (QB >> 4)), k = dk + (uint64_t)(st * (KVB >> 4));
 #pragma unroll
-    for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        tc5_mma(tmem + i * 128, q + (uint64_t)(h * 1024 + u * 2), k + (uint64_t)(h * 1024 + u * 2), id_s, (h | u) != 0);
+    for (int u = 0; u < D / 16; ++u) {
+      const uint64_t at = (uint64_t)((u >> 2) * 1024 + (u & 3) * 2);
+      tc5_mma(tmem + i * 128, x + at, k + at, id_s, u != 0);
+    }
     tc5_commit(&sh.s_full[i]);
   };
   tc_each(a, sh, bad, [&](const TcWork& w) {
     const int steps = w.steps;
     if (steps == 0) return true;
-    if (!mbar_wait(&sh.q_full, items & 1u) || !mbar_wait(&sh.k_full[kq & 1u], (kq / 2) & 1u)) return false;
+    if (!mbar_wait(&sh.q_full, items & 1u) || !mbar_wait(&sh.k_full[q & 1u], (q / 2) & 1u)) return false;
     ++items;
     tc5_fence_after();
 #pragma unroll 1
-    for (int i = 0; i < 2; ++i) scores(i, kq & 1u);
-    tc5_commit(&sh.k_empty[kq & 1u]);
+    for (int i = 0; i < 2; ++i) scores(i, q & 1u);
 #pragma unroll 1
-    for (int j = 0; j < steps; ++j, ++kq) {
-      const uint32_t st = kq & 1u, nx = st ^ 1u;
-      if (!mbar_wait(&sh.v_full[st], (kq / 2) & 1u)) return false;
+    for (int j = 0; j < steps; ++j, ++q) {
+      const uint32_t st = q & 1u, nx = st ^ 1u;
+      if (!mbar_wait(&sh.v_full[st], (q / 2) & 1u)) return false;
+      const uint64_t v = dv + (uint64_t)(st * (KVB >> 4));
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
-        if (!mbar_wait(&sh.p_full[i], kq & 1u)) return false;
+        if (!mbar_wait(&sh.p_full[i], q & 1u)) return false;
         tc5_fence_after();
-        const uint64_t v = dv + (uint64_t)(st * (KVB >> 4));
 #pragma unroll
-        for (int k = 0; k < TC_KV / 16; ++k)
-          tc5_mma_ta(tmem + 256 + i * D, tmem + i * 128 + 8 * k, v + (uint64_t)(k * 128), id_o, (j | k) != 0);
-        if (i == 1) tc5_commit(&sh.v_empty[st]);
+        for (int u = 0; u < TC_KV / 16; ++u)
+          tc5_mma_ta(tmem + 256 + i * D, tmem + i * 128 + 8 * u, v + (uint64_t)(u * 128), id_o, (j | u) != 0);
+        tc5_commit(&sh.o_full[i]);
         if (j + 1 < steps) {
-          if (i == 0 && !mbar_wait(&sh.k_full[nx], ((kq + 1) / 2) & 1u)) return false;
+          if (i == 0 && !mbar_wait(&sh.k_full[nx], ((q + 1) / 2) & 1u)) return false;
+          // products into different accumulators are not ordered: O has to have taken the P that these scores overwrite
+          if (!mbar_wait(&sh.o_full[i], q & 1u)) return false;
           tc5_fence_after();
           scores(i, nx);
-          if (i == 1) tc5_commit(&sh.k_empty[nx]);
-        } else {
-          tc5_commit(&sh.o_full[i]);
         }
       }
     }
@@ -616,8 +639,6 @@ __global__ void __launch_bounds__(TC_NT, 1) attend_tc_kernel(AttendArgs a) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.k_full[i], 4);
       mbar_init(&sh.v_full[i], 4);
-      mbar_init(&sh.k_empty[i], 1);
-      mbar_init(&sh.v_empty[i], 1);
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 4);
       mbar_init(&sh.o_full[i], 1);

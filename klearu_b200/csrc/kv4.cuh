@@ -145,20 +145,21 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ void store8_bf16(__nv_bfloat16* p, bool vec, const float* x) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+__device__ __forceinline__ void store8_raw(__nv_bfloat16* p, bool vec, uint4 v) {
   if (vec) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-    unsigned short* s = reinterpret_cast<unsigned short*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[2 * i] = (unsigned short)(w[i] & 0xffffu);
-      s[2 * i + 1] = (unsigned short)(w[i] >> 16);
-    }
+    *reinterpret_cast<uint4*>(p) = v;
+    return;
   }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  unsigned short* s = reinterpret_cast<unsigned short*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s[2 * i] = (unsigned short)(w[i] & 0xffffu);
+    s[2 * i + 1] = (unsigned short)(w[i] >> 16);
+  }
+}
+__device__ __forceinline__ void store8_bf16(__nv_bfloat16* p, bool vec, const float* x) {
+  store8_raw(p, vec, make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])));
 }
 
 }  // namespace kl
