@@ -24,27 +24,33 @@ from ._lib import HeadRowsC, SeqBatchC, check
 from .core import Context, default_context
 
 
+_BF16 = torch.bfloat16
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def launch(ctx: Context, what: str, *args) -> None:
     """One C call on torch's current stream of the context's device."""
-    s = torch.cuda.current_stream(ctx.device).cuda_stream
-    own = ctx.stream.cuda_stream
+    s = _raw_stream(ctx.device)
+    lib, own = ctx.lib, ctx.stream.cuda_stream
     with ctx.launch_lock:
-        if s != own:
-            ctx.lib.kl_ctx_set_stream(ctx.h, s)
-        try:
-            status = getattr(ctx.lib, what)(*args)
-            if status:
-                check(status, ctx.h, what)
-        finally:
-            if s != own:
-                ctx.lib.kl_ctx_set_stream(ctx.h, own)
+        if s == own:
+            status = getattr(lib, what)(*args)
+        else:
+            lib.kl_ctx_set_stream(ctx.h, s)
+            try:
+                status = getattr(lib, what)(*args)
+            finally:
+                lib.kl_ctx_set_stream(ctx.h, own)
+        if status:
+            check(status, ctx.h, what)
 
 
 def want(ctx: Context, t: torch.Tensor, what: str, dtype) -> None:
     """What every tensor argument has to be."""
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != ctx.device:
+    if not isinstance(t, torch.Tensor) or t.get_device() != ctx.device:
         raise ValueError(f"{what} must be a tensor on cuda:{ctx.device}")
-    if t.dtype not in dtype if isinstance(dtype, tuple) else t.dtype != dtype:
+    if t.dtype is not dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
         raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires a gradient, and this call has no backward pass")
@@ -122,18 +128,24 @@ class SeqBatch:
         self._tensors = (cu_q, kv_len, page_table)
         self.num_seqs, self.max_q = n, int(max_q)
         self.max_kv = 2**31 - 1 if max_kv is None else min(int(max_kv), 2**31 - 1)
-        self.device = cu_q.device
+        self.device = cu_q.device.index
+        self.sizes = (n, self.max_q, self.max_kv, page_table.shape[1])
+        self._c: dict[int, object] = {}  # the C struct by num_tokens
 
     cu_q = property(lambda self: self._tensors[0])
     kv_len = property(lambda self: self._tensors[1])
     page_table = property(lambda self: self._tensors[2])
 
-    def c(self, num_tokens: int) -> SeqBatchC:
-        cu_q, kv_len, table = self._tensors
-        wide = table.shape[1]
-        return SeqBatchC(cu_q.data_ptr(), kv_len.data_ptr(), table.data_ptr(),
-                         table.stride(0) if self.num_seqs > 1 else wide, wide, self.num_seqs, num_tokens,
-                         min(self.max_q, 2**31 - 1), self.max_kv)
+    def c(self, num_tokens: int):
+        """A reference to the C struct for a call with so many rows."""
+        got = self._c.get(num_tokens)
+        if got is None:
+            cu_q, kv_len, table = self._tensors
+            wide = table.shape[1]
+            got = self._c[num_tokens] = C.byref(SeqBatchC(
+                cu_q.data_ptr(), kv_len.data_ptr(), table.data_ptr(), table.stride(0) if self.num_seqs > 1 else wide, wide,
+                self.num_seqs, num_tokens, min(self.max_q, 2**31 - 1), self.max_kv))
+        return got
 
 
 class Kv4Cache:
@@ -156,16 +168,23 @@ class Kv4Cache:
         if getattr(self, "h", None):
             self.lib.kl_kv4_destroy(self.h)
 
-    def _rows(self, t: torch.Tensor, what: str, tokens: int | None = None, heads: int | None = None) -> HeadRowsC:
-        want(self.ctx, t, what, torch.bfloat16)
-        if t.dim() != 3 or t.shape[2] != self.head_dim or t.stride(2) != 1:
+    def _rows(self, t: torch.Tensor, what: str, tokens: int | None = None, heads: int | None = None):
+        want(self.ctx, t, what, _BF16)
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or shape[2] != self.head_dim or stride[2] != 1:
             raise ValueError(f"{what} must be [tokens][heads][{self.head_dim}], contiguous in the last dimension")
-        if (tokens is not None and t.shape[0] != tokens) or (heads is not None and t.shape[1] != heads):
-            raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tokens} tokens and {heads} heads")
-        return HeadRowsC(t.data_ptr(), t.stride(0), t.stride(1))
+        if (tokens is not None and shape[0] != tokens) or (heads is not None and shape[1] != heads):
+            raise ValueError(f"{what} has shape {tuple(shape)}, expected {tokens} tokens and {heads} heads")
+        return C.byref(HeadRowsC(t.data_ptr(), stride[0], stride[1]))
 
-    def _batch(self, batch: SeqBatch, tokens: int) -> SeqBatchC:
-        if batch.device.index != self.ctx.device:
+    def _new(self, like: torch.Tensor, tokens: int, heads: int):
+        """A new [tokens][heads][head_dim] tensor and its C rows."""
+        d = self.head_dim
+        t = like.new_empty((tokens, heads, d))
+        return t, C.byref(HeadRowsC(t.data_ptr(), heads * d, d))
+
+    def _batch(self, batch: SeqBatch, tokens: int):
+        if batch.device != self.ctx.device:
             raise ValueError(f"the batch must be on cuda:{self.ctx.device}")
         return batch.c(tokens)
 
@@ -184,8 +203,9 @@ class Kv4Cache:
             rq = self._rows(q, "q", t)
             heads = q.shape[1]
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-            ro = self._rows(q_out, "q_out", t, heads)
+                q_out, ro = self._new(q, t, heads)
+            else:
+                ro = self._rows(q_out, "q_out", t, heads)
         elif q_out is not None:
             raise ValueError("q_out without q")
         if positions is not None:
@@ -196,9 +216,8 @@ class Kv4Cache:
             raise ValueError("the rope must share the cache's context")
         c = self._batch(batch, t)
         if t:
-            launch(self.ctx, "kl_kv4_append", self.h, rope.h if rope is not None else None, C.byref(c),
-                   None if positions is None else positions.data_ptr(), heads,
-                   C.byref(rq) if heads else None, C.byref(rk), C.byref(rv), C.byref(ro) if heads else None)
+            launch(self.ctx, "kl_kv4_append", self.h, rope.h if rope is not None else None, c,
+                   None if positions is None else positions.data_ptr(), heads, rq, rk, rv, ro)
         return q_out
 
     def read(self, batch: SeqBatch, num_tokens: int, k_out: torch.Tensor | None = None,
@@ -209,13 +228,22 @@ class Kv4Cache:
         they are."""
         if num_tokens < 0:
             raise ValueError("num_tokens must be >= 0")
-        shape = (num_tokens, self.kv_heads, self.head_dim)
-        k_out, v_out = (torch.empty(shape, dtype=torch.bfloat16, device=batch.device) if x is None else x
-                        for x in (k_out, v_out))
-        rk, rv = self._rows(k_out, "k_out", *shape[:2]), self._rows(v_out, "v_out", *shape[:2])
         c = self._batch(batch, num_tokens)
+        heads = self.kv_heads
+        if k_out is None and v_out is None:
+            both = torch.empty((2, num_tokens, heads, self.head_dim), dtype=_BF16, device=batch.kv_len.device)
+            k_out, v_out = both.unbind()
+            at, d = both.data_ptr(), heads * self.head_dim
+            rk = C.byref(HeadRowsC(at, d, self.head_dim))
+            rv = C.byref(HeadRowsC(at + 2 * num_tokens * d, d, self.head_dim))
+        else:
+            if k_out is None:
+                k_out = torch.empty_like(v_out)
+            elif v_out is None:
+                v_out = torch.empty_like(k_out)
+            rk, rv = self._rows(k_out, "k_out", num_tokens, heads), self._rows(v_out, "v_out", num_tokens, heads)
         if num_tokens:
-            launch(self.ctx, "kl_kv4_read", self.h, C.byref(c), C.byref(rk), C.byref(rv))
+            launch(self.ctx, "kl_kv4_read", self.h, c, rk, rv)
         return k_out, v_out
 
     def attend(self, q: torch.Tensor, batch: SeqBatch, scale: float | None = None, window: int = 0,
@@ -230,19 +258,20 @@ class Kv4Cache:
         rq = self._rows(q, "q")
         t, heads = q.shape[0], q.shape[1]
         if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-        ro = self._rows(out, "out", t, heads)
+            out, ro = self._new(q, t, heads)
+        else:
+            ro = self._rows(out, "out", t, heads)
         c = self._batch(batch, t)
         if t == 0 or heads == 0:
             return out
-        key = (t, heads, window, batch.num_seqs, batch.max_q, batch.max_kv, c.table_width)
+        key = (batch.sizes, t, heads, window)
         need = self._workspace.get(key)
         if need is None:
             n = C.c_size_t()
-            launch(self.ctx, "kl_kv4_attend_workspace", self.h, C.byref(c), heads, window, C.byref(n))
+            launch(self.ctx, "kl_kv4_attend_workspace", self.h, c, heads, window, C.byref(n))
             need = self._workspace[key] = n.value
         # from torch's allocator in stream order: a captured graph keeps one of its own
-        space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        launch(self.ctx, "kl_kv4_attend", self.h, C.byref(c), heads, C.byref(rq), C.byref(ro),
-               self.head_dim**-0.5 if scale is None else scale, window, space.data_ptr() if need else None, need)
+        space = q.new_empty((need + 1) // 2) if need else None
+        launch(self.ctx, "kl_kv4_attend", self.h, c, heads, rq, ro, self.head_dim**-0.5 if scale is None else scale, window,
+               space.data_ptr() if need else None, need)
         return out

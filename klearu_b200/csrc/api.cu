@@ -3732,6 +3732,7 @@ AttendShape attend_shape(kl_kv4_t c, const kl_seq_batch* s, int q_heads, int win
   a.D = c->head_dim;
   a.q_heads = q_heads;
   a.kv_heads = c->view.kv_heads;
+  a.page_size = c->view.page_size;
   a.num_seqs = s->num_seqs;
   a.num_tokens = s->num_tokens;
   a.max_q = std::max(1, std::min(s->max_q, s->num_tokens));

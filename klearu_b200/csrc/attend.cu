@@ -17,13 +17,25 @@ namespace kl {
 namespace {
 
 constexpr int AT_W = 4;       // warps per block
-constexpr int AT_STAGES = 4;  // tiles in flight per warp
+constexpr int AT_STAGES = 6;  // tiles of a warp's ring, refilled two at a time
 
 struct SplitPlan {
   int chunk;      // tokens per block, a multiple of 16 AT_W
   int chunks;     // blocks along a sequence
   int row_tiles;  // blocks along a sequence's rows
+  // tile / tiles_per_page = umulhi(tile, magic) >> shift, exact below 2^31 (magic = ceil(2^(32 + shift) / d), where
+  // 2^shift < d <= 2^(shift + 1)); d = 1: magic 0
+  uint32_t magic, shift;
 };
+__device__ __forceinline__ int page_col(const SplitPlan& p, int tile) {
+  return p.magic ? (int)(__umulhi((uint32_t)tile, p.magic) >> p.shift) : tile;
+}
+// Shared memory of a block: the rings, and where the warps join.
+template <int D, int NR>
+constexpr int split_smem() {
+  constexpr int ring = AT_W * AT_STAGES * kv4_tile_bytes(D), join = AT_W * 8 * NR * D * 4;
+  return ring > join ? ring : join;
+}
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -75,8 +87,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
   constexpr int TB = kv4_tile_bytes(D), CODES = kv4_codes(D);
   constexpr int KW = D / 32;  // words of K per lane and token
   constexpr int MT = D / 16;  // O^T fragments
-  constexpr int RING = AT_W * AT_STAGES * TB, JOIN = AT_W * 8 * NR * D * 4;
-  __shared__ __align__(128) unsigned char ring[RING > JOIN ? RING : JOIN];
+  extern __shared__ __align__(128) unsigned char ring[];
   __shared__ uint64_t full[AT_W][AT_STAGES];
   __shared__ int tile_ok[AT_W][AT_STAGES];
   __shared__ float2 ml[AT_W][8 * NR];
@@ -108,20 +119,25 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
       // ---- the ring's first fills: lane i takes the warp's tile i ----
       const int32_t* table = a.seq.table + b * a.seq.table_ld;
       const int tpp = a.cache.tiles_per_page;
-      auto issue = [&](int i, int32_t page) {  // by one lane
+      const int64_t page_bytes = (int64_t)a.cache.kv_heads * tpp * TB;
+      const unsigned char* heads = a.cache.base + (int64_t)kvh * tpp * TB;
+      auto issue = [&](int i, int col, int32_t page) {  // by a lane
         const uint32_t st = (used + i) % AT_STAGES;
-        const int tile = t0 + warp + i * AT_W;
+        const int off = t0 + warp + i * AT_W - col * tpp;
         const bool ok = page >= 0 && page < a.cache.num_pages;
         tile_ok[warp][st] = ok;
         if (ok) {
           mbar_arrive_expect_tx(&full[warp][st], TB);
-          bulk_load(mine + st * TB, kv4_tile(a.cache, TB, page, kvh, tile % tpp), TB, &full[warp][st]);
+          bulk_load(mine + st * TB, heads + page * page_bytes + off * TB, TB, &full[warp][st]);
         } else {
           atomicOr(a.err, DERR_BOUNDS);
           mbar_arrive(&full[warp][st]);
         }
       };
-      if (lane < AT_STAGES && lane < n) issue(lane, table[(t0 + warp + lane * AT_W) / tpp]);
+      if (lane < AT_STAGES && lane < n) {
+        const int col = page_col(p, t0 + warp + lane * AT_W);
+        issue(lane, col, table[col]);
+      }
 
       // ---- q: row g's dims [t D/4, (t+1) D/4), scaled by a power of two ----
       uint32_t qf[NR][2 * KW][2];
@@ -196,7 +212,13 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
           down[r][u] = 1.f;
           most[r][u] = 0.f;
         }
-      int32_t next_page = n > AT_STAGES ? table[(t0 + warp + AT_STAGES * AT_W) / tpp] : 0;
+      // the refills' lanes, one for each of two tiles, have the next one's page at hand
+      int next = AT_STAGES + lane, next_col = 0;
+      int32_t next_page = 0;
+      if (lane < 2 && next < n) {
+        next_col = page_col(p, t0 + warp + next * AT_W);
+        next_page = table[next_col];
+      }
 
       for (int i = 0; i < n; ++i) {
         const uint32_t st = (used + i) % AT_STAGES;
@@ -226,18 +248,24 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
         const uint2 pr[2] = {*reinterpret_cast<const uint2*>(tile + 2 * CODES + g * 8),
                              *reinterpret_cast<const uint2*>(tile + 2 * CODES + (g + 8) * 8)};
         const bool ok = tile_ok[warp][st];
-        __syncwarp();  // the stage has been read
-        if (lane == 0 && i + AT_STAGES < n) {
-          issue(i + AT_STAGES, next_page);
-          if (i + AT_STAGES + 1 < n) next_page = table[(t0 + warp + (i + AT_STAGES + 1) * AT_W) / tpp];
+        if (i & 1) {  // two stages have been read: they are filled again
+          __syncwarp();
+          if (lane < 2 && next < n) {
+            issue(next, next_col, next_page);
+            next += 2;
+            if (next < n) {
+              next_col = page_col(p, t0 + warp + next * AT_W);
+              next_page = table[next_col];
+            }
+          }
         }
         if (!ok) continue;
 
-        float x[NR][4];
+        float x[NR][4], x2[NR][4];  // two chains of products
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) x[r][u] = 0.f;
+          for (int u = 0; u < 4; ++u) x[r][u] = x2[r][u] = 0.f;
 #pragma unroll
         for (int w = 0; w < KW; ++w)
 #pragma unroll
@@ -245,7 +273,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
             const uint32_t u0 = kw[0][w] >> (8 * h), u1 = kw[1][w] >> (8 * h);
 #pragma unroll
             for (int r = 0; r < NR; ++r)
-              mma_f16(x[r], u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qf[r][2 * w + h][0],
+              mma_f16(h ? x2[r] : x[r], u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qf[r][2 * w + h][0],
                       qf[r][2 * w + h][1]);
           }
         // x[r][2 k + i]: key g + 8 k, row 2t + i
@@ -258,7 +286,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
 #pragma unroll
           for (int r = 0; r < NR; ++r)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) x[r][2 * k + u] = fmaf(x[r][2 * k + u] * ks, f[r][u], km * qs[r][u]);
+            for (int u = 0; u < 2; ++u) x[r][2 * k + u] = fmaf((x[r][2 * k + u] + x2[r][2 * k + u]) * ks, f[r][u], km * qs[r][u]);
         }
         const int j0 = (t0 + warp + i * AT_W) * 16;
         const bool partial = j0 + 15 > see_all_to || j0 < see_all_from;
@@ -483,6 +511,11 @@ SplitPlan split_plan(const AttendShape& s) {
   chunk = std::max<int64_t>(chunk, std::min<int64_t>(round_up(span, 16 * AT_W), 256));
   p.chunk = (int)chunk;
   p.chunks = (int)std::max<int64_t>(1, ceil_div(span, chunk));
+  const int d = s.page_size / KV4_TILE;
+  if (d > 1) {
+    while ((2u << p.shift) < (unsigned)d) ++p.shift;
+    p.magic = (uint32_t)((((uint64_t)1 << (32 + p.shift)) + d - 1) / d);
+  }
   return p;
 }
 
@@ -490,7 +523,11 @@ template <int D, int NR>
 void launch_split(const AttendArgs& a, const SplitPlan& p, cudaStream_t st) {
   const dim3 grid((unsigned)(p.chunks * p.row_tiles), (unsigned)a.cache.kv_heads,
                   (unsigned)std::min(a.seq.num_seqs, 65535));
-  attend_split_kernel<D, NR><<<grid, AT_W * 32, 0, st>>>(a, p);
+  static OncePerDevice once;
+  once([] {
+    cudaFuncSetAttribute(attend_split_kernel<D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem<D, NR>());
+  });
+  attend_split_kernel<D, NR><<<grid, AT_W * 32, split_smem<D, NR>(), st>>>(a, p);
   count_launch();
   if (p.chunks == 1) return;
   cudaLaunchConfig_t cfg{};

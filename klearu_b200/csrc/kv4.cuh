@@ -87,7 +87,7 @@ struct AttendArgs {
   int* err;
 };
 struct AttendShape {
-  int D, q_heads, kv_heads, num_seqs, num_tokens;
+  int D, q_heads, kv_heads, page_size, num_seqs, num_tokens;
   int max_q, max_kv;  // of any sequence; hints: they choose the launch, not the result
   int window;
 };

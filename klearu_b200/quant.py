@@ -27,19 +27,20 @@ class Q8Rows(NamedTuple):
     hidden: torch.Tensor | None
 
 
-def _two(t: torch.Tensor, what: str) -> None:
-    if t.dim() != 2 or (t.numel() and t.stride(1) != 1):
+def _two(t: torch.Tensor, what: str) -> int:
+    """The row stride of a 2-D tensor that is contiguous in its last dimension."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.numel()):
         raise ValueError(f"{what} must be 2-D, contiguous in its last dimension")
-
-
-def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
 
 
 def _rows_q8(x, weight, residual, eps, norm, one_plus, hidden, ctx) -> Q8Rows:
-    ctx = ctx or default_context()
+    if ctx is None:  # the tensor's device says which context
+        if not isinstance(x, torch.Tensor) or not x.is_cuda:
+            raise ValueError("x must be a CUDA tensor")
+        ctx = default_context(x.get_device())
     want(ctx, x, "x", (torch.float32, torch.bfloat16))
-    _two(x, "x")
+    ldx = _two(x, "x")
     rows, cols = x.shape
     if cols == 0:
         raise ValueError("x has no columns")
@@ -47,21 +48,26 @@ def _rows_q8(x, weight, residual, eps, norm, one_plus, hidden, ctx) -> Q8Rows:
         want(ctx, weight, "weight", torch.float32)
         if weight.shape != (cols,) or not weight.is_contiguous():
             raise ValueError("weight must be contiguous, one for each column")
-    for t, name in ((residual, "residual"), (hidden, "hidden")):
-        if t is not None:
-            want(ctx, t, name, torch.float32)
-            _two(t, name)
-            if t.shape != x.shape:
-                raise ValueError(f"{name} must have x's shape")
+    ldr = ldh = 0
+    if residual is not None:
+        want(ctx, residual, "residual", torch.float32)
+        ldr = _two(residual, "residual")
+    if hidden is not None:
+        want(ctx, hidden, "hidden", torch.float32)
+        ldh = _two(hidden, "hidden")
+    if (ldr and residual.shape != x.shape) or (ldh and hidden.shape != x.shape):
+        raise ValueError("residual and hidden must have x's shape")
     ld = -(-cols // 16) * 16
-    codes = torch.empty(rows, ld, dtype=torch.int8, device=x.device)[:, :cols]
-    scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    codes = x.new_empty((rows, ld), dtype=torch.int8)
+    if ld != cols:
+        codes = codes[:, :cols]
+    scales = x.new_empty(rows, dtype=torch.float32)
     if rows:
         launch(ctx, "kl_norm_q8", ctx.h, x.data_ptr(),
-               _lib.DTYPE_BF16 if x.dtype == torch.bfloat16 else _lib.DTYPE_F32, _ld(x),
-               None if residual is None else residual.data_ptr(), 0 if residual is None else _ld(residual),
+               _lib.DTYPE_BF16 if x.dtype == torch.bfloat16 else _lib.DTYPE_F32, ldx,
+               None if residual is None else residual.data_ptr(), ldr,
                None if weight is None else weight.data_ptr(), rows, cols, eps, norm, int(one_plus),
-               None if hidden is None else hidden.data_ptr(), 0 if hidden is None else _ld(hidden),
+               None if hidden is None else hidden.data_ptr(), ldh,
                codes.data_ptr(), ld, scales.data_ptr())
     return Q8Rows(codes, scales, hidden)
 
@@ -75,7 +81,7 @@ def add_rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tenso
     update the residual stream in place; by default, with a residual, a new
     tensor.  A row that is not finite gets scale NaN."""
     if hidden is None and residual is not None:
-        hidden = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+        hidden = x.new_empty(x.shape, dtype=torch.float32)
     return _rows_q8(x, weight, residual, eps, 1, one_plus_weight, hidden, ctx)
 
 
@@ -94,7 +100,7 @@ class Q8Linear:
         self.ctx = ctx or default_context()
         self.lib = self.ctx.lib
         want(self.ctx, codes, "codes", torch.int8)
-        _two(codes, "codes")
+        ld = _two(codes, "codes")
         self.out_features, self.in_features = codes.shape
         for t, name in ((scales, "scales"), (bias, "bias")):
             if t is not None:
@@ -103,7 +109,7 @@ class Q8Linear:
                     raise ValueError(f"{name} must be contiguous, one for each output")
         h = C.c_void_p()
         launch(self.ctx, "kl_q8_linear_create", self.ctx.h, self.in_features, self.out_features, codes.data_ptr(),
-               _ld(codes), scales.data_ptr(), None if bias is None else bias.data_ptr(), C.byref(h))
+               ld, scales.data_ptr(), None if bias is None else bias.data_ptr(), C.byref(h))
         self.h = h
 
     @classmethod
@@ -128,11 +134,10 @@ class Q8Linear:
         f32; f32 or bf16 out, added to an f32 ``out`` with ``accumulate``."""
         want(self.ctx, codes, "codes", torch.int8)
         want(self.ctx, scales, "scales", torch.float32)
-        _two(codes, "codes")
+        ld = _two(codes, "codes")
         rows = codes.shape[0]
         if codes.shape[1] != self.in_features or scales.shape != (rows,) or not scales.is_contiguous():
             raise ValueError("codes must be [rows][in_features], scales contiguous, one for each row")
-        ld = _ld(codes)
         if rows == 1:
             ld = -(-ld // 16) * 16  # a single row has no next one
         if rows and (codes.data_ptr() % 16 or ld % 16):
@@ -142,13 +147,13 @@ class Q8Linear:
                 raise ValueError("accumulate needs out")
             if out_dtype not in (torch.float32, torch.bfloat16):
                 raise ValueError("out_dtype must be float32 or bfloat16")
-            out = torch.empty(rows, self.out_features, dtype=out_dtype, device=codes.device)
+            out = codes.new_empty((rows, self.out_features), dtype=out_dtype)
         want(self.ctx, out, "out", torch.float32 if accumulate else (torch.float32, torch.bfloat16))
-        _two(out, "out")
+        ldo = _two(out, "out")
         if out.shape != (rows, self.out_features):
             raise ValueError("out must be [rows][out_features]")
         if rows:
             launch(self.ctx, "kl_q8_linear_forward", self.h, codes.data_ptr(), ld, scales.data_ptr(), rows,
-                   out.data_ptr(), _lib.DTYPE_BF16 if out.dtype == torch.bfloat16 else _lib.DTYPE_F32, _ld(out),
+                   out.data_ptr(), _lib.DTYPE_BF16 if out.dtype == torch.bfloat16 else _lib.DTYPE_F32, ldo,
                    int(accumulate))
         return out
