@@ -17,7 +17,7 @@ namespace kl {
 namespace {
 
 constexpr int AT_W = 4;       // warps per block
-constexpr int AT_STAGES = 6;  // tiles of a warp's ring, refilled two at a time
+constexpr int AT_STAGES = 3;  // pairs of tiles of a warp's ring
 
 struct SplitPlan {
   int chunk;      // tokens per block, a multiple of 16 AT_W
@@ -33,7 +33,7 @@ __device__ __forceinline__ int page_col(const SplitPlan& p, int tile) {
 // Shared memory of a block: the rings, and where the warps join.
 template <int D, int NR>
 constexpr int split_smem() {
-  constexpr int ring = AT_W * AT_STAGES * kv4_tile_bytes(D), join = AT_W * 8 * NR * D * 4;
+  constexpr int ring = AT_W * AT_STAGES * 2 * kv4_tile_bytes(D), join = AT_W * 8 * NR * D * 4;
   return ring > join ? ring : join;
 }
 
@@ -89,16 +89,16 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
   constexpr int MT = D / 16;  // O^T fragments
   extern __shared__ __align__(128) unsigned char ring[];
   __shared__ uint64_t full[AT_W][AT_STAGES];
-  __shared__ int tile_ok[AT_W][AT_STAGES];
+  __shared__ int tile_ok[AT_W][AT_STAGES][2];
   __shared__ float2 ml[AT_W][8 * NR];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, group = a.q_heads / a.cache.kv_heads, ps = a.cache.page_size;
   const int chunk_id = blockIdx.x / p.row_tiles;
-  unsigned char* mine = ring + warp * AT_STAGES * TB;
-  if (lane < AT_STAGES) mbar_init(&full[warp][lane], 1);
+  unsigned char* mine = ring + warp * AT_STAGES * 2 * TB;
+  if (lane < AT_STAGES) mbar_init(&full[warp][lane], 2);
   fence_mbar_init();
   __syncthreads();
-  uint32_t used = 0;  // tiles that this warp has put through its ring
+  uint32_t used = 0;  // pairs of tiles that this warp has put through its ring
   const float log2e = 1.4426950408889634f;
 
   for (int b = blockIdx.z; b < a.seq.num_seqs; b += gridDim.z) {
@@ -114,29 +114,30 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
       const int chunk = max(p.chunk, (int)round_up(ceil_div(span, p.chunks), 16 * AT_W));
       const int k0 = min(hi, lo + chunk_id * chunk), k1 = max(k0, min(hi, k0 + chunk));
       const int t0 = k0 >> 4, tiles = (k1 - k0 + 15) >> 4;  // k0 is a multiple of 16 wherever tiles > 0
-      const int n = tiles > warp ? (tiles - warp + AT_W - 1) / AT_W : 0;  // this warp's tiles: warp, warp + AT_W, ...
+      // this warp's tiles are warp, warp + AT_W, ..; it takes them in pairs, for two chains of everything
+      const int mine_n = tiles > warp ? (tiles - warp + AT_W - 1) / AT_W : 0, n = (mine_n + 1) / 2;
 
       // ---- the ring's first fills: lane i takes the warp's tile i ----
       const int32_t* table = a.seq.table + b * a.seq.table_ld;
       const int tpp = a.cache.tiles_per_page;
       const int64_t page_bytes = (int64_t)a.cache.kv_heads * tpp * TB;
       const unsigned char* heads = a.cache.base + (int64_t)kvh * tpp * TB;
-      auto issue = [&](int i, int col, int32_t page) {  // by a lane
-        const uint32_t st = (used + i) % AT_STAGES;
+      auto issue = [&](int i, int col, int32_t page) {  // by a lane, for tile i; beyond the last: nothing to see
+        const uint32_t st = (used + (i >> 1)) % AT_STAGES;
         const int off = t0 + warp + i * AT_W - col * tpp;
-        const bool ok = page >= 0 && page < a.cache.num_pages;
-        tile_ok[warp][st] = ok;
+        const bool ok = i < mine_n && page >= 0 && page < a.cache.num_pages;
+        tile_ok[warp][st][i & 1] = ok;
         if (ok) {
           mbar_arrive_expect_tx(&full[warp][st], TB);
-          bulk_load(mine + st * TB, heads + page * page_bytes + off * TB, TB, &full[warp][st]);
+          bulk_load(mine + (2 * st + (i & 1)) * TB, heads + page * page_bytes + off * TB, TB, &full[warp][st]);
         } else {
-          atomicOr(a.err, DERR_BOUNDS);
+          if (i < mine_n) atomicOr(a.err, DERR_BOUNDS);
           mbar_arrive(&full[warp][st]);
         }
       };
-      if (lane < AT_STAGES && lane < n) {
-        const int col = page_col(p, t0 + warp + lane * AT_W);
-        issue(lane, col, table[col]);
+      if (lane < 2 * AT_STAGES && lane < 2 * n) {
+        const int col = lane < mine_n ? page_col(p, t0 + warp + lane * AT_W) : 0;
+        issue(lane, col, lane < mine_n ? table[col] : 0);
       }
 
       // ---- q: row g's dims [t D/4, (t+1) D/4), scaled by a power of two ----
@@ -204,18 +205,13 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
           lift[r][i] = -INFINITY;  // a score above this moves the row's reference
         }
       }
-      float down[NR][2], most[NR][2];  // 2^-E, and the largest weight that it keeps within f16's range
+      float down[NR][2];  // 2^-E of a row's weights; first so large that any that matters asks for another
 #pragma unroll
-      for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          down[r][u] = 1.f;
-          most[r][u] = 0.f;
-        }
+      for (int r = 0; r < NR; ++r) down[r][0] = down[r][1] = 8.507059e37f;  // 2^126
       // the refills' lanes, one for each of two tiles, have the next one's page at hand
-      int next = AT_STAGES + lane, next_col = 0;
+      int next = 2 * AT_STAGES + lane, next_col = 0;
       int32_t next_page = 0;
-      if (lane < 2 && next < n) {
+      if (lane < 2 && next < mine_n) {
         next_col = page_col(p, t0 + warp + next * AT_W);
         next_page = table[next_col];
       }
@@ -229,169 +225,176 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
             mbar_wait(&full[warp][(used + k) % AT_STAGES], ((used + k) / AT_STAGES) & 1u);
           break;
         }
-        const unsigned char* tile = mine + st * TB;
-        uint32_t kw[2][KW], ve[2][KW / 2], vo[2][KW / 2];
-        if (D == 128) {
+        const unsigned char* tile = mine + 2 * st * TB;
+        uint32_t ve[2][2][KW / 2], vo[2][2][KW / 2];
+        float x[2][NR][4], vs[2][2], vm[2][2];  // x[.][r][2 k + u]: key g + 8 k of the tile, row 2t + u
+        bool ok[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 k = *reinterpret_cast<const uint4*>(tile + h * 512 + lane * 16);
-            const uint4 v = *reinterpret_cast<const uint4*>(tile + CODES + h * 512 + lane * 16);
-            kw[h][0] = k.x; kw[h][1] = k.y; kw[h][KW - 2] = k.z; kw[h][KW - 1] = k.w;
-            ve[h][0] = v.x; ve[h][KW / 2 - 1] = v.y; vo[h][0] = v.z; vo[h][KW / 2 - 1] = v.w;
-          }
-        } else {
-          const uint4 k = *reinterpret_cast<const uint4*>(tile + lane * 16);
-          const uint4 v = *reinterpret_cast<const uint4*>(tile + CODES + lane * 16);
-          kw[0][0] = k.x; kw[0][1] = k.y; kw[1][0] = k.z; kw[1][1] = k.w;
-          ve[0][0] = v.x; vo[0][0] = v.y; ve[1][0] = v.z; vo[1][0] = v.w;
-        }
-        const uint2 pr[2] = {*reinterpret_cast<const uint2*>(tile + 2 * CODES + g * 8),
-                             *reinterpret_cast<const uint2*>(tile + 2 * CODES + (g + 8) * 8)};
-        const bool ok = tile_ok[warp][st];
-        if (i & 1) {  // two stages have been read: they are filled again
-          __syncwarp();
-          if (lane < 2 && next < n) {
-            issue(next, next_col, next_page);
-            next += 2;
-            if (next < n) {
-              next_col = page_col(p, t0 + warp + next * AT_W);
-              next_page = table[next_col];
+        for (int c = 0; c < 2; ++c, tile += TB) {
+          uint32_t kw[2][KW];
+          if (D == 128) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint4 k = *reinterpret_cast<const uint4*>(tile + h * 512 + lane * 16);
+              const uint4 v = *reinterpret_cast<const uint4*>(tile + CODES + h * 512 + lane * 16);
+              kw[h][0] = k.x; kw[h][1] = k.y; kw[h][KW - 2] = k.z; kw[h][KW - 1] = k.w;
+              ve[c][h][0] = v.x; ve[c][h][KW / 2 - 1] = v.y; vo[c][h][0] = v.z; vo[c][h][KW / 2 - 1] = v.w;
             }
+          } else {
+            const uint4 k = *reinterpret_cast<const uint4*>(tile + lane * 16);
+            const uint4 v = *reinterpret_cast<const uint4*>(tile + CODES + lane * 16);
+            kw[0][0] = k.x; kw[0][1] = k.y; kw[1][0] = k.z; kw[1][1] = k.w;
+            ve[c][0][0] = v.x; vo[c][0][0] = v.y; ve[c][1][0] = v.z; vo[c][1][0] = v.w;
           }
-        }
-        if (!ok) continue;
-
-        float x[NR][4], x2[NR][4];  // two chains of products
+          ok[c] = tile_ok[warp][st][c];
+          uint2 pr[2] = {*reinterpret_cast<const uint2*>(tile + 2 * CODES + g * 8),
+                         *reinterpret_cast<const uint2*>(tile + 2 * CODES + (g + 8) * 8)};
+          if (!ok[c]) pr[0] = pr[1] = make_uint2(0, 0);
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+          for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) x[r][u] = x2[r][u] = 0.f;
+            for (int u = 0; u < 4; ++u) x[c][r][u] = 0.f;
 #pragma unroll
-        for (int w = 0; w < KW; ++w)
+          for (int w = 0; w < KW; ++w)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t u0 = kw[0][w] >> (8 * h), u1 = kw[1][w] >> (8 * h);
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t u0 = kw[0][w] >> (8 * h), u1 = kw[1][w] >> (8 * h);
+#pragma unroll
+              for (int r = 0; r < NR; ++r)
+                mma_f16(x[c][r], u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u,
+                        qf[r][2 * w + h][0], qf[r][2 * w + h][1]);
+            }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float ks = __uint_as_float(pr[k].x << 16);
+            float km = __uint_as_float(pr[k].x & 0xffff0000u);
+            vs[c][k] = __uint_as_float(pr[k].y << 16);
+            vm[c][k] = __uint_as_float(pr[k].y & 0xffff0000u);
+            // a value that is NaN makes the score NaN for whoever sees it, and is nothing to the others
+            if (vm[c][k] != vm[c][k]) {
+              km = vm[c][k];
+              vm[c][k] = 0.f;
+            }
 #pragma unroll
             for (int r = 0; r < NR; ++r)
-              mma_f16(h ? x2[r] : x[r], u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qf[r][2 * w + h][0],
-                      qf[r][2 * w + h][1]);
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                x[c][r][2 * k + u] = fmaf(x[c][r][2 * k + u] * ks, f[r][u], km * qs[r][u]);
           }
-        // x[r][2 k + i]: key g + 8 k, row 2t + i
-        float vs[2], vm[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float ks = __uint_as_float(pr[k].x << 16), km = __uint_as_float(pr[k].x & 0xffff0000u);
-          vs[k] = __uint_as_float(pr[k].y << 16);
-          vm[k] = __uint_as_float(pr[k].y & 0xffff0000u);
-#pragma unroll
-          for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) x[r][2 * k + u] = fmaf((x[r][2 * k + u] + x2[r][2 * k + u]) * ks, f[r][u], km * qs[r][u]);
         }
-        const int j0 = (t0 + warp + i * AT_W) * 16;
-        const bool partial = j0 + 15 > see_all_to || j0 < see_all_from;
-        uint32_t unseen = 0;
-        if (partial) {
+        __syncwarp();  // the stage has been read: it is filled again
+        if (lane < 2 && i + AT_STAGES < n) {
+          issue(next, next_col, next_page);
+          next += 2;
+          if (next < mine_n) {
+            next_col = page_col(p, t0 + warp + next * AT_W);
+            next_page = table[next_col];
+          }
+        }
+
+        const int j0 = (t0 + warp + 2 * i * AT_W) * 16;  // the first tile's first key; the second's is 16 AT_W on
+        if (j0 + 16 * AT_W + 15 > see_all_to || j0 < see_all_from || !ok[0] || !ok[1]) {
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int j = j0 + g + 8 * (u >> 1), q = pos[r][u & 1];
-              if (j > q || (a.window > 0 && j <= q - a.window)) {
-                x[r][u] = -INFINITY;
-                unseen |= 1u << (4 * r + u);
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const int j = j0 + c * 16 * AT_W + g + 8 * (u >> 1), q = pos[r][u & 1];
+                if (!ok[c] || j > q || (a.window > 0 && j <= q - a.window)) x[c][r][u] = -INFINITY;
               }
-            }
         }
+        float top[NR][2];
         bool up = false;
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) up = up || x[r][u] > lift[r][u] || x[r][2 + u] > lift[r][u];
+          for (int u = 0; u < 2; ++u) {
+            top[r][u] = fmaxf(fmaxf(x[0][r][u], x[0][r][2 + u]), fmaxf(x[1][r][u], x[1][r][2 + u]));
+            up = up || top[r][u] > lift[r][u];
+          }
         if (__any_sync(FULL, up)) {
           // move the references to the maxima seen so far (a probability is at most 2^8 until the next move)
 #pragma unroll
           for (int r = 0; r < NR; ++r)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              float top = fmaxf(x[r][u], x[r][2 + u]);
 #pragma unroll
-              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
-              if (top > lift[r][u] - 8.f || lift[r][u] == -INFINITY) {
-                const bool none = lift[r][u] == -INFINITY;
-                const float now = none ? top : fmaxf(top, ref[r][u]);
-                if (now != -INFINITY) {
-                  const float keep = none ? 0.f : exp2f(ref[r][u] - now);
-                  // sums taken with no finite score so far are NaN or zero: both stay what they are
-                  l[r][u] *= none ? 1.f : keep;
-                  vb[r][u] *= none ? 1.f : keep;
+              for (int d = 4; d < 32; d <<= 1) top[r][u] = fmaxf(top[r][u], __shfl_xor_sync(FULL, top[r][u], d));
+              const bool none = lift[r][u] == -INFINITY;
+              if ((top[r][u] > ref[r][u] || none) && top[r][u] != -INFINITY) {
+                // sums taken with no finite score so far are NaN or zero: both stay what they are
+                const float keep = none ? 1.f : exp2f(ref[r][u] - top[r][u]);
+                l[r][u] *= keep;
+                vb[r][u] *= keep;
 #pragma unroll
-                  for (int m = 0; m < MT; ++m) {
-                    o[m][r][u] *= none ? 1.f : keep;
-                    o[m][r][2 + u] *= none ? 1.f : keep;
-                  }
-                  ref[r][u] = now;
-                  lift[r][u] = now + 8.f;
+                for (int m = 0; m < MT; ++m) {
+                  o[m][r][u] *= keep;
+                  o[m][r][2 + u] *= keep;
                 }
+                ref[r][u] = top[r][u];
+                lift[r][u] = top[r][u] + 8.f;
               }
             }
         }
-        float w[NR][4];
         bool heavy = false;
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const float y = exp2_fast(x[r][u] - ref[r][u & 1]);
-            l[r][u & 1] += y;
-            w[r][u] = y * vs[u >> 1];
-            heavy = heavy || w[r][u] > most[r][u & 1];
-            if (!partial || !(unseen >> (4 * r + u) & 1u)) vb[r][u & 1] = fmaf(y, vm[u >> 1], vb[r][u & 1]);
-          }
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const float y = exp2_fast(x[c][r][u] - ref[r][u & 1]);
+              l[r][u & 1] += y;
+              vb[r][u & 1] = fmaf(y, vm[c][u >> 1], vb[r][u & 1]);
+              x[c][r][u] = y * vs[c][u >> 1];  // the weight of a code
+              heavy = heavy || x[c][r][u] * down[r][u & 1] > 32768.f;
+            }
         if (__any_sync(FULL, heavy)) {
 #pragma unroll
           for (int r = 0; r < NR; ++r)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              float top = fmaxf(w[r][u], w[r][2 + u]);
+              float most = fmaxf(fmaxf(x[0][r][u], x[0][r][2 + u]), fmaxf(x[1][r][u], x[1][r][2 + u]));
 #pragma unroll
-              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
-              if (top > most[r][u]) {  // E: this weight at 2^8; later ones may pass it by 2^7
-                const int e = max(-126, min(127, 8 - ((int)(__float_as_uint(top) >> 23) - 127)));
-                const float now = __uint_as_float((uint32_t)(e + 127) << 23);
-                const float keep = most[r][u] == 0.f ? 1.f : now / down[r][u];
+              for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(FULL, most, d));
+              if (most * down[r][u] > 32768.f) {  // E: this weight at 2^8; later ones may pass it by 2^7
+                const int e = max(-126, 8 - ((int)(__float_as_uint(most) >> 23) - 127));
+                const float now = __uint_as_float((uint32_t)(e + 127) << 23), keep = now / down[r][u];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                   o[m][r][u] *= keep;
                   o[m][r][2 + u] *= keep;
                 }
                 down[r][u] = now;
-                most[r][u] = 32768.f / now;
               }
             }
         }
-        uint32_t pb[NR][2];
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pb[NR][2];
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            pb[r][k] = transpose8(pack_f16(w[r][2 * k] * down[r][0], w[r][2 * k + 1] * down[r][1]));
+          for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int w = 0; w < KW / 2; ++w) {
-          uint32_t lo2[2], hi2[2];  // dims 0 2 4 6 and 1 3 5 7 of the word, tokens 2t and 2t + 1 side by side
+            for (int k = 0; k < 2; ++k)
+              pb[r][k] = transpose8(pack_f16(x[c][r][2 * k] * down[r][0], x[c][r][2 * k + 1] * down[r][1]));
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            lo2[h] = __byte_perm(ve[h][w], vo[h][w], 0x5410);
-            hi2[h] = __byte_perm(ve[h][w], vo[h][w], 0x7632);
-          }
+          for (int w = 0; w < KW / 2; ++w) {
+            uint32_t lo2[2], hi2[2];  // dims 0 2 4 6 and 1 3 5 7 of the word, tokens 2t and 2t + 1 side by side
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const uint32_t mask = d & 1 ? 0x00f000f0u : 0x000f000fu;
-            const int s = d & 2 ? 8 : 0;
+            for (int h = 0; h < 2; ++h) {
+              lo2[h] = __byte_perm(ve[c][h][w], vo[c][h][w], 0x5410);
+              hi2[h] = __byte_perm(ve[c][h][w], vo[c][h][w], 0x7632);
+            }
 #pragma unroll
-            for (int r = 0; r < NR; ++r)
-              mma_f16(o[4 * w + d][r], lo2[0] >> s & mask, hi2[0] >> s & mask, lo2[1] >> s & mask, hi2[1] >> s & mask,
-                      pb[r][0], pb[r][1]);
+            for (int d = 0; d < 4; ++d) {
+              const uint32_t mask = d & 1 ? 0x00f000f0u : 0x000f000fu;
+              const int s = d & 2 ? 8 : 0;
+#pragma unroll
+              for (int r = 0; r < NR; ++r)
+                mma_f16(o[4 * w + d][r], lo2[0] >> s & mask, hi2[0] >> s & mask, lo2[1] >> s & mask, hi2[1] >> s & mask,
+                        pb[r][0], pb[r][1]);
+            }
           }
         }
       }
