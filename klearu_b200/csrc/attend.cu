@@ -461,14 +461,17 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
   }
 }
 
-// One warp per (token, query head): the chunks' rows, brought to one reference
-// and summed in the chunks' order.
-template <int D>
-__global__ void __launch_bounds__(128) attend_join_kernel(AttendArgs a, int chunks) {
+// W warps per (token, query head): the chunks' rows, brought to one reference
+// and summed, each warp every W-th chunk, the warps in order.  One warp reads
+// 74 chunks in 19 us, a load's latency each; eight, four loads at a time, in 4.
+template <int D, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attend_join_kernel(AttendArgs a, int chunks) {
   constexpr int E = D / 32;
+  __shared__ float part[W][D];
+  __shared__ float sums[W];
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, me = W == 1 ? 0 : warp;
+  const int64_t i = W == 1 ? (int64_t)blockIdx.x * 4 + warp : (int64_t)blockIdx.x;
   if (i >= (int64_t)a.seq.num_tokens * a.q_heads) return;
   const int64_t tok = i / a.q_heads;
   const int head = (int)(i % a.q_heads);
@@ -482,13 +485,44 @@ __global__ void __launch_bounds__(128) attend_join_kernel(AttendArgs a, int chun
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
   const float rf = top == -INFINITY ? 0.f : top;
   float sum = 0.f, acc[E] = {};
-  for (int c = 0; c < chunks; ++c) {
-    const float2 v = ml[c * step];
-    if (v.y == 0.f) continue;  // saw nothing
-    const float keep = exp2f(v.x - rf);
-    sum = fmaf(keep, v.y, sum);
+  for (int c0 = me; c0 < chunks; c0 += 4 * W) {
+    float2 v[4];
+    float r[4][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(keep, rows[c * step * D + e], acc[e]);
+    for (int u = 0; u < 4; ++u) {
+      const int c = c0 + u * W;
+      v[u] = c < chunks ? ml[c * step] : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        // a chunk that saw nothing wrote no row
+        const float2 x = v[u].y != 0.f ? *reinterpret_cast<const float2*>(rows + c * step * D + e) : make_float2(0.f, 0.f);
+        r[u][e] = x.x;
+        r[u][e + 1] = x.y;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float keep = v[u].y != 0.f ? exp2f(v[u].x - rf) : 0.f;
+      sum = fmaf(keep, v[u].y, sum);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(keep, r[u][e], acc[e]);
+    }
+  }
+  if (W > 1) {
+    if (lane == 0) sums[me] = sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[me][lane * E + e] = acc[e];
+    __syncthreads();
+    if (warp > 0) return;
+    sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      sum += sums[w];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += part[w][lane * E + e];
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.p) + tok * a.out.token + head * a.out.head + lane * E;
@@ -533,16 +567,20 @@ void launch_split(const AttendArgs& a, const SplitPlan& p, cudaStream_t st) {
   attend_split_kernel<D, NR><<<grid, AT_W * 32, split_smem<D, NR>(), st>>>(a, p);
   count_launch();
   if (p.chunks == 1) return;
+  // eight warps to a row where the rows are few enough for one turn of the machine, or the chunks many
+  const int64_t rows = (int64_t)a.seq.num_tokens * a.q_heads;
+  const bool wide = p.chunks > 4 && (rows <= 1024 || p.chunks > 16);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ceil_div((int64_t)a.seq.num_tokens * a.q_heads, 4));
-  cfg.blockDim = 128;
+  cfg.gridDim = dim3((unsigned)(wide ? rows : ceil_div(rows, 4)));
+  cfg.blockDim = wide ? 256 : 128;
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, a, p.chunks);
+  if (wide) cudaLaunchKernelEx(&cfg, attend_join_kernel<D, 8>, a, p.chunks);
+  else cudaLaunchKernelEx(&cfg, attend_join_kernel<D, 1>, a, p.chunks);
   count_launch();
 }
 
