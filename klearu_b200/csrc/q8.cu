@@ -16,14 +16,33 @@ namespace {
 
 __device__ __forceinline__ bool finite32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
+__device__ __forceinline__ float norm_weight(const NormQ8Args& a, int c) {
+  return a.weight ? (a.one_plus ? 1.f + a.weight[c] : a.weight[c]) : 1.f;
+}
+__device__ __forceinline__ void norm_weights8(const NormQ8Args& a, int c, float* w) {
+  if (!a.weight) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 1.f;
+    return;
+  }
+  *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(a.weight + c);
+  *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(a.weight + c + 4);
+  if (a.one_plus) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 1.f + w[i];
+  }
+}
 // rint(127 u / top) for u = h * w in 64 bits.  The f32 quotient decides unless
 // it is within 1e-4 of a border between two codes (its own error is below
 // 3 roundings of 127, 2.3e-5): only then are the 64-bit product and quotient
 // taken, so the codes are those of the definition.
+__device__ __noinline__ int q8_exact(float h, float w, double top) {
+  return (int)rint((double)h * (double)w * 127.0 / top);
+}
 __device__ __forceinline__ int q8_code(float h, float w, float p, float inv, double top) {
   const float t = p * inv;
   const float r = rintf(t);
-  if (fabsf(fabsf(t - r) - 0.5f) < 1e-4f) return (int)rint((double)h * (double)w * 127.0 / top);
+  if (fabsf(fabsf(t - r) - 0.5f) < 1e-4f) return q8_exact(h, w, top);
   return (int)r;
 }
 
@@ -43,8 +62,117 @@ __device__ __forceinline__ float block_reduce(float v, float* tmp, bool is_max) 
   return v;
 }
 
-// One block per row; the row's h waits in shared memory between the pass that
-// finds its sum of squares and maximum and the pass that writes the codes.
+// One block per row, a row's 8 NV blockDim values in registers, 16 bytes and
+// more a load; one pass over memory.
+template <int NV, class T>
+__global__ void __launch_bounds__(1024) norm_q8_vec_kernel(NormQ8Args a) {
+  __shared__ float2 tmp[32];
+  __shared__ unsigned long long top_s;
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const float* r = a.residual ? a.residual + row * a.ldr : nullptr;
+  float* ho = a.hidden ? a.hidden + row * a.ldh : nullptr;
+  float h[NV][8], p[NV][8], ss = 0.f, mx = 0.f;
+  bool fin = true;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * blockDim.x + threadIdx.x) * 8;
+    if (c < a.cols) {
+      if (sizeof(T) == 2) {
+        const uint4 u = *reinterpret_cast<const uint4*>(x + c);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          h[v][2 * i] = __uint_as_float(w[i] << 16);
+          h[v][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      } else {
+        *reinterpret_cast<float4*>(&h[v][0]) = *reinterpret_cast<const float4*>(x + c);
+        *reinterpret_cast<float4*>(&h[v][4]) = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + c + 4);
+      }
+      if (r) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const float4 y = *reinterpret_cast<const float4*>(r + c + i);
+          h[v][i] += y.x;
+          h[v][i + 1] += y.y;
+          h[v][i + 2] += y.z;
+          h[v][i + 3] += y.w;
+        }
+      }
+      if (ho) {
+        *reinterpret_cast<float4*>(ho + c) = make_float4(h[v][0], h[v][1], h[v][2], h[v][3]);
+        *reinterpret_cast<float4*>(ho + c + 4) = make_float4(h[v][4], h[v][5], h[v][6], h[v][7]);
+      }
+      float w8[8];
+      norm_weights8(a, c, w8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[v][i] = h[v][i] * w8[i];
+        fin = fin && finite32(p[v][i]) && finite32(h[v][i]);
+        ss = fmaf(h[v][i], h[v][i], ss);
+        mx = fmaxf(mx, fabsf(p[v][i]));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[v][i] = p[v][i] = 0.f;
+    }
+  }
+  mx = fin ? mx : INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ss += __shfl_xor_sync(FULL, ss, o);
+    mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
+  }
+  const int warps = blockDim.x >> 5;
+  if ((threadIdx.x & 31) == 0) tmp[threadIdx.x >> 5] = make_float2(ss, mx);
+  if (threadIdx.x == 0) top_s = 0ull;
+  __syncthreads();
+  const float2 of = (int)(threadIdx.x & 31) < warps ? tmp[threadIdx.x & 31] : make_float2(0.f, 0.f);
+  ss = of.x;
+  mx = of.y;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ss += __shfl_xor_sync(FULL, ss, o);
+    mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
+  }
+  // the largest |h w| in 64 bits is among those whose f32 product is largest
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (fabsf(p[v][i]) == mx && c < a.cols)
+        atomicMax(&top_s, (unsigned long long)__double_as_longlong(fabs((double)h[v][i] * (double)norm_weight(a, c + i))));
+  }
+  __syncthreads();
+  const double top = __longlong_as_double((long long)top_s);
+  const float rinv = a.norm ? 1.f / sqrtf(ss / (float)a.cols + a.eps) : 1.f;
+  const bool good = finite32(mx) && finite32(ss);
+  if (threadIdx.x == 0) a.scales[row] = good ? mx * rinv / 127.f : __int_as_float(0x7fffffff);
+  const float inv = good && mx > 0.f ? 127.f / mx : 0.f;
+  int8_t* co = a.codes + row * a.ldc;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * blockDim.x + threadIdx.x) * 8;
+    if (c >= a.cols) continue;
+    uint32_t out[2] = {0, 0};
+    if (inv > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float t = p[v][i] * inv, b = t + 12582912.f;  // 1.5 * 2^23: rounds to a whole number, in the low bits
+        int code = (int)__float_as_uint(b);
+        if (fabsf(fabsf(t - (b - 12582912.f)) - 0.5f) < 1e-4f) code = q8_exact(h[v][i], norm_weight(a, c + i), top);
+        out[i >> 2] |= (uint32_t)(code & 255) << (8 * (i & 3));
+      }
+    }
+    *reinterpret_cast<uint2*>(co + c) = make_uint2(out[0], out[1]);
+  }
+}
+
+// The same for any alignment and width: the row's h waits in shared memory
+// between the pass that finds its sum of squares and maximum and the pass that
+// writes the codes.
 template <int NT, class T>
 __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
   extern __shared__ float nq_h[];
@@ -62,7 +190,7 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
     if (r) h += r[i];
     if (ho) ho[i] = h;
     nq_h[i] = h;
-    const float w = a.weight ? (a.one_plus ? 1.f + a.weight[i] : a.weight[i]) : 1.f;
+    const float w = norm_weight(a, i);
     const float p = h * w;
     fin = fin && finite32(p) && finite32(h);
     ss = fmaf(h, h, ss);
@@ -72,7 +200,7 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
   mx = block_reduce<NT>(fin ? mx : INFINITY, tmp, true);
   // the largest |h w| in 64 bits is among those whose f32 product is largest
   for (int i = threadIdx.x; i < a.cols; i += NT) {
-    const float w = a.weight ? (a.one_plus ? 1.f + a.weight[i] : a.weight[i]) : 1.f;
+    const float w = norm_weight(a, i);
     if (fabsf(nq_h[i] * w) == mx)
       atomicMax(&top_s, (unsigned long long)__double_as_longlong(fabs((double)nq_h[i] * (double)w)));
   }
@@ -84,7 +212,7 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
   const float inv = good && mx > 0.f ? 127.f / mx : 0.f;
   int8_t* co = a.codes + row * a.ldc;
   for (int i = threadIdx.x; i < a.cols; i += NT) {
-    const float w = a.weight ? (a.one_plus ? 1.f + a.weight[i] : a.weight[i]) : 1.f;
+    const float w = norm_weight(a, i);
     co[i] = inv > 0.f ? (int8_t)q8_code(nq_h[i], w, nq_h[i] * w, inv, top) : (int8_t)0;
   }
 }
@@ -240,7 +368,8 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
     for (int j = rank; j < rows; j += splits) {
       int acc = 0;
       const uint32_t at = smem_u32(part + j * 128 + threadIdx.x);
-      for (int r = 0; r < splits; ++r) acc += ld_cluster(at, (uint32_t)r);
+#pragma unroll 8
+      for (int r = 0; r < 8; ++r) acc += r < splits ? ld_cluster(at, (uint32_t)r) : 0;
       if (c < a.n) q8_store(a, row + j, c, q8_value(a, acc, a.a_scale[row + j], sw, bias));
     }
     __syncwarp();
@@ -350,6 +479,71 @@ int q8_sms() {
   return n;
 }
 
+// Up to four rows: every warp streams pairs of channels' weights, four 16-byte
+// loads of each in flight per lane, against the rows in shared memory, four
+// products an instruction.  No ring, tensor memory or join to set up: with one
+// row and 50 MB of weights that is 5 of 16 us.
+constexpr int Q8_VW = 4;  // warps per block
+template <int M>
+__global__ void __launch_bounds__(Q8_VW * 32) q8_vector_kernel(Q8Args a) {
+  extern __shared__ __align__(16) int8_t q8_rows[];  // [M][ldw], zero from k on as the weights are
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = (blockIdx.x * Q8_VW + warp) * 2;
+  const int8_t* w0 = a.w + (int64_t)min(c0, a.n - 1) * a.ldw;
+  const int8_t* w1 = a.w + (int64_t)min(c0 + 1, a.n - 1) * a.ldw;
+  const int words = (int)(a.ldw >> 4);  // of 16 bytes
+  uint4 x[2][4];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = at + u * 32 + lane;
+      x[0][u] = i < words ? __ldcs(reinterpret_cast<const uint4*>(w0) + i) : make_uint4(0, 0, 0, 0);
+      x[1][u] = i < words ? __ldcs(reinterpret_cast<const uint4*>(w1) + i) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  load(0);  // the first weights on their way while the rows are staged
+  for (int i = threadIdx.x; i < M * words; i += Q8_VW * 32) {
+    const int r = i / words, at = (i - r * words) * 16;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (at + 16 <= a.k) {
+      v = *reinterpret_cast<const uint4*>(a.a + r * a.lda + at);
+    } else if (at < a.k) {
+      uint32_t b[4] = {0, 0, 0, 0};
+      for (int e = 0; at + e < a.k; ++e) b[e >> 2] |= (uint32_t)(uint8_t)a.a[r * a.lda + at + e] << (8 * (e & 3));
+      v = make_uint4(b[0], b[1], b[2], b[3]);
+    }
+    reinterpret_cast<uint4*>(q8_rows)[i] = v;
+  }
+  __syncthreads();
+  int acc[M][2] = {};
+  for (int at = 0; at < words; at += 128) {
+    if (at > 0) load(at);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = min(at + u * 32 + lane, words - 1);  // beyond the end the weights are zero
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const uint4 y = reinterpret_cast<const uint4*>(q8_rows)[m * words + i];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          acc[m][c] = __dp4a((int)x[c][u].x, (int)y.x, acc[m][c]);
+          acc[m][c] = __dp4a((int)x[c][u].y, (int)y.y, acc[m][c]);
+          acc[m][c] = __dp4a((int)x[c][u].z, (int)y.z, acc[m][c]);
+          acc[m][c] = __dp4a((int)x[c][u].w, (int)y.w, acc[m][c]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int sum = warp_sum(acc[m][c]);
+      if (lane == 0 && c0 + c < a.n)
+        q8_store(a, m, c0 + c, q8_value(a, sum, a.a_scale[m], a.w_scale[c0 + c], a.bias ? a.bias[c0 + c] : 0.f));
+    }
+}
+
 __global__ void q8_pack_kernel(const int8_t* src, int64_t ld, int k, int8_t* dst, int64_t ldw) {
   const int64_t r = blockIdx.y;
   const int c = blockIdx.x * blockDim.x + threadIdx.x;
@@ -358,7 +552,28 @@ __global__ void q8_pack_kernel(const int8_t* src, int64_t ld, int k, int8_t* dst
 
 }  // namespace
 
+// Vectors where the weights and every row start on 16 bytes (codes 8) and cols is a multiple of
+// 8 up to 16384: 8 values a thread while the rows do not fill the machine, 16
+// where they do (fewer threads to wait for at the two barriers).
+static bool norm_vec(const NormQ8Args& a) {
+  auto on = [](const void* p, int64_t ld, int size, int to) {
+    return !p || (reinterpret_cast<uintptr_t>(p) % to == 0 && ld * size % to == 0);
+  };
+  return a.cols % 8 == 0 && a.cols <= 16384 && on(a.x, a.ldx, a.x_bf16 ? 2 : 4, 16) && on(a.residual, a.ldr, 4, 16) &&
+         on(a.hidden, a.ldh, 4, 16) && on(a.codes, a.ldc, 1, 8) && on(a.weight, 0, 4, 16);
+}
 void launch_norm_q8(const NormQ8Args& a, int rows, cudaStream_t st) {
+  if (norm_vec(a)) {
+    const bool two = a.cols > 8192 || rows > 296;
+    const int threads = (int)round_up(ceil_div(a.cols, two ? 16 : 8), 32);
+    if (a.x_bf16)
+      two ? norm_q8_vec_kernel<2, __nv_bfloat16><<<rows, threads, 0, st>>>(a)
+          : norm_q8_vec_kernel<1, __nv_bfloat16><<<rows, threads, 0, st>>>(a);
+    else
+      two ? norm_q8_vec_kernel<2, float><<<rows, threads, 0, st>>>(a) : norm_q8_vec_kernel<1, float><<<rows, threads, 0, st>>>(a);
+    count_launch();
+    return;
+  }
   static OncePerDevice once;
   once([] {
     cudaFuncSetAttribute(norm_q8_kernel<256, float>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_Q8_MAX_COLS * 4);
@@ -377,9 +592,9 @@ void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, in
         src + r * ld, ld, k, dst + r * ldw, ldw), count_launch();
 }
 
-// Rows per tile and splits of K for few tiles.  A block streams its share of
-// the weights at the memory's rate and pays about as much again as 64 KB of
-// them for filling its ring and joining; two blocks fit an SM up to 64 rows.
+// Rows per tile and splits of K for few tiles: the blocks that an SM takes share
+// its bandwidth, so the most that one SM streams is what counts, and each split
+// adds about 24 KB worth of filling and joining.
 struct Q8Plan {
   bool persistent;
   int nt, splits;
@@ -387,16 +602,14 @@ struct Q8Plan {
 static Q8Plan q8_plan(const Q8Args& a) {
   const int sms = q8_sms();
   const int ch = (int)ceil_div(a.n, 128), kc = (int)ceil_div(a.k, Q8_KB);
-  int nt = 16;
-  while (nt < 256 && nt < a.m) nt *= 2;
+  const int nt = (int)std::min<int64_t>(256, round_up(a.m, 16));
   const int64_t tiles = ceil_div(a.m, nt) * ch;
   if (nt == 256 && tiles >= 2 * sms) return {true, 256, 1};
   Q8Plan best{false, nt, 1};
   double least = 1e30;
-  const int resident = sms * (nt <= 64 ? 2 : 1);
-  for (int s = 1; s <= 8 && s <= std::max(1, kc); s *= 2) {
+  for (int s = 1; s <= 8 && s <= std::max(1, kc); ++s) {
     const double bytes = (double)ceil_div(kc, s) * (Q8_WTILE + nt * Q8_KB);
-    const double cost = (double)ceil_div(tiles * s, resident) * (bytes + (s > 1 ? 96.0 : 64.0) * 1024);
+    const double cost = (double)ceil_div(tiles * s, sms) * bytes + s * 24.0 * 1024;
     if (cost < least) {
       least = cost;
       best.splits = s;
@@ -411,6 +624,19 @@ bool launch_q8_matmul(const Q8Args& a, cudaStream_t st) {
     cudaFuncSetAttribute(q8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
     cudaFuncSetAttribute(q8_persistent_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
   });
+  // four rows at most, their codes within the 48 KB of shared memory that leave an SM four blocks
+  if (a.m <= 4 && a.m * a.ldw <= 48 * 1024) {
+    const unsigned grid = (unsigned)ceil_div(a.n, 2 * Q8_VW);
+    const size_t sm = (size_t)(a.m * a.ldw);
+    switch (a.m) {
+      case 1: q8_vector_kernel<1><<<grid, Q8_VW * 32, sm, st>>>(a); break;
+      case 2: q8_vector_kernel<2><<<grid, Q8_VW * 32, sm, st>>>(a); break;
+      case 3: q8_vector_kernel<3><<<grid, Q8_VW * 32, sm, st>>>(a); break;
+      default: q8_vector_kernel<4><<<grid, Q8_VW * 32, sm, st>>>(a); break;
+    }
+    count_launch();
+    return true;
+  }
   const Q8Plan p = q8_plan(a);
   const int kc = (int)ceil_div(a.k, Q8_KB), stage = Q8_WTILE + p.nt * Q8_KB;
   CUtensorMap wm, am;
