@@ -254,12 +254,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-__device__ __forceinline__ int ld_cluster(uint32_t saddr, uint32_t rank) {
+__device__ __forceinline__ void st_cluster(uint32_t saddr, uint32_t rank, int v) {
   uint32_t p;
-  int v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(p) : "r"(saddr), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(p) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.s32 [%0], %1;\n" ::"r"(p), "r"(v) : "memory");
 }
 
 // The TMA side of a tile: K chunks [c0, c1) through the ring; q counts chunks
@@ -299,10 +297,10 @@ __device__ __forceinline__ void q8_drain(const Q8Tile& t, uint64_t* full, uint32
     mbar_wait(&full[r % t.stages], (r / t.stages) & 1u);
 }
 
-// Few tiles: one tile per cluster, its K split over the cluster's blocks; the
-// 32-bit sums of the others are read over distributed shared memory (whole
-// numbers: any order gives the same sum), each block finishing its share of
-// the tile's rows.  One launch, no workspace.
+// Few tiles: one tile per cluster, its K split over the cluster's blocks; each
+// block finishes a share of the tile's rows, for which the others store their
+// 32-bit sums in its shared memory (whole numbers: any order gives the same
+// sum).  One launch, no workspace.
 __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ CUtensorMap wm,
                                                        const __grid_constant__ CUtensorMap am, Q8Args a, Q8Tile t,
                                                        int splits) {
@@ -310,6 +308,7 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
   __shared__ uint64_t full[12], empty[12], done;
   __shared__ uint32_t tmem_s;
   __shared__ int fail;
+  __shared__ float sa[256];  // the tile's row scales: read between stores to out, they must not wait for memory
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(q8_dyn) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = splits > 1 ? (int)cluster_rank() : 0;
@@ -324,6 +323,7 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
     fail = 0;
     fence_mbar_init();
   }
+  for (int j = threadIdx.x; j < t.nt; j += 128) sa[j] = row + j < a.m ? a.a_scale[row + j] : 0.f;
   if (warp == 1) tc5_alloc(&tmem_s, t.tmem_cols);
   tc5_fence_before();
   __syncthreads();
@@ -352,28 +352,35 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
       tc5_ld_wait();
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (c < a.n && j + i < rows) q8_store(a, row + j + i, c, q8_value(a, (int)v[i], a.a_scale[row + j + i], sw, bias));
+        if (c < a.n && j + i < rows) q8_store(a, row + j + i, c, q8_value(a, (int)v[i], sa[j + i], sw, bias));
     }
   } else {
-    int* part = reinterpret_cast<int*>(sm);  // [row][channel]; the ring has no copy in flight and no MMA reads it
+    // Row j is finished by block j % splits: each block stores its sums of that row there, [from][j / splits][channel],
+    // over the ring, which no copy or MMA uses any more once all blocks are here.
+    const uint32_t part = smem_u32(sm);
+    const int each = (t.nt + splits - 1) / splits;
+    __syncwarp();
+    cluster_sync();
     for (int j = 0; j < rows; j += 16) {
       uint32_t v[16];
       tc5_ld16_async(mine + j, v);
       tc5_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) part[(j + i) * 128 + threadIdx.x] = c0 < c1 ? (int)v[i] : 0;
+      for (int i = 0; i < 16; ++i) {
+        const int to = (j + i) % splits, slot = (j + i) / splits;
+        if (j + i < rows)
+          st_cluster(part + (uint32_t)(((rank * each + slot) * 128 + (int)threadIdx.x) * 4), (uint32_t)to, (int)v[i]);
+      }
     }
     __syncwarp();
     cluster_sync();
+    const int* sums = reinterpret_cast<const int*>(sm);
+#pragma unroll 4
     for (int j = rank; j < rows; j += splits) {
       int acc = 0;
-      const uint32_t at = smem_u32(part + j * 128 + threadIdx.x);
-#pragma unroll 8
-      for (int r = 0; r < 8; ++r) acc += r < splits ? ld_cluster(at, (uint32_t)r) : 0;
-      if (c < a.n) q8_store(a, row + j, c, q8_value(a, acc, a.a_scale[row + j], sw, bias));
+      for (int r = 0; r < splits; ++r) acc += sums[(r * each + j / splits) * 128 + threadIdx.x];
+      if (c < a.n) q8_store(a, row + j, c, q8_value(a, acc, sa[j], sw, bias));
     }
-    __syncwarp();
-    cluster_sync();  // the other blocks may still read this one's sums
   }
   tc5_fence_before();
   __syncthreads();
@@ -392,6 +399,7 @@ __global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_c
   __shared__ uint64_t full[12], empty[12], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_s;
   __shared__ int fail;
+  __shared__ float sa[4][Q8_PN];  // each writing warp's copy of its tile's row scales
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(q8_dyn) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -444,7 +452,10 @@ __global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_c
       const int c = i % ch_tiles * 128 + quad * 32 + lane, row = i / ch_tiles * Q8_PN;
       const int rows = min(Q8_PN, a.m - row);
       const float sw = c < a.n ? a.w_scale[c] : 0.f, bias = a.bias && c < a.n ? a.bias[c] : 0.f;
-      if (*vf || !mbar_wait(&acc_full[b], (uint32_t)(n / 2) & 1u)) {
+      __syncwarp();
+      for (int j = lane; j < Q8_PN; j += 32) sa[quad][j] = row + j < a.m ? a.a_scale[row + j] : 0.f;
+      __syncwarp();
+      if (__any_sync(FULL, *vf || !mbar_wait(&acc_full[b], (uint32_t)(n / 2) & 1u))) {
         atomicExch(&fail, 1);
         break;
       }
@@ -456,7 +467,7 @@ __global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_c
 #pragma unroll
         for (int u = 0; u < 16; ++u)
           if (c < a.n && j + u < rows)
-            q8_store(a, row + j + u, c, q8_value(a, (int)v[u], a.a_scale[row + j + u], sw, bias));
+            q8_store(a, row + j + u, c, q8_value(a, (int)v[u], sa[quad][j + u], sw, bias));
       }
       tc5_fence_before();
       __syncwarp();
@@ -592,9 +603,11 @@ void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, in
         src + r * ld, ld, k, dst + r * ldw, ldw), count_launch();
 }
 
-// Rows per tile and splits of K for few tiles: the blocks that an SM takes share
-// its bandwidth, so the most that one SM streams is what counts, and each split
-// adds about 24 KB worth of filling and joining.
+// Rows per tile and splits of K for few tiles.  A chunk of 128 bytes of K takes
+// an SM the longest of its weights at its share of the memory's rate (43 bytes a
+// ns with all SMs at it), its operands at the L2's (100), and its MMAs (1.1 ns a
+// row); each turn of blocks some 2 us to start and end, a split 1 us and 15 ns a
+// row to join.
 struct Q8Plan {
   bool persistent;
   int nt, splits;
@@ -602,18 +615,25 @@ struct Q8Plan {
 static Q8Plan q8_plan(const Q8Args& a) {
   const int sms = q8_sms();
   const int ch = (int)ceil_div(a.n, 128), kc = (int)ceil_div(a.k, Q8_KB);
-  const int nt = (int)std::min<int64_t>(256, round_up(a.m, 16));
-  const int64_t tiles = ceil_div(a.m, nt) * ch;
-  if (nt == 256 && tiles >= 2 * sms) return {true, 256, 1};
-  Q8Plan best{false, nt, 1};
+  const int most = (int)std::min<int64_t>(256, round_up(a.m, 16));
+  if (most == 256 && ceil_div(a.m, 256) * ch >= 2 * sms) return {true, 256, 1};
+  Q8Plan best{false, most, 1};
   double least = 1e30;
-  for (int s = 1; s <= 8 && s <= std::max(1, kc); ++s) {
-    const double bytes = (double)ceil_div(kc, s) * (Q8_WTILE + nt * Q8_KB);
-    const double cost = (double)ceil_div(tiles * s, sms) * bytes + s * 24.0 * 1024;
-    if (cost < least) {
-      least = cost;
-      best.splits = s;
+  for (int nt = most;; nt = std::max(16, (int)round_up(nt / 2, 16))) {
+    const int64_t tiles = ceil_div(a.m, nt) * ch;
+    for (int s = 1; s <= 8 && s <= kc; ++s) {
+      const int64_t blocks = tiles * s;
+      const double share = std::min(1.0, (double)blocks / sms) / 43;
+      const double chunk = std::max({Q8_WTILE * share, (Q8_WTILE + nt * Q8_KB) / 100.0, nt * 1.1});
+      const double cost = (double)ceil_div(blocks, sms) * (double)ceil_div(kc, s) * chunk +
+                          2000.0 * (double)ceil_div(blocks, sms * (nt <= 64 ? 2 : 1)) + (s > 1 ? 1000.0 + 15.0 * nt : 0.0);
+      if (cost < least) {
+        least = cost;
+        best.nt = nt;
+        best.splits = s;
+      }
     }
+    if (nt <= 64) break;  // smaller tiles read the weights again for nothing
   }
   return best;
 }
@@ -658,7 +678,7 @@ bool launch_q8_matmul(const Q8Args& a, cudaStream_t st) {
   // the ring: up to 104 KB where two blocks share an SM, else up to 200 KB; it also holds the sums to join
   t.stages = std::min(12, (p.nt <= 64 ? 104 : 200) * 1024 / stage);
   size_t bytes = (size_t)t.stages * stage;
-  if (p.splits > 1) bytes = std::max(bytes, (size_t)p.nt * 128 * 4);
+  if (p.splits > 1) bytes = std::max(bytes, (size_t)ceil_div(p.nt, p.splits) * p.splits * 128 * 4);
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = 128;
   cfg.dynamicSmemBytes = bytes + 1024;
