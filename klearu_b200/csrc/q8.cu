@@ -234,15 +234,43 @@ struct Q8Tile {
   uint32_t tmem_cols;
 };
 
-__device__ __forceinline__ float q8_value(const Q8Args& a, int acc, float sa, float sw, float bias) {
+enum Q8Out { Q8_F32, Q8_BF16, Q8_ADD };  // add: to an f32 out
+__device__ __forceinline__ float q8_value(int acc, float sa, float sw, float bias) {
   return fmaf((float)acc * sa, sw, bias);
 }
-__device__ __forceinline__ void q8_store(const Q8Args& a, int64_t r, int64_t c, float v) {
-  if (a.out_bf16) {
-    static_cast<__nv_bfloat16*>(a.out)[r * a.ldo + c] = __float2bfloat16_rn(v);
-  } else {
-    float* o = static_cast<float*>(a.out) + r * a.ldo + c;
-    *o = a.accumulate ? *o + v : v;
+template <int OUT>
+__device__ __forceinline__ void q8_put(char* p, float v) {
+  if (OUT == Q8_BF16) *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v);
+  else if (OUT == Q8_F32) *reinterpret_cast<float*>(p) = v;
+  else *reinterpret_cast<float*>(p) += v;
+}
+template <int OUT>
+__device__ __forceinline__ char* q8_at(const Q8Args& a, int64_t r, int64_t c) {
+  return static_cast<char*>(a.out) + (r * a.ldo + c) * (OUT == Q8_BF16 ? 2 : 4);
+}
+// Rows [0, rows) of a tile from the thread's lane of tensor memory to channel c
+// of out; sa: the rows' scales.  The warp takes part as one; live: c is a channel.
+template <int OUT>
+__device__ __forceinline__ void q8_rows(const Q8Args& a, uint32_t taddr, int64_t row, int rows, int64_t c, bool live,
+                                        const float* sa, float sw, float bias) {
+  char* p = q8_at<OUT>(a, row, c);
+  const int64_t step = a.ldo * (OUT == Q8_BF16 ? 2 : 4);
+#pragma unroll 1
+  for (int j = 0; j < rows; j += 16) {
+    uint32_t v[16];
+    float s[16];
+    tc5_ld16_async(taddr + j, v);
+#pragma unroll
+    for (int u = 0; u < 16; u += 4) *reinterpret_cast<float4*>(s + u) = *reinterpret_cast<const float4*>(sa + j + u);
+    tc5_ld_wait();
+    if (live && j + 16 <= rows) {
+#pragma unroll
+      for (int u = 0; u < 16; ++u, p += step) q8_put<OUT>(p, q8_value((int)v[u], s[u], sw, bias));
+    } else if (live) {
+#pragma unroll
+      for (int u = 0; u < 16; ++u, p += step)
+        if (j + u < rows) q8_put<OUT>(p, q8_value((int)v[u], s[u], sw, bias));
+    }
   }
 }
 
@@ -301,6 +329,7 @@ __device__ __forceinline__ void q8_drain(const Q8Tile& t, uint64_t* full, uint32
 // block finishes a share of the tile's rows, for which the others store their
 // 32-bit sums in its shared memory (whole numbers: any order gives the same
 // sum).  One launch, no workspace.
+template <int OUT>
 __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ CUtensorMap wm,
                                                        const __grid_constant__ CUtensorMap am, Q8Args a, Q8Tile t,
                                                        int splits) {
@@ -308,12 +337,14 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
   __shared__ uint64_t full[12], empty[12], done;
   __shared__ uint32_t tmem_s;
   __shared__ int fail;
-  __shared__ float sa[256];  // the tile's row scales: read between stores to out, they must not wait for memory
+  __shared__ __align__(16) float sa[256];  // the tile's row scales: read between stores to out, they must not wait for memory
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(q8_dyn) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = splits > 1 ? (int)cluster_rank() : 0;
   const int ch = (blockIdx.x / splits) * 128, row = blockIdx.y * t.nt;
   const int c0 = (int)((int64_t)t.kc * rank / splits), c1 = (int)((int64_t)t.kc * (rank + 1) / splits);
+  const int c = ch + threadIdx.x, first = min(c0 + t.stages, c1);
+  uint32_t q = 0;  // chunks issued, or multiplied
   if (threadIdx.x == 0) {
     for (int s = 0; s < t.stages; ++s) {
       mbar_init(&full[s], 1);
@@ -322,7 +353,11 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
     mbar_init(&done, 1);
     fail = 0;
     fence_mbar_init();
+    // the ring's first fills go out before anything else is ready
+    q8_load(&wm, &am, t, sm, full, empty, ch, row, c0, first, q, &fail);
   }
+  // what the end needs, while the ring fills
+  const float sw = c < a.n ? a.w_scale[c] : 0.f, bias = a.bias && c < a.n ? a.bias[c] : 0.f;
   for (int j = threadIdx.x; j < t.nt; j += 128) sa[j] = row + j < a.m ? a.a_scale[row + j] : 0.f;
   if (warp == 1) tc5_alloc(&tmem_s, t.tmem_cols);
   tc5_fence_before();
@@ -330,30 +365,19 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
   tc5_fence_after();
   const uint32_t tmem = tmem_s;
   if (warp == 0 && lane == 0) {
-    uint32_t q = 0;
-    if (!q8_load(&wm, &am, t, sm, full, empty, ch, row, c0, c1, q, &fail)) atomicExch(&fail, 1);
+    if (!q8_load(&wm, &am, t, sm, full, empty, ch, row, first, c1, q, &fail)) atomicExch(&fail, 1);
     q8_drain(t, full, q);
   } else if (warp == 1 && lane == 0) {
-    uint32_t q = 0;
     if (!q8_mma(t, sm, full, empty, tmem, c1 - c0, q, &fail)) atomicExch(&fail, 1);
     tc5_commit(&done);
     if (!mbar_wait(&done, 0)) atomicExch(&fail, 1);
   }
   __syncthreads();
   tc5_fence_after();
-  const int c = ch + threadIdx.x;
-  const float sw = c < a.n ? a.w_scale[c] : 0.f, bias = a.bias && c < a.n ? a.bias[c] : 0.f;
   const uint32_t mine = tmem + ((uint32_t)warp << 21);  // lane 32 * warp
   const int rows = min(t.nt, a.m - row);
   if (splits == 1) {
-    for (int j = 0; j < rows; j += 16) {
-      uint32_t v[16];
-      tc5_ld16_async(mine + j, v);
-      tc5_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (c < a.n && j + i < rows) q8_store(a, row + j + i, c, q8_value(a, (int)v[i], sa[j + i], sw, bias));
-    }
+    q8_rows<OUT>(a, mine, row, rows, c, c < a.n, sa, sw, bias);
   } else {
     // Row j is finished by block j % splits: each block stores its sums of that row there, [from][j / splits][channel],
     // over the ring, which no copy or MMA uses any more once all blocks are here.
@@ -361,25 +385,28 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
     const int each = (t.nt + splits - 1) / splits;
     __syncwarp();
     cluster_sync();
+    int to = 0;
+    uint32_t at = part + (uint32_t)((rank * each * 128 + (int)threadIdx.x) * 4);
     for (int j = 0; j < rows; j += 16) {
       uint32_t v[16];
       tc5_ld16_async(mine + j, v);
       tc5_ld_wait();
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int to = (j + i) % splits, slot = (j + i) / splits;
-        if (j + i < rows)
-          st_cluster(part + (uint32_t)(((rank * each + slot) * 128 + (int)threadIdx.x) * 4), (uint32_t)to, (int)v[i]);
+        if (j + i < rows) st_cluster(at, (uint32_t)to, (int)v[i]);
+        if (++to == splits) {
+          to = 0;
+          at += 512;
+        }
       }
     }
     __syncwarp();
     cluster_sync();
     const int* sums = reinterpret_cast<const int*>(sm);
-#pragma unroll 4
-    for (int j = rank; j < rows; j += splits) {
+    for (int j = rank, slot = 0; j < rows; j += splits, ++slot) {
       int acc = 0;
-      for (int r = 0; r < splits; ++r) acc += sums[(r * each + j / splits) * 128 + threadIdx.x];
-      if (c < a.n) q8_store(a, row + j, c, q8_value(a, acc, sa[j], sw, bias));
+      for (int r = 0; r < splits; ++r) acc += sums[(r * each + slot) * 128 + threadIdx.x];
+      if (c < a.n) q8_put<OUT>(q8_at<OUT>(a, row + j, c), q8_value(acc, sa[j], sw, bias));
     }
   }
   tc5_fence_before();
@@ -391,7 +418,8 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
 // Many tiles: one block per SM takes tiles in turn, two accumulators in tensor
 // memory so that the tile before is written while the next one multiplies.
 constexpr int Q8_PN = 256;
-constexpr int Q8_PNT = 192;
+constexpr int Q8_PNT = 320;  // 10 warps: loads, MMAs, 8 that write, two to a quarter of the lanes
+template <int OUT>
 __global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_constant__ CUtensorMap wm,
                                                                   const __grid_constant__ CUtensorMap am, Q8Args a,
                                                                   Q8Tile t, int ch_tiles, int tiles) {
@@ -399,7 +427,7 @@ __global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_c
   __shared__ uint64_t full[12], empty[12], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_s;
   __shared__ int fail;
-  __shared__ float sa[4][Q8_PN];  // each writing warp's copy of its tile's row scales
+  __shared__ __align__(16) float sa[8][Q8_PN / 2];  // each writing warp's copy of its half of the tile's row scales
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(q8_dyn) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -409,7 +437,7 @@ __global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_c
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);
+      mbar_init(&acc_empty[b], 8);
     }
     fail = 0;
     fence_mbar_init();
@@ -446,29 +474,23 @@ __global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_c
     }
   } else {
     const int quad = warp & 3;  // the tensor-memory lanes that this warp may read
+    const int half = (warp - 2) >> 2;
+    float* scale = sa[warp - 2];
     int n = 0;
     for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
       const int b = n & 1;
-      const int c = i % ch_tiles * 128 + quad * 32 + lane, row = i / ch_tiles * Q8_PN;
-      const int rows = min(Q8_PN, a.m - row);
+      const int c = i % ch_tiles * 128 + quad * 32 + lane, row = i / ch_tiles * Q8_PN + half * (Q8_PN / 2);
+      const int rows = max(0, min(Q8_PN / 2, a.m - row));
       const float sw = c < a.n ? a.w_scale[c] : 0.f, bias = a.bias && c < a.n ? a.bias[c] : 0.f;
       __syncwarp();
-      for (int j = lane; j < Q8_PN; j += 32) sa[quad][j] = row + j < a.m ? a.a_scale[row + j] : 0.f;
+      for (int j = lane; j < Q8_PN / 2; j += 32) scale[j] = row + j < a.m ? a.a_scale[row + j] : 0.f;
       __syncwarp();
       if (__any_sync(FULL, *vf || !mbar_wait(&acc_full[b], (uint32_t)(n / 2) & 1u))) {
         atomicExch(&fail, 1);
         break;
       }
       tc5_fence_after();
-      for (int j = 0; j < rows; j += 16) {
-        uint32_t v[16];
-        tc5_ld16_async(tmem + ((uint32_t)quad << 21) + b * Q8_PN + j, v);
-        tc5_ld_wait();
-#pragma unroll
-        for (int u = 0; u < 16; ++u)
-          if (c < a.n && j + u < rows)
-            q8_store(a, row + j + u, c, q8_value(a, (int)v[u], sa[quad][j + u], sw, bias));
-      }
+      q8_rows<OUT>(a, tmem + ((uint32_t)quad << 21) + b * Q8_PN + half * (Q8_PN / 2), row, rows, c, c < a.n, scale, sw, bias);
       tc5_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[b]);
@@ -495,7 +517,7 @@ int q8_sms() {
 // products an instruction.  No ring, tensor memory or join to set up: with one
 // row and 50 MB of weights that is 5 of 16 us.
 constexpr int Q8_VW = 4;  // warps per block
-template <int M>
+template <int OUT, int M>
 __global__ void __launch_bounds__(Q8_VW * 32) q8_vector_kernel(Q8Args a) {
   extern __shared__ __align__(16) int8_t q8_rows[];  // [M][ldw], zero from k on as the weights are
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -551,7 +573,7 @@ __global__ void __launch_bounds__(Q8_VW * 32) q8_vector_kernel(Q8Args a) {
     for (int c = 0; c < 2; ++c) {
       const int sum = warp_sum(acc[m][c]);
       if (lane == 0 && c0 + c < a.n)
-        q8_store(a, m, c0 + c, q8_value(a, sum, a.a_scale[m], a.w_scale[c0 + c], a.bias ? a.bias[c0 + c] : 0.f));
+        q8_put<OUT>(q8_at<OUT>(a, m, c0 + c), q8_value(sum, a.a_scale[m], a.w_scale[c0 + c], a.bias ? a.bias[c0 + c] : 0.f));
     }
 }
 
@@ -638,31 +660,31 @@ static Q8Plan q8_plan(const Q8Args& a) {
   return best;
 }
 
-bool launch_q8_matmul(const Q8Args& a, cudaStream_t st) {
-  static OncePerDevice once;
-  once([] {
-    cudaFuncSetAttribute(q8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-    cudaFuncSetAttribute(q8_persistent_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-  });
+template <int OUT>
+static bool launch_q8(const Q8Args& a, cudaStream_t st) {
   // four rows at most, their codes within the 48 KB of shared memory that leave an SM four blocks
   if (a.m <= 4 && a.m * a.ldw <= 48 * 1024) {
     const unsigned grid = (unsigned)ceil_div(a.n, 2 * Q8_VW);
     const size_t sm = (size_t)(a.m * a.ldw);
     switch (a.m) {
-      case 1: q8_vector_kernel<1><<<grid, Q8_VW * 32, sm, st>>>(a); break;
-      case 2: q8_vector_kernel<2><<<grid, Q8_VW * 32, sm, st>>>(a); break;
-      case 3: q8_vector_kernel<3><<<grid, Q8_VW * 32, sm, st>>>(a); break;
-      default: q8_vector_kernel<4><<<grid, Q8_VW * 32, sm, st>>>(a); break;
+      case 1: q8_vector_kernel<OUT, 1><<<grid, Q8_VW * 32, sm, st>>>(a); break;
+      case 2: q8_vector_kernel<OUT, 2><<<grid, Q8_VW * 32, sm, st>>>(a); break;
+      case 3: q8_vector_kernel<OUT, 3><<<grid, Q8_VW * 32, sm, st>>>(a); break;
+      default: q8_vector_kernel<OUT, 4><<<grid, Q8_VW * 32, sm, st>>>(a); break;
     }
     count_launch();
     return true;
   }
+  static OncePerDevice once;
+  once([] {
+    cudaFuncSetAttribute(q8_split_kernel<OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    cudaFuncSetAttribute(q8_persistent_kernel<OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 215 * 1024);
+  });
   const Q8Plan p = q8_plan(a);
   const int kc = (int)ceil_div(a.k, Q8_KB), stage = Q8_WTILE + p.nt * Q8_KB;
   CUtensorMap wm, am;
-  if (!tma_map_u8(&wm, a.w, a.n, a.ldw, a.ldw, Q8_KB, 128) || !tma_map_u8(&am, a.a, a.m, a.k, a.lda, Q8_KB, p.nt)) {
+  if (!tma_map_u8(&wm, a.w, a.n, a.ldw, a.ldw, Q8_KB, 128) || !tma_map_u8(&am, a.a, a.m, a.k, a.lda, Q8_KB, p.nt))
     return false;
-  }
   Q8Tile t{p.nt, 0, kc, 32};
   while ((int)t.tmem_cols < p.nt) t.tmem_cols *= 2;
   const int ch = (int)ceil_div(a.n, 128);
@@ -670,7 +692,7 @@ bool launch_q8_matmul(const Q8Args& a, cudaStream_t st) {
   if (p.persistent) {
     t.stages = 4;
     const int64_t tiles = row_tiles * ch;
-    q8_persistent_kernel<<<(unsigned)std::min<int64_t>(tiles, q8_sms()), Q8_PNT, t.stages * stage + 1024, st>>>(
+    q8_persistent_kernel<OUT><<<(unsigned)std::min<int64_t>(tiles, q8_sms()), Q8_PNT, t.stages * stage + 1024, st>>>(
         wm, am, a, t, ch, (int)tiles);
     count_launch();
     return true;
@@ -689,9 +711,12 @@ bool launch_q8_matmul(const Q8Args& a, cudaStream_t st) {
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   cfg.gridDim = dim3((unsigned)(ch * p.splits), (unsigned)row_tiles, 1);
-  cudaLaunchKernelEx(&cfg, q8_split_kernel, wm, am, a, t, p.splits);
+  cudaLaunchKernelEx(&cfg, q8_split_kernel<OUT>, wm, am, a, t, p.splits);
   count_launch();
   return true;
+}
+bool launch_q8_matmul(const Q8Args& a, cudaStream_t st) {
+  return a.out_bf16 ? launch_q8<Q8_BF16>(a, st) : a.accumulate ? launch_q8<Q8_ADD>(a, st) : launch_q8<Q8_F32>(a, st);
 }
 
 }  // namespace kl
