@@ -3694,7 +3694,6 @@ struct kl_kv4_s {
 struct kl_q8_linear_s {
   kl_ctx_t ctx;
   int device = 0, in = 0, out = 0;
-  int64_t ldw = 0;
   DBuf w, scale, bias;
   bool has_bias = false;
 };
@@ -3889,10 +3888,9 @@ extern "C" kl_status kl_q8_linear_create(kl_ctx_t ctx, int in_dim, int out_dim, 
   l->device = ctx->device;
   l->in = in_dim;
   l->out = out_dim;
-  l->ldw = round_up(in_dim, 128);
-  l->w.alloc((size_t)l->ldw * out_dim);
+  l->w.alloc(q8_weight_bytes(out_dim, in_dim));
   l->scale.alloc((size_t)out_dim * 4);
-  launch_q8_pack(codes, ld, out_dim, in_dim, l->w.as<int8_t>(), l->ldw, ctx->stream);
+  launch_q8_pack(codes, ld, out_dim, in_dim, l->w.as<int8_t>(), ctx->stream);
   ck_launch("q8_linear pack");
   ck(cudaMemcpyAsync(l->scale.p, scales, (size_t)out_dim * 4, cudaMemcpyDeviceToDevice, ctx->stream), "copy");
   l->has_bias = bias != nullptr;
@@ -3919,7 +3917,7 @@ extern "C" kl_status kl_q8_linear_forward(kl_q8_linear_t l, const int8_t* a, int
           "q8_linear_forward: a's rows must start on 16 bytes, lda >= in_dim");
   require(ldo >= l->out, "q8_linear_forward: ldo is below out_dim");
   const Q8Args q{a, l->w.as<int8_t>(), a_scales, l->scale.as<float>(), l->has_bias ? l->bias.as<float>() : nullptr,
-                 out, lda, l->ldw, ldo, rows, l->out, l->in, out_dtype == KL_DTYPE_BF16 ? 1 : 0, accumulate ? 1 : 0,
+                 out, lda, ldo, rows, l->out, l->in, out_dtype == KL_DTYPE_BF16 ? 1 : 0, accumulate ? 1 : 0,
                  ctx__->err.as<int>()};
   if (!launch_q8_matmul(q, ctx__->stream)) raise(KL_ECUDA, "q8_linear_forward: a TMA tensor map could not be encoded");
   ck_launch("q8_linear_forward");

@@ -427,7 +427,7 @@ struct NormQ8Args {
   int one_plus, norm, x_bf16;
 };
 void launch_norm_q8(const NormQ8Args& a, int rows, cudaStream_t st);
-// A [m][lda] (rows on 16 bytes), W [n][ldw] zero from k to ldw, ldw a multiple of 128.
+// A [m][lda] (rows on 16 bytes); W as launch_q8_pack lays it out, of q8_weight_bytes.
 struct Q8Args {
   const int8_t* a;
   const int8_t* w;
@@ -435,12 +435,13 @@ struct Q8Args {
   const float* w_scale;
   const float* bias;  // nullable
   void* out;
-  int64_t lda, ldw, ldo;
+  int64_t lda, ldo;
   int m, n, k;
   int out_bf16, accumulate;
   int* err;
 };
-void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, int64_t ldw, cudaStream_t st);
+size_t q8_weight_bytes(int n, int k);
+void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, cudaStream_t st);
 // False when a tensor map could not be encoded (nothing launched).
 bool launch_q8_matmul(const Q8Args& a, cudaStream_t st);
 

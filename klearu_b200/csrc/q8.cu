@@ -218,12 +218,16 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
 }
 
 // ---- the product ----
+// The weights are kept as tiles of 128 channels by 128 bytes of K, each 16 KB
+// contiguous and in the swizzled order that the tensor core reads (chunk e of 16
+// bytes of channel r at e ^ (r & 7)), so that one untiled copy brings a tile:
+// fetched as boxes out of rows 4 KB apart they came at 40 bytes a ns and SM.
 // out^T in tiles: 128 output channels (rows of W: the MMA's M) by nt rows of A
 // (its N), so that the weights, the larger operand of a decode step, fill the
 // 128 lanes whatever the number of rows, and a warp's stores of one row of out
-// are 32 neighbouring channels.  Both operands arrive by TMA in boxes of 128
-// bytes of K (128-byte swizzle), four MMAs of K = 32 each; rows and K beyond
-// the matrices arrive as zeros.
+// are 32 neighbouring channels.  A arrives by TMA in boxes of 128 bytes of K
+// (128-byte swizzle); four MMAs of K = 32 to a chunk; rows and K beyond the
+// matrices are zeros.
 constexpr int Q8_KB = 128;               // bytes of K per stage
 constexpr int Q8_WTILE = 128 * Q8_KB;    // weight bytes of a stage
 
@@ -232,6 +236,7 @@ struct Q8Tile {
   int stages;
   int kc;      // K chunks of 128
   uint32_t tmem_cols;
+  int join;  // rows that a block of a split finishes, a multiple of 4
 };
 
 enum Q8Out { Q8_F32, Q8_BF16, Q8_ADD };  // add: to an f32 out
@@ -279,50 +284,72 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
 }
-__device__ __forceinline__ void st_cluster(uint32_t saddr, uint32_t rank, int v) {
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void st_cluster4(uint32_t saddr, uint32_t rank, const uint32_t* v) {
   uint32_t p;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(p) : "r"(saddr), "r"(rank));
-  asm volatile("st.shared::cluster.s32 [%0], %1;\n" ::"r"(p), "r"(v) : "memory");
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+  asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }
 
-// The TMA side of a tile: K chunks [c0, c1) through the ring; q counts chunks
-// since the kernel began.  False when a wait gave up.
-__device__ __forceinline__ bool q8_load(const CUtensorMap* wm, const CUtensorMap* am, const Q8Tile& t, unsigned char* sm,
-                                        uint64_t* full, uint64_t* empty, int ch, int row, int c0, int c1, uint32_t& q,
-                                        volatile int* fail) {
-  const int stage = Q8_WTILE + t.nt * Q8_KB;
-  for (int c = c0; c < c1; ++c, ++q) {
-    const int s = (int)(q % t.stages);
-    const uint32_t round = q / t.stages;
-    if (*fail || (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1u))) return false;
-    mbar_arrive_expect_tx(&full[s], (uint32_t)stage);
-    tma_load_2d(sm + s * stage, wm, c * Q8_KB, ch, &full[s]);
-    tma_load_2d(sm + s * stage + Q8_WTILE, am, c * Q8_KB, row, &full[s]);
+// Where a ring stands: its stage, and how often it has been round.  Counted, not
+// divided out: these loops are one thread's, and two divisions a chunk of K made
+// a chunk 800 cycles long.
+struct Q8Ring {
+  int stage = 0;
+  uint32_t round = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      ++round;
+    }
+  }
+};
+// The loading side of a tile: K chunks [c0, c1) through the ring.  False when a
+// wait gave up.
+__device__ __forceinline__ bool q8_load(const int8_t* w, const CUtensorMap* am, const Q8Tile& t, unsigned char* sm,
+                                        uint64_t* full, uint64_t* empty, int ch, int row, int c0, int c1, Q8Ring& q) {
+  const int8_t* tile = w + ((int64_t)(ch >> 7) * t.kc + c0) * Q8_WTILE;
+  const int size = Q8_WTILE + t.nt * Q8_KB;
+  for (int c = c0; c < c1; ++c, q.next(t.stages), tile += Q8_WTILE) {
+    uint64_t* bar = full + q.stage;
+    unsigned char* to = sm + q.stage * size;
+    if (q.round > 0 && !mbar_wait(&empty[q.stage], (q.round - 1) & 1u)) return false;
+    mbar_arrive_expect_tx(bar, (uint32_t)size);
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(to)),
+        "l"(tile), "r"(Q8_WTILE), "r"(smem_u32(bar))
+        : "memory");
+    tma_load_2d(to + Q8_WTILE, am, c * Q8_KB, row, bar);
   }
   return true;
 }
 __device__ __forceinline__ bool q8_mma(const Q8Tile& t, unsigned char* sm, uint64_t* full, uint64_t* empty, uint32_t tmem,
-                                       int chunks, uint32_t& q, volatile int* fail) {
-  const int stage = Q8_WTILE + t.nt * Q8_KB;
-  const uint32_t idesc = i8_idesc(128, t.nt);
-  for (int c = 0; c < chunks; ++c, ++q) {
-    const int s = (int)(q % t.stages);
-    if (*fail || !mbar_wait(&full[s], (q / t.stages) & 1u)) return false;
+                                       int chunks, Q8Ring& q) {
+  const uint32_t idesc = i8_idesc(128, t.nt), size = (uint32_t)(Q8_WTILE + t.nt * Q8_KB) >> 4;
+  const uint64_t d0 = sw128_desc(smem_u32(sm));
+  for (int c = 0; c < chunks; ++c, q.next(t.stages)) {
+    if (!mbar_wait(&full[q.stage], q.round & 1u)) return false;
     tc5_fence_after();
-    const uint64_t dw = sw128_desc(smem_u32(sm + s * stage)), da = sw128_desc(smem_u32(sm + s * stage + Q8_WTILE));
+    const uint64_t dw = d0 + (uint64_t)(q.stage * size), da = dw + (Q8_WTILE >> 4);
 #pragma unroll
     for (int k = 0; k < 4; ++k) tc5_mma_i8(tmem, dw + 2 * k, da + 2 * k, idesc, (c | k) != 0);
-    tc5_commit(&empty[s]);
+    tc5_commit(&empty[q.stage]);
   }
   return true;
 }
-// no copy may be in flight when the block ends
-__device__ __forceinline__ void q8_drain(const Q8Tile& t, uint64_t* full, uint32_t q) {
-  for (uint32_t r = q > (uint32_t)t.stages ? q - t.stages : 0; r < q; ++r)
-    mbar_wait(&full[r % t.stages], (r / t.stages) & 1u);
+// No copy may be in flight when the block ends: the last round of every stage.
+__device__ __forceinline__ void q8_drain(const Q8Tile& t, uint64_t* full, const Q8Ring& q) {
+  for (int s = 0; s < t.stages; ++s) {
+    const uint32_t rounds = q.round + (s < q.stage ? 1 : 0);
+    if (rounds > 0) mbar_wait(&full[s], (rounds - 1) & 1u);
+  }
 }
 
 // Few tiles: one tile per cluster, its K split over the cluster's blocks; each
@@ -330,8 +357,7 @@ __device__ __forceinline__ void q8_drain(const Q8Tile& t, uint64_t* full, uint32
 // 32-bit sums in its shared memory (whole numbers: any order gives the same
 // sum).  One launch, no workspace.
 template <int OUT>
-__global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ CUtensorMap wm,
-                                                       const __grid_constant__ CUtensorMap am, Q8Args a, Q8Tile t,
+__global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ CUtensorMap am, Q8Args a, Q8Tile t,
                                                        int splits) {
   extern __shared__ unsigned char q8_dyn[];
   __shared__ uint64_t full[12], empty[12], done;
@@ -344,8 +370,11 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
   const int ch = (blockIdx.x / splits) * 128, row = blockIdx.y * t.nt;
   const int c0 = (int)((int64_t)t.kc * rank / splits), c1 = (int)((int64_t)t.kc * (rank + 1) / splits);
   const int c = ch + threadIdx.x, first = min(c0 + t.stages, c1);
-  uint32_t q = 0;  // chunks issued, or multiplied
+  int* part = reinterpret_cast<int*>(sm + t.stages * (Q8_WTILE + t.nt * Q8_KB));  // of a split: behind the ring
+  Q8Ring q;  // of chunks loaded, or multiplied
+  if (splits > 1) cluster_arrive();
   if (threadIdx.x == 0) {
+    prefetch_map(&am);
     for (int s = 0; s < t.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -354,7 +383,7 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
     fail = 0;
     fence_mbar_init();
     // the ring's first fills go out before anything else is ready
-    q8_load(&wm, &am, t, sm, full, empty, ch, row, c0, first, q, &fail);
+    q8_load(a.w, &am, t, sm, full, empty, ch, row, c0, first, q);
   }
   // what the end needs, while the ring fills
   const float sw = c < a.n ? a.w_scale[c] : 0.f, bias = a.bias && c < a.n ? a.bias[c] : 0.f;
@@ -365,10 +394,10 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
   tc5_fence_after();
   const uint32_t tmem = tmem_s;
   if (warp == 0 && lane == 0) {
-    if (!q8_load(&wm, &am, t, sm, full, empty, ch, row, first, c1, q, &fail)) atomicExch(&fail, 1);
+    if (!q8_load(a.w, &am, t, sm, full, empty, ch, row, first, c1, q)) atomicExch(&fail, 1);
     q8_drain(t, full, q);
   } else if (warp == 1 && lane == 0) {
-    if (!q8_mma(t, sm, full, empty, tmem, c1 - c0, q, &fail)) atomicExch(&fail, 1);
+    if (!q8_mma(t, sm, full, empty, tmem, c1 - c0, q)) atomicExch(&fail, 1);
     tc5_commit(&done);
     if (!mbar_wait(&done, 0)) atomicExch(&fail, 1);
   }
@@ -379,34 +408,40 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
   if (splits == 1) {
     q8_rows<OUT>(a, mine, row, rows, c, c < a.n, sa, sw, bias);
   } else {
-    // Row j is finished by block j % splits: each block stores its sums of that row there, [from][j / splits][channel],
-    // over the ring, which no copy or MMA uses any more once all blocks are here.
-    const uint32_t part = smem_u32(sm);
-    const int each = (t.nt + splits - 1) / splits;
-    __syncwarp();
-    cluster_sync();
-    int to = 0;
-    uint32_t at = part + (uint32_t)((rank * each * 128 + (int)threadIdx.x) * 4);
+    // Block r finishes rows [r each, (r + 1) each), for which each block stores its sums there, [from][channel][row].
+    const int each = t.join;
+    cluster_wait();  // all blocks have begun, their shared memory is there
+    const uint32_t at = smem_u32(part + (rank * 128 + (int)threadIdx.x) * each);
+#pragma unroll 1
     for (int j = 0; j < rows; j += 16) {
       uint32_t v[16];
       tc5_ld16_async(mine + j, v);
       tc5_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (j + i < rows) st_cluster(at, (uint32_t)to, (int)v[i]);
-        if (++to == splits) {
-          to = 0;
-          at += 512;
-        }
-      }
+      for (int u = 0; u < 16; u += 4)
+        if (j + u < rows) st_cluster4(at + 4 * (uint32_t)((j + u) % each), (uint32_t)((j + u) / each), v + u);
     }
     __syncwarp();
-    cluster_sync();
-    const int* sums = reinterpret_cast<const int*>(sm);
-    for (int j = rank, slot = 0; j < rows; j += splits, ++slot) {
-      int acc = 0;
-      for (int r = 0; r < splits; ++r) acc += sums[(r * each + slot) * 128 + threadIdx.x];
-      if (c < a.n) q8_put<OUT>(q8_at<OUT>(a, row + j, c), q8_value(acc, sa[j], sw, bias));
+    cluster_arrive();
+    cluster_wait();
+    const int from = rank * each, end = min(from + each, rows);
+#pragma unroll 2
+    for (int j = from; j < end; j += 4) {
+      int s[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (r < splits) {
+          const int4 v = *reinterpret_cast<const int4*>(part + (r * 128 + (int)threadIdx.x) * each + j - from);
+          s[0] += v.x;
+          s[1] += v.y;
+          s[2] += v.z;
+          s[3] += v.w;
+        }
+      }
+      char* p = q8_at<OUT>(a, row + j, c);
+#pragma unroll
+      for (int u = 0; u < 4; ++u, p += a.ldo * (OUT == Q8_BF16 ? 2 : 4))
+        if (c < a.n && j + u < end) q8_put<OUT>(p, q8_value(s[u], sa[j + u], sw, bias));
     }
   }
   tc5_fence_before();
@@ -420,8 +455,7 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
 constexpr int Q8_PN = 256;
 constexpr int Q8_PNT = 320;  // 10 warps: loads, MMAs, 8 that write, two to a quarter of the lanes
 template <int OUT>
-__global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_constant__ CUtensorMap wm,
-                                                                  const __grid_constant__ CUtensorMap am, Q8Args a,
+__global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_constant__ CUtensorMap am, Q8Args a,
                                                                   Q8Tile t, int ch_tiles, int tiles) {
   extern __shared__ unsigned char q8_dyn[];
   __shared__ uint64_t full[12], empty[12], acc_full[2], acc_empty[2];
@@ -450,9 +484,9 @@ __global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_c
   volatile int* vf = &fail;
   if (warp == 0) {
     if (lane == 0) {
-      uint32_t q = 0;
+      Q8Ring q;
       for (int i = blockIdx.x; i < tiles; i += gridDim.x)
-        if (!q8_load(&wm, &am, t, sm, full, empty, i % ch_tiles * 128, i / ch_tiles * Q8_PN, 0, t.kc, q, vf)) {
+        if (*vf || !q8_load(a.w, &am, t, sm, full, empty, i % ch_tiles * 128, i / ch_tiles * Q8_PN, 0, t.kc, q)) {
           atomicExch(&fail, 1);
           break;
         }
@@ -460,12 +494,12 @@ __global__ void __launch_bounds__(Q8_PNT, 1) q8_persistent_kernel(const __grid_c
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      uint32_t q = 0;
+      Q8Ring q;
       int n = 0;
       for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
         const int b = n & 1;
         if ((n >= 2 && !mbar_wait(&acc_empty[b], (uint32_t)(n / 2 - 1) & 1u)) ||
-            (tc5_fence_after(), !q8_mma(t, sm, full, empty, tmem + b * Q8_PN, t.kc, q, vf))) {
+            (tc5_fence_after(), *vf || !q8_mma(t, sm, full, empty, tmem + b * Q8_PN, t.kc, q))) {
           atomicExch(&fail, 1);
           break;
         }
@@ -512,26 +546,28 @@ int q8_sms() {
   return n;
 }
 
-// Up to four rows: every warp streams pairs of channels' weights, four 16-byte
+// One or two rows: every warp streams pairs of channels' weights, four 16-byte
 // loads of each in flight per lane, against the rows in shared memory, four
 // products an instruction.  No ring, tensor memory or join to set up: with one
 // row and 50 MB of weights that is 5 of 16 us.
 constexpr int Q8_VW = 4;  // warps per block
 template <int OUT, int M>
 __global__ void __launch_bounds__(Q8_VW * 32) q8_vector_kernel(Q8Args a) {
-  extern __shared__ __align__(16) int8_t q8_rows[];  // [M][ldw], zero from k on as the weights are
+  extern __shared__ __align__(16) int8_t q8_rows[];  // [M][128 kc], zero from k on as the weights are
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c0 = (blockIdx.x * Q8_VW + warp) * 2;
-  const int8_t* w0 = a.w + (int64_t)min(c0, a.n - 1) * a.ldw;
-  const int8_t* w1 = a.w + (int64_t)min(c0 + 1, a.n - 1) * a.ldw;
-  const int words = (int)(a.ldw >> 4);  // of 16 bytes
+  const int words = (a.k + Q8_KB - 1) / Q8_KB * 8;  // of 16 bytes
+  const int8_t* tile = a.w + (int64_t)(c0 >> 7) * (words >> 3) * Q8_WTILE + (c0 & 127) * Q8_KB;  // c0 is even
+  const int s0 = c0 & 7;
   uint4 x[2][4];
   auto load = [&](int at) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int i = at + u * 32 + lane;
-      x[0][u] = i < words ? __ldcs(reinterpret_cast<const uint4*>(w0) + i) : make_uint4(0, 0, 0, 0);
-      x[1][u] = i < words ? __ldcs(reinterpret_cast<const uint4*>(w1) + i) : make_uint4(0, 0, 0, 0);
+      const int8_t* p = tile + (int64_t)(i >> 3) * Q8_WTILE;
+      const bool in = i < words && c0 < a.n;
+      x[0][u] = in ? __ldcs(reinterpret_cast<const uint4*>(p + (((i & 7) ^ s0) << 4))) : make_uint4(0, 0, 0, 0);
+      x[1][u] = in ? __ldcs(reinterpret_cast<const uint4*>(p + Q8_KB + (((i & 7) ^ (s0 + 1)) << 4))) : make_uint4(0, 0, 0, 0);
     }
   };
   load(0);  // the first weights on their way while the rows are staged
@@ -577,10 +613,15 @@ __global__ void __launch_bounds__(Q8_VW * 32) q8_vector_kernel(Q8Args a) {
     }
 }
 
-__global__ void q8_pack_kernel(const int8_t* src, int64_t ld, int k, int8_t* dst, int64_t ldw) {
-  const int64_t r = blockIdx.y;
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c < ldw) dst[r * ldw + c] = c < k ? src[r * ld + c] : (int8_t)0;
+__global__ void q8_pack_kernel(const int8_t* src, int64_t ld, int n, int k, int kc, int8_t* dst) {
+  const int p = blockIdx.x * blockDim.x + threadIdx.x;  // 16 bytes of K
+  const int64_t r = (int64_t)blockIdx.z * 65535 + blockIdx.y;
+  if (p >= kc * 8 || r >= round_up(n, 128)) return;
+  uint32_t b[4] = {0, 0, 0, 0};
+  if (r < n)
+    for (int e = 0; e < 16 && p * 16 + e < k; ++e) b[e >> 2] |= (uint32_t)(uint8_t)src[r * ld + p * 16 + e] << (8 * (e & 3));
+  *reinterpret_cast<uint4*>(dst + ((r >> 7) * kc + (p >> 3)) * Q8_WTILE + (r & 127) * Q8_KB + (((p & 7) ^ (int)(r & 7)) << 4)) =
+      make_uint4(b[0], b[1], b[2], b[3]);
 }
 
 }  // namespace
@@ -619,59 +660,60 @@ void launch_norm_q8(const NormQ8Args& a, int rows, cudaStream_t st) {
   count_launch();
 }
 
-void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, int64_t ldw, cudaStream_t st) {
-  for (int r = 0; r < n; r += 65535)
-    q8_pack_kernel<<<dim3((unsigned)ceil_div(ldw, 256), std::min(65535, n - r)), 256, 0, st>>>(
-        src + r * ld, ld, k, dst + r * ldw, ldw), count_launch();
+size_t q8_weight_bytes(int n, int k) { return (size_t)ceil_div(n, 128) * ceil_div(k, Q8_KB) * Q8_WTILE; }
+void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, cudaStream_t st) {
+  const int kc = (int)ceil_div(k, Q8_KB);
+  const int64_t rows = round_up(n, 128);
+  q8_pack_kernel<<<dim3((unsigned)ceil_div(kc * 8, 128), (unsigned)std::min<int64_t>(rows, 65535),
+                        (unsigned)ceil_div(rows, 65535)),
+                   128, 0, st>>>(src, ld, n, k, kc, dst);
+  count_launch();
 }
 
-// Rows per tile and splits of K for few tiles.  A chunk of 128 bytes of K takes
-// an SM the longest of its weights at its share of the memory's rate (43 bytes a
-// ns with all SMs at it), its operands at the L2's (100), and its MMAs (1.1 ns a
-// row); each turn of blocks some 2 us to start and end, a split 1 us and 15 ns a
-// row to join.
+// Rows per tile and splits of K, by what was measured: a block takes 0.3 us and
+// 0.25 ns a row of its tile for a chunk of 128 bytes of K (one thread's loop), two
+// blocks share an SM up to 64 rows; the weights take 6.2 bytes a ns from memory
+// and 12 where other tiles of rows read them again; 2 us a further turn of blocks,
+// 3 us to join a split.  More tiles of 256 rows than SMs: the persistent kernel.
 struct Q8Plan {
   bool persistent;
   int nt, splits;
 };
 static Q8Plan q8_plan(const Q8Args& a) {
   const int sms = q8_sms();
-  const int ch = (int)ceil_div(a.n, 128), kc = (int)ceil_div(a.k, Q8_KB);
+  const int64_t ch = ceil_div(a.n, 128), kc = ceil_div(a.k, Q8_KB);
   const int most = (int)std::min<int64_t>(256, round_up(a.m, 16));
-  if (most == 256 && ceil_div(a.m, 256) * ch >= 2 * sms) return {true, 256, 1};
+  if (most == 256 && ceil_div(a.m, 256) * ch > sms) return {true, 256, 1};
+  const double bytes = (double)ch * kc * Q8_WTILE;
   Q8Plan best{false, most, 1};
   double least = 1e30;
   for (int nt = most;; nt = std::max(16, (int)round_up(nt / 2, 16))) {
-    const int64_t tiles = ceil_div(a.m, nt) * ch;
-    for (int s = 1; s <= 8 && s <= kc; ++s) {
-      const int64_t blocks = tiles * s;
-      const double share = std::min(1.0, (double)blocks / sms) / 43;
-      const double chunk = std::max({Q8_WTILE * share, (Q8_WTILE + nt * Q8_KB) / 100.0, nt * 1.1});
-      const double cost = (double)ceil_div(blocks, sms) * (double)ceil_div(kc, s) * chunk +
-                          2000.0 * (double)ceil_div(blocks, sms * (nt <= 64 ? 2 : 1)) + (s > 1 ? 1000.0 + 15.0 * nt : 0.0);
+    const int64_t row_tiles = ceil_div(a.m, nt);
+    for (int s = 1; s <= (nt <= 64 ? 8 : 1) && s <= kc; ++s) {  // a split's sums are stored behind a small ring
+      const int64_t turns = ceil_div(row_tiles * ch * s, sms * (nt <= 64 ? 2 : 1));
+      const double loop = (double)(turns * ceil_div(kc, s)) * (300 + 0.25 * nt);
+      const double stream = bytes / 6200 + (double)(row_tiles - 1) * bytes / 12000;
+      const double cost = std::max(loop, stream) + 2000.0 * (double)(turns - 1) + (s > 1 ? 3000.0 : 0.0);
       if (cost < least) {
         least = cost;
         best.nt = nt;
         best.splits = s;
       }
     }
-    if (nt <= 64) break;  // smaller tiles read the weights again for nothing
+    if (nt <= 32) break;
   }
   return best;
 }
 
 template <int OUT>
 static bool launch_q8(const Q8Args& a, cudaStream_t st) {
-  // four rows at most, their codes within the 48 KB of shared memory that leave an SM four blocks
-  if (a.m <= 4 && a.m * a.ldw <= 48 * 1024) {
+  // two rows at most (three take as long as a tile of 16), their codes within the 48 KB of shared memory that leave an SM four blocks
+  const int kc = (int)ceil_div(a.k, Q8_KB);
+  if (a.m <= 2 && a.m * kc * Q8_KB <= 48 * 1024) {
     const unsigned grid = (unsigned)ceil_div(a.n, 2 * Q8_VW);
-    const size_t sm = (size_t)(a.m * a.ldw);
-    switch (a.m) {
-      case 1: q8_vector_kernel<OUT, 1><<<grid, Q8_VW * 32, sm, st>>>(a); break;
-      case 2: q8_vector_kernel<OUT, 2><<<grid, Q8_VW * 32, sm, st>>>(a); break;
-      case 3: q8_vector_kernel<OUT, 3><<<grid, Q8_VW * 32, sm, st>>>(a); break;
-      default: q8_vector_kernel<OUT, 4><<<grid, Q8_VW * 32, sm, st>>>(a); break;
-    }
+    const size_t sm = (size_t)(a.m * kc * Q8_KB);
+    if (a.m == 1) q8_vector_kernel<OUT, 1><<<grid, Q8_VW * 32, sm, st>>>(a);
+    else q8_vector_kernel<OUT, 2><<<grid, Q8_VW * 32, sm, st>>>(a);
     count_launch();
     return true;
   }
@@ -681,11 +723,10 @@ static bool launch_q8(const Q8Args& a, cudaStream_t st) {
     cudaFuncSetAttribute(q8_persistent_kernel<OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 215 * 1024);
   });
   const Q8Plan p = q8_plan(a);
-  const int kc = (int)ceil_div(a.k, Q8_KB), stage = Q8_WTILE + p.nt * Q8_KB;
-  CUtensorMap wm, am;
-  if (!tma_map_u8(&wm, a.w, a.n, a.ldw, a.ldw, Q8_KB, 128) || !tma_map_u8(&am, a.a, a.m, a.k, a.lda, Q8_KB, p.nt))
-    return false;
-  Q8Tile t{p.nt, 0, kc, 32};
+  const int stage = Q8_WTILE + p.nt * Q8_KB;
+  CUtensorMap am;
+  if (!tma_map_u8(&am, a.a, a.m, a.k, a.lda, Q8_KB, p.nt)) return false;
+  Q8Tile t{p.nt, 0, kc, 32, 0};
   while ((int)t.tmem_cols < p.nt) t.tmem_cols *= 2;
   const int ch = (int)ceil_div(a.n, 128);
   const int64_t row_tiles = ceil_div(a.m, p.nt);
@@ -693,14 +734,15 @@ static bool launch_q8(const Q8Args& a, cudaStream_t st) {
     t.stages = 4;
     const int64_t tiles = row_tiles * ch;
     q8_persistent_kernel<OUT><<<(unsigned)std::min<int64_t>(tiles, q8_sms()), Q8_PNT, t.stages * stage + 1024, st>>>(
-        wm, am, a, t, ch, (int)tiles);
+        am, a, t, ch, (int)tiles);
     count_launch();
     return true;
   }
-  // the ring: up to 104 KB where two blocks share an SM, else up to 200 KB; it also holds the sums to join
-  t.stages = std::min(12, (p.nt <= 64 ? 104 : 200) * 1024 / stage);
-  size_t bytes = (size_t)t.stages * stage;
-  if (p.splits > 1) bytes = std::max(bytes, (size_t)ceil_div(p.nt, p.splits) * p.splits * 128 * 4);
+  // the ring and the sums to join: up to 104 KB where two blocks share an SM, else up to 200 KB
+  t.join = (int)round_up(ceil_div(p.nt, p.splits), 4);
+  const int join = p.splits > 1 ? t.join * p.splits * 128 * 4 : 0;
+  t.stages = std::min(12, ((p.nt <= 64 ? 104 : 200) * 1024 - join) / stage);
+  const size_t bytes = (size_t)t.stages * stage + join;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = 128;
   cfg.dynamicSmemBytes = bytes + 1024;
@@ -711,7 +753,7 @@ static bool launch_q8(const Q8Args& a, cudaStream_t st) {
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   cfg.gridDim = dim3((unsigned)(ch * p.splits), (unsigned)row_tiles, 1);
-  cudaLaunchKernelEx(&cfg, q8_split_kernel<OUT>, wm, am, a, t, p.splits);
+  cudaLaunchKernelEx(&cfg, q8_split_kernel<OUT>, am, a, t, p.splits);
   count_launch();
   return true;
 }
