@@ -3731,7 +3731,6 @@ AttendShape attend_shape(kl_kv4_t c, const kl_seq_batch* s, int q_heads, int win
   a.D = c->head_dim;
   a.q_heads = q_heads;
   a.kv_heads = c->view.kv_heads;
-  a.page_size = c->view.page_size;
   a.num_seqs = s->num_seqs;
   a.num_tokens = s->num_tokens;
   a.max_q = std::max(1, std::min(s->max_q, s->num_tokens));
@@ -3784,7 +3783,7 @@ extern "C" kl_status kl_kv4_create(kl_ctx_t ctx, int64_t num_pages, int page_siz
   c->mem.alloc((size_t)num_pages * kv_heads * (page_size / KV4_TILE) * kv4_tile_bytes(head_dim));
   // zero steps and minima: a token that was never written reads as zero
   ck(cudaMemsetAsync(c->mem.p, 0, c->mem.bytes, ctx->stream), "memset");
-  c->view = Kv4View{c->mem.as<unsigned char>(), num_pages, page_size, kv_heads, page_size / KV4_TILE};
+  c->view = kv4_view(c->mem.as<unsigned char>(), num_pages, page_size, kv_heads);
   ck(cudaStreamSynchronize(ctx->stream), "sync");
   *out = c.release();
   KL_API_END

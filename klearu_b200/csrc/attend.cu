@@ -23,13 +23,7 @@ struct SplitPlan {
   int chunk;      // tokens per block, a multiple of 16 AT_W
   int chunks;     // blocks along a sequence
   int row_tiles;  // blocks along a sequence's rows
-  // tile / tiles_per_page = umulhi(tile, magic) >> shift, exact below 2^31 (magic = ceil(2^(32 + shift) / d), where
-  // 2^shift < d <= 2^(shift + 1)); d = 1: magic 0
-  uint32_t magic, shift;
 };
-__device__ __forceinline__ int page_col(const SplitPlan& p, int tile) {
-  return p.magic ? (int)(__umulhi((uint32_t)tile, p.magic) >> p.shift) : tile;
-}
 // Shared memory of a block: the rings, and where the warps join.
 template <int D, int NR>
 constexpr int split_smem() {
@@ -136,7 +130,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
         }
       };
       if (lane < 2 * AT_STAGES && lane < 2 * n) {
-        const int col = lane < mine_n ? page_col(p, t0 + warp + lane * AT_W) : 0;
+        const int col = lane < mine_n ? kv4_column(a.cache, t0 + warp + lane * AT_W) : 0;
         issue(lane, col, lane < mine_n ? table[col] : 0);
       }
 
@@ -212,7 +206,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
       int next = 2 * AT_STAGES + lane, next_col = 0;
       int32_t next_page = 0;
       if (lane < 2 && next < mine_n) {
-        next_col = page_col(p, t0 + warp + next * AT_W);
+        next_col = kv4_column(a.cache, t0 + warp + next * AT_W);
         next_page = table[next_col];
       }
 
@@ -287,7 +281,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
           issue(next, next_col, next_page);
           next += 2;
           if (next < mine_n) {
-            next_col = page_col(p, t0 + warp + next * AT_W);
+            next_col = kv4_column(a.cache, t0 + warp + next * AT_W);
             next_page = table[next_col];
           }
         }
@@ -548,11 +542,6 @@ SplitPlan split_plan(const AttendShape& s) {
   chunk = std::max<int64_t>(chunk, std::min<int64_t>(round_up(span, 16 * AT_W), 256));
   p.chunk = (int)chunk;
   p.chunks = (int)std::max<int64_t>(1, ceil_div(span, chunk));
-  const int d = s.page_size / KV4_TILE;
-  if (d > 1) {
-    while ((2u << p.shift) < (unsigned)d) ++p.shift;
-    p.magic = (uint32_t)((((uint64_t)1 << (32 + p.shift)) + d - 1) / d);
-  }
   return p;
 }
 

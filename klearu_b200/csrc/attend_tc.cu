@@ -422,7 +422,6 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
   constexpr int TB = kv4_tile_bytes(D), CODES = kv4_codes(D), KVB = TcSmem<D>::KV;
   const int lane = threadIdx.x & 31, tid = threadIdx.x - 256, sub = tid & 15;
   const int kvh = blockIdx.y;
-  const int ps = a.cache.page_size, tpp = a.cache.tiles_per_page;
   uint32_t kq = 0;
   int ev_before = 0;
   bool alive = true;
@@ -432,15 +431,17 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, TcShared& sh, uns
     uint2 kp;
     auto page_of = [&](int j) {
       const int n = w.lo + j * TC_KV + (tid & ~15);
-      return j < w.steps && n < w.hi ? table[n / ps] : -1;
+      return j < w.steps && n < w.hi ? table[kv4_column(a.cache, n >> 4)] : -1;
     };
     auto is_hole = [&](int j, int32_t page) {
       return j < w.steps && w.lo + j * TC_KV + (tid & ~15) < w.hi && (page < 0 || page >= a.cache.num_pages);
     };
     // this thread's 16-token tile of step j, null where there is none
     auto tile_of = [&](int j, int32_t page) -> const unsigned char* {
-      const int n = w.lo + j * TC_KV + (tid & ~15);
-      return page < 0 || page >= a.cache.num_pages ? nullptr : kv4_tile(a.cache, TB, page, kvh, (n >> 4) % tpp);
+      const int n = (w.lo + j * TC_KV + (tid & ~15)) >> 4;
+      return page < 0 || page >= a.cache.num_pages
+                 ? nullptr
+                 : kv4_tile(a.cache, TB, page, kvh, n - kv4_column(a.cache, n) * a.cache.tiles_per_page);
     };
     auto fetch_k = [&](const unsigned char* tile) {
       kp = make_uint2(0, 0);

@@ -104,8 +104,9 @@ __device__ __forceinline__ Place find_place(const Kv4View& cache, const SeqView&
   r.pos = positions ? positions[t] : index;
   r.kind = 1;
   if (index < 0) return r;  // in front of its sequence's first token: padding
-  r.off = index % cache.page_size;
-  r.page = seq.table[b * seq.table_ld + index / cache.page_size];
+  const int col = kv4_column(cache, index >> 4);
+  r.off = index - col * cache.page_size;
+  r.page = seq.table[b * seq.table_ld + col];
   if (r.page < 0 || r.page >= cache.num_pages) {
     *bad = true;
     r.page = -1;

@@ -51,7 +51,23 @@ struct Kv4View {
   int64_t num_pages;
   int page_size, kv_heads;
   int tiles_per_page;  // page_size / 16
+  // tile / tiles_per_page = umulhi(tile, magic) >> shift for tiles below 2^31: magic = ceil(2^(32 + shift) / d),
+  // 2^shift < d <= 2^(shift + 1); d = 1: magic 0
+  uint32_t magic, shift;
 };
+__host__ inline Kv4View kv4_view(unsigned char* base, int64_t num_pages, int page_size, int kv_heads) {
+  Kv4View v{base, num_pages, page_size, kv_heads, page_size / KV4_TILE, 0, 0};
+  const uint32_t d = (uint32_t)v.tiles_per_page;
+  if (d > 1) {
+    while ((2u << v.shift) < d) ++v.shift;
+    v.magic = (uint32_t)((((uint64_t)1 << (32 + v.shift)) + d - 1) / d);
+  }
+  return v;
+}
+// The column of the page table that a sequence's tile of 16 tokens is in.
+__device__ __forceinline__ int kv4_column(const Kv4View& c, int tile) {
+  return c.magic ? (int)(__umulhi((uint32_t)tile, c.magic) >> c.shift) : tile;
+}
 __device__ __forceinline__ unsigned char* kv4_tile(const Kv4View& c, int tile_bytes, int64_t page, int head, int tile) {
   return c.base + ((page * c.kv_heads + head) * c.tiles_per_page + tile) * (int64_t)tile_bytes;
 }
@@ -87,7 +103,7 @@ struct AttendArgs {
   int* err;
 };
 struct AttendShape {
-  int D, q_heads, kv_heads, page_size, num_seqs, num_tokens;
+  int D, q_heads, kv_heads, num_seqs, num_tokens;
   int max_q, max_kv;  // of any sequence; hints: they choose the launch, not the result
   int window;
 };
