@@ -177,6 +177,84 @@ def test_append_leaves_other_rows_and_tokens(gpu_ctx):
     gpu_ctx.sync()
 
 
+@pytest.mark.parametrize("interleaved,rot", [(None, 0), (True, 128), (False, 128), (False, 48), (True, 64)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_append_of_many_tokens(gpu_ctx, dim, interleaved, rot):
+    """Prompts so long that a block takes several tokens; ragged, with padding and rows behind the last sequence."""
+    heads, kv_heads, page = 16, 8, 48
+    q_len, kv_len = [3001, 0, 5, 1800, 1], [3001, 4, 2, 1999, 700]  # the third: three rows of padding
+    t = sum(q_len) + 3
+    rot = min(rot, dim)
+    batch, pages = make_batch(q_len, kv_len, page)
+    cache = Kv4Cache(pages, page, kv_heads, dim, ctx=gpu_ctx)
+    rope = RopeTable(rot, 4096, interleaved=interleaved, ctx=gpu_ctx) if rot else None
+    q, k, v = (randn(t, h, dim, seed=s) for h, s in ((heads, 1), (kv_heads, 2), (kv_heads, 3)))
+    q_out = torch.full_like(q, 7.0)
+    cache.append(k, v, batch, q=q, rope=rope, q_out=q_out)
+    gk, gv = cache.read(batch, t)
+    pos = torch.cat([torch.arange(b - a, b, device=DEV) for a, b in zip(q_len, kv_len)])
+    live = pos >= 0
+    pos = pos.clamp(min=0)
+    turned_q, turned_k = (R.rotate(x[:-3], pos, rope.inv_freq, interleaved) if rope else x[:-3].double() for x in (q, k))
+    tol = R.HALF * turned_q.abs() + 3 * 2.0**-24 * (q[:-3].double().abs() + q.double().abs().amax())
+    off = (q_out[:-3].double() - turned_q).abs()
+    assert (off[live] <= tol[live]).all()
+    assert (q_out[:-3][~live] == 0).all() and (q_out[-3:] == 7).all()
+    assert torch.equal(gv[:-3][live], R.held(v[:-3]).float().bfloat16()[live])
+    c, s, m = R.codes(turned_k)
+    off, step = (gk[:-3].double() - (c * s + m)).abs()[live], (15 * s + m.abs())[live]
+    assert (off <= 1.01 * s[live] + 2 * R.HALF * step).all()
+    assert (off > R.HALF * step).double().mean() < 1e-3
+
+
+def test_more_tokens_than_a_grid_is_high(gpu_ctx):
+    t = 4 * 65535 + 77
+    batch, pages = make_batch([t], [t], 1024)
+    cache = Kv4Cache(pages, 1024, 1, 64, ctx=gpu_ctx)
+    k, v = randn(t, 1, 64, seed=1), randn(t, 1, 64, seed=2)
+    cache.append(k, v, batch)
+    gk, gv = cache.read(batch, t)
+    assert torch.equal(gk, R.held(k).float().bfloat16()) and torch.equal(gv, R.held(v).float().bfloat16())
+
+
+@pytest.mark.parametrize("max_q", [1, 60])
+def test_more_sequences_than_a_grid_is_high(gpu_ctx, max_q):
+    """70000 sequences of one token, every fifth without any; a token that sees only itself gives its value."""
+    n = 70000
+    kv = [0 if i % 5 == 0 else 1 for i in range(n)]
+    table = torch.randperm(n, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(n, 1).to(DEV)
+    batch = SeqBatch(torch.arange(n + 1, dtype=torch.int32, device=DEV), i32(kv), table, max_q=max_q, max_kv=1)
+    cache = Kv4Cache(n, 16, 1, 64, ctx=gpu_ctx)
+    q, k, v = randn(n, 2, 64, seed=1), randn(n, 1, 64, seed=2), randn(n, 1, 64, seed=3)
+    cache.append(k, v, batch)
+    out = cache.attend(q, batch)
+    want = torch.where(torch.tensor(kv, device=DEV)[:, None, None] > 0, R.held(v), 0.0)
+    # a value and the output are rounded once each
+    assert ((out.double() - want).abs() <= 2 * R.HALF * 1.01 * (want.abs() + (v.double().abs().amax(-1, keepdim=True) / 7))).all()
+
+
+@pytest.mark.parametrize("q_len", [[1, 3], [300, 70]])
+def test_offsets_beyond_32_bits(gpu_ctx, q_len):
+    """Pages behind the first 4 GB of a cache, rows of queries and outputs behind 4 GB of theirs."""
+    kv_heads, dim, page, kv_len = 8, 128, 1024, [1500, 700]
+    pages = 4100
+    cache = Kv4Cache(pages, page, kv_heads, dim, ctx=gpu_ctx)
+    table = i32([[4099, 3], [4098, 0]])
+    n = sum(kv_len)
+    k, v = randn(n, kv_heads, dim, seed=1), randn(n, kv_heads, dim, seed=2)
+    cache.append(k, v, SeqBatch(i32([0, 1500, 2200]), i32(kv_len), table, max_q=1500))
+    batch = SeqBatch(i32([0, q_len[0], sum(q_len)]), i32(kv_len), table, max_q=max(q_len))
+    gk, _ = cache.read(batch, sum(q_len))
+    want = R.held(torch.cat([k[1500 - q_len[0] : 1500], k[2200 - q_len[1] :]]))
+    assert torch.equal(gk, want.float().bfloat16())
+    t, far = sum(q_len), 4_400_000_000 // (2 * sum(q_len)) // 8 * 8
+    q = torch.empty(t, far, dtype=torch.bfloat16, device=DEV)[:, far - 16 * dim :].unflatten(1, (16, dim))
+    q.copy_(randn(t, 16, dim, seed=4))
+    out = torch.empty(t, far, dtype=torch.bfloat16, device=DEV)[:, far - 16 * dim :].unflatten(1, (16, dim))
+    cache.attend(q, batch, out=out)
+    check_attend(out, q, batch, R.held(k), R.held(v), q_len, kv_len)
+
+
 def test_not_finite_values_read_back_as_nan(gpu_ctx):
     batch, pages = make_batch([5], [5], 16)
     cache = Kv4Cache(pages, 16, 2, 64, ctx=gpu_ctx)

@@ -113,6 +113,50 @@ def test_product(gpu_ctx, m, n, k):
     assert ((out.double() - full).abs() <= 6 * U * size).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(257, 9700, 40), (700, 8001, 200), (1025, 4096, 272), (2560, 2000, 1000)])
+def test_product_of_many_tiles(gpu_ctx, m, n, k):
+    """More tiles of 256 x 128 than the device has processors, so that each takes several, ragged at both edges."""
+    a, w = codes(m, k, 1), codes(n, k, 2, pad=False)
+    sa, sw, bias = 0.1 + randn(m, seed=3).abs(), 0.01 + randn(n, seed=4).abs(), randn(n, seed=5)
+    want = (a.double() @ w.double().T) * sa.double()[:, None] * sw.double()
+    lin = Q8Linear(w, sw, bias=bias, ctx=gpu_ctx)
+    got = lin.forward(a, sa)
+    assert ((got.double() - want - bias.double()).abs() <= 5 * U * (want.abs() + bias.double().abs())).all()
+    wide = torch.full((m, n + 9), 7.0, dtype=torch.bfloat16, device=DEV)
+    lin.forward(a, sa, out=wide[:, 1 : n + 1])
+    tol = 2.0**-8 * (want + bias.double()).abs() + 5 * U * (want.abs() + bias.double().abs())
+    assert ((wide[:, 1 : n + 1].double() - want - bias.double()).abs() <= tol).all()
+    assert (wide[:, :1] == 7).all() and (wide[:, n + 1 :] == 7).all()
+    start = randn(m, n + 3, seed=6)
+    out = start.clone()[:, 2 : n + 2]
+    lin.forward(a, sa, out=out, accumulate=True)
+    full = want + bias.double() + start[:, 2 : n + 2].double()
+    size = want.abs() + bias.double().abs() + start[:, 2 : n + 2].double().abs()
+    assert ((out.double() - full).abs() <= 6 * U * size).all()
+
+
+def test_offsets_beyond_32_bits(gpu_ctx):
+    """Rows so far apart that byte offsets pass 2^32."""
+    far = 20_000_000  # 300 rows: 6e9 bytes of codes
+    wide = torch.empty(300, far, dtype=torch.int8, device=DEV)
+    out = torch.empty(300, far // 4, dtype=torch.float32, device=DEV)
+    n, k = 40, 96
+    w, sw = codes(n, k, 2, pad=False), 0.01 + randn(n, seed=4).abs()
+    lin = Q8Linear(w, sw, ctx=gpu_ctx)
+    x = randn(300, k, seed=1)
+    rows = quantize_rows_q8(x, ctx=gpu_ctx)
+    for m in (300, 64, 2):
+        a = wide[300 - m :, far - 128 : far - 128 + k]
+        a.copy_(rows.codes[300 - m :])
+        o = out[300 - m :, far // 4 - 45 : far // 4 - 5]
+        lin.forward(a, rows.scales[300 - m :], out=o)
+        want = (a.double() @ w.double().T) * rows.scales[300 - m :, None].double() * sw.double()
+        assert ((o.double() - want).abs() <= 4 * U * want.abs()).all()
+    y = out[:, :k]
+    y.copy_(x)
+    assert torch.equal(quantize_rows_q8(y, ctx=gpu_ctx).codes, rows.codes)
+
+
 def test_product_extremes(gpu_ctx):
     """-128 and the largest sums that 32 bits have to hold; NaN scales stay in their rows and channels."""
     k = 131071
