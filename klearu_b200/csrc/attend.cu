@@ -524,22 +524,29 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attend_join_kernel(Atte
   for (int e = 0; e < E; ++e) out[e] = __float2bfloat16_rn(acc[e] * inv);
 }
 
+// The longest stretch of keys that a tile of rows may see.
+int64_t plan_span(const AttendShape& s, int rows_per_tile) {
+  if (s.window <= 0) return s.max_kv;
+  return std::min<int64_t>(s.max_kv, (int64_t)s.window + ceil_div(rows_per_tile, s.q_heads / s.kv_heads) + 16);
+}
+
 SplitPlan split_plan(const AttendShape& s) {
-  const int group = s.q_heads / s.kv_heads;
-  const int64_t rows = (int64_t)s.max_q * group;
+  const int64_t rows = (int64_t)s.max_q * (s.q_heads / s.kv_heads);
   const int nr = rows <= 8 ? 1 : 2;
   SplitPlan p{};
   p.row_tiles = (int)std::min<int64_t>(ceil_div(rows, 8 * nr), 64);
-  // the longest stretch of keys that a tile of rows may see
-  int64_t span = s.max_kv;
-  if (s.window > 0) span = std::min<int64_t>(span, (int64_t)s.window + ceil_div(8 * nr, group) + 16);
+  const int64_t span = plan_span(s, 8 * nr);
   const int64_t items = (int64_t)s.num_seqs * s.kv_heads * p.row_tiles;
-  const int64_t resident = 148 * (nr == 1 ? 4 : 3);
-  // a batch's sequences are ragged: eight turns even them out; a few long ones are cut for one
-  const int64_t want = items >= 148 ? 8 * resident : resident;
-  int64_t chunks = std::max<int64_t>(1, want / items);
+  // Turns of the machine.  A few long sequences are cut for one: one of 60000 tokens takes 29 us so, 36 with two,
+  // 41 with four.  A batch is ragged and up to four even it out: 19 of up to 8000 take 51, 42, 47 and with eight
+  // 58 us, 64 of them 108, 89, 85 and 96.
+  const int64_t want = 148 * (nr == 1 ? 4 : 3) * std::min<int64_t>(4, std::max<int64_t>(1, items / 64));
+  const int64_t chunks = std::max<int64_t>(1, want / items);
   int64_t chunk = round_up(std::max<int64_t>(ceil_div(span, chunks), 16 * AT_W), 16 * AT_W);
-  chunk = std::max<int64_t>(chunk, std::min<int64_t>(round_up(span, 16 * AT_W), 256));
+  // Shorter chunks cost more in the join than they save: 64 sequences of up to 1000 take 23 us in one chunk each and
+  // 31 in four, 32 of up to 2000 35 us in chunks of 256 and 26 in 512; where there are few, 256 keep the latency low
+  // (one sequence of 2000: 10 us against 12 with 512).
+  chunk = std::max<int64_t>(chunk, std::min<int64_t>(round_up(span, 16 * AT_W), items >= 256 ? 1024 : items >= 128 ? 512 : 256));
   p.chunk = (int)chunk;
   p.chunks = (int)std::max<int64_t>(1, ceil_div(span, chunk));
   return p;
@@ -555,10 +562,14 @@ void launch_split(const AttendArgs& a, const SplitPlan& p, cudaStream_t st) {
   });
   attend_split_kernel<D, NR><<<grid, AT_W * 32, split_smem<D, NR>(), st>>>(a, p);
   count_launch();
-  if (p.chunks == 1) return;
-  // eight warps to a row where the rows are few enough for one turn of the machine, or the chunks many
+}
+
+// Eight warps to a row where the rows are few enough for one turn of the machine, or the chunks many.  One sequence of
+// 60000 tokens, 74 chunks: 29 us against 35 with one warp; 64 of 8000, 4 chunks: 101 against 96.
+template <int D>
+void launch_join(const AttendArgs& a, int chunks, cudaStream_t st) {
   const int64_t rows = (int64_t)a.seq.num_tokens * a.q_heads;
-  const bool wide = p.chunks > 4 && (rows <= 1024 || p.chunks > 16);
+  const bool wide = chunks > 4 && (rows <= 1024 || chunks > 16);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(wide ? rows : ceil_div(rows, 4)));
   cfg.blockDim = wide ? 256 : 128;
@@ -568,31 +579,59 @@ void launch_split(const AttendArgs& a, const SplitPlan& p, cudaStream_t st) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  if (wide) cudaLaunchKernelEx(&cfg, attend_join_kernel<D, 8>, a, p.chunks);
-  else cudaLaunchKernelEx(&cfg, attend_join_kernel<D, 1>, a, p.chunks);
+  if (wide) cudaLaunchKernelEx(&cfg, attend_join_kernel<D, 8>, a, chunks);
+  else cudaLaunchKernelEx(&cfg, attend_join_kernel<D, 1>, a, chunks);
   count_launch();
+}
+
+struct AttendPlan {
+  bool tc;
+  int chunks;
+  SplitPlan split;
+};
+
+// Which kernel.  Per key of a sequence and key head the split kernel takes 30 ps and 30 more for each tile of 16 rows;
+// the tensor-core kernel 2.4 us for 128 keys and 256 rows on each of 148 processors.  Where its blocks leave
+// processors idle it gets chunks of the keys, of 256 at least (one sequence of 2000, 64 new tokens: 25 us, 29 with 512).
+// Both sides, split and tensor core, 4 query heads on each of 8 key heads, us:
+//   new tokens                4          12         16         32         64         500
+//   1 sequence of 60000    37   80    74   81    96   82   186   86   351   93   2467  581
+//   1 of 2000              14   19    17   21    17   21    23   23    33   25    132   45
+//   16 of up to 8000       61  162   118  163   147  162   249  164   419  165   2920  741
+//   64 of up to 4000       90  220   180  223   228  223   410  224   775  230   5432 1368
+AttendPlan attend_plan(const AttendShape& s) {
+  const int64_t rows = (int64_t)s.max_q * (s.q_heads / s.kv_heads), heads = (int64_t)s.num_seqs * s.kv_heads;
+  const int64_t span = plan_span(s, 256), steps = ceil_div(span, 128), blocks = heads * ceil_div(rows, 256);
+  const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(148 / blocks, steps / 2));
+  const double tc = 2.4 * (double)ceil_div(blocks * chunks, 148) * (double)ceil_div(steps, chunks);
+  const double split = 30e-6 * (double)heads * (double)span * (double)(1 + ceil_div(rows, 16));
+  AttendPlan p{tc < split, (int)chunks, {}};
+  // hints may be far off: the workspace stays below half a gigabyte
+  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 29) / (4 * std::max<int64_t>(1, (int64_t)s.num_tokens * s.q_heads) * (s.D + 2)));
+  if (!p.tc) p.split = split_plan(s), p.chunks = p.split.chunks;
+  p.chunks = p.split.chunks = (int)std::min<int64_t>(p.chunks, most);
+  return p;
 }
 
 }  // namespace
 
-// Above 48 rows of one key head and sequence the tensor-core kernel's 256-row
-// blocks, below it 16-row tiles that read the keys again for each.
-static bool many_rows(const AttendShape& s) { return (int64_t)s.max_q * (s.q_heads / s.kv_heads) > 48; }
-
 size_t attend_workspace(const AttendShape& s) {
-  if (many_rows(s)) return 0;
-  const SplitPlan p = split_plan(s);
-  if (p.chunks == 1) return 0;
-  const int64_t rows = (int64_t)p.chunks * s.num_tokens * s.q_heads;
+  const int chunks = attend_plan(s).chunks;
+  if (chunks == 1) return 0;
+  const int64_t rows = (int64_t)chunks * s.num_tokens * s.q_heads;
   return (size_t)(round_up(rows * 2, 4) + rows * s.D) * 4;
 }
 
 void launch_attend(const AttendArgs& a, const AttendShape& s, cudaStream_t st) {
-  if (many_rows(s)) return launch_attend_tc(a, s, st);
-  const SplitPlan p = split_plan(s);
-  const bool one = (int64_t)s.max_q * (s.q_heads / s.kv_heads) <= 8;
-  if (s.D == 128) one ? launch_split<128, 1>(a, p, st) : launch_split<128, 2>(a, p, st);
-  else one ? launch_split<64, 1>(a, p, st) : launch_split<64, 2>(a, p, st);
+  const AttendPlan p = attend_plan(s);
+  if (p.tc) {
+    launch_attend_tc(a, s, p.chunks, st);
+  } else {
+    const bool one = (int64_t)s.max_q * (s.q_heads / s.kv_heads) <= 8;
+    if (s.D == 128) one ? launch_split<128, 1>(a, p.split, st) : launch_split<128, 2>(a, p.split, st);
+    else one ? launch_split<64, 1>(a, p.split, st) : launch_split<64, 2>(a, p.split, st);
+  }
+  if (p.chunks > 1) s.D == 128 ? launch_join<128>(a, p.chunks, st) : launch_join<64>(a, p.chunks, st);
 }
 
 }  // namespace kl

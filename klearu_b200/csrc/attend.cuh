@@ -5,7 +5,8 @@
 
 namespace kl {
 
-void launch_attend_tc(const AttendArgs& a, const AttendShape& s, cudaStream_t st);  // attend_tc.cu
+// attend_tc.cu; with more than one chunk of the keys the join is the caller's
+void launch_attend_tc(const AttendArgs& a, const AttendShape& s, int chunks, cudaStream_t st);
 
 // 2^x by the special function unit; results below 2^-126 are zero
 __device__ __forceinline__ float exp2_fast(float x) {
