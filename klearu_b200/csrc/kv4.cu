@@ -33,18 +33,18 @@ struct Turn {
 template <int MODE>
 __device__ __forceinline__ void load_turn(Turn& t, const float2* row, int l, int rot, bool interleaved) {
   const int d0 = 8 * l, half = rot >> 1;
-  if (MODE == TURN_PAIRS || MODE == TURN_HALVES) {
+  if constexpr (MODE == TURN_PAIRS || MODE == TURN_HALVES) {
     if (d0 >= rot) return;
     const float4* p = reinterpret_cast<const float4*>(row + (MODE == TURN_PAIRS ? 4 * l : d0 < half ? d0 : d0 - half));
 #pragma unroll
     for (int i = 0; i < (MODE == TURN_PAIRS ? 2 : 4); ++i) *reinterpret_cast<float4*>(&t.cs[2 * i]) = p[i];
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = interleaved ? d0 + 2 * i : d0 + i;
-    t.cs[i] = make_float2(1.f, 0.f);
-    if ((!interleaved || i < 4) && d < rot) t.cs[i] = row[interleaved ? d >> 1 : d < half ? d : d - half];
+    for (int i = 0; i < 8; ++i) {
+      const int d = interleaved ? d0 + 2 * i : d0 + i;
+      t.cs[i] = make_float2(1.f, 0.f);
+      if ((!interleaved || i < 4) && d < rot) t.cs[i] = row[interleaved ? d >> 1 : d < half ? d : d - half];
+    }
   }
 }
 // Turns lane-held dims [8 l, 8 l + 8) of the row at p; dims from rot on stay.
@@ -84,8 +84,18 @@ __device__ __forceinline__ void turn8(float* x, const Turn& t, const __nv_bfloat
   }
 }
 
+__device__ __forceinline__ void async_copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
 constexpr int AP_NT = 256;
-constexpr int AP_TOKENS = 4;  // tokens of a block, each looked up by a warp
+constexpr int AP_RING = 4;     // rows of a thread's ring
+constexpr int AP_BLOCKS = 4;   // of an SM
+constexpr int AP_EACH = 12;    // most vectors of a group
+constexpr int RD_TOKENS = 4;   // most tokens of a block that reads
 
 // Where a token stands: its page and place in it, its position.
 struct Place {
@@ -93,13 +103,13 @@ struct Place {
   int off, pos;
   int kind;  // 0: of no sequence, left as it is; 1: padding or bad, zeros; 2: live
 };
-// By a warp.  *bad: something had to be left out.
-__device__ __forceinline__ Place find_place(const Kv4View& cache, const SeqView& seq, const int32_t* positions, int t,
+// Token t of sequence b.  *bad: something had to be left out.
+__device__ __forceinline__ Place find_place(const Kv4View& cache, const SeqView& seq, const int32_t* positions, int b, int t,
                                             bool table, int64_t max_pos, bool* bad) {
   Place r{-1, 0, 0, 0};
-  const int b = find_seq(seq.cu_q, seq.num_seqs, t);
   if (b >= seq.num_seqs) return r;
   const SeqSpan s = seq_span(seq, b, cache.page_size, bad);
+  if (t < s.row) return r;  // in front of the first sequence
   const int index = s.kv_len - s.q_len + (t - s.row);
   r.pos = positions ? positions[t] : index;
   r.kind = 1;
@@ -119,6 +129,29 @@ __device__ __forceinline__ Place find_place(const Kv4View& cache, const SeqView&
   return r;
 }
 
+// The places of a block's n tokens from t0 on: its first warp searches the first one's sequence, each lane walks on to
+// its own token's, which is hardly ever more than a step away, or searches in what is left.  One chain of loads for all.
+__device__ __forceinline__ void find_places(const Kv4View& cache, const SeqView& seq, const int32_t* positions, int t0, int n,
+                                            bool table, int64_t max_pos, Place* places, int* err) {
+  if (threadIdx.x >= 32) return;
+  const int lane = threadIdx.x, t = t0 + min(lane, n - 1), ns = seq.num_seqs;
+  int b = find_seq(seq.cu_q, ns, t0);
+  for (int i = 0; i < 3 && b < ns && seq.cu_q[b + 1] <= t; ++i) ++b;
+  if (b < ns && seq.cu_q[b + 1] <= t) {
+    int lo = b + 1, hi = ns;
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      if (seq.cu_q[mid + 1] <= t) lo = mid + 1;
+      else hi = mid;
+    }
+    b = lo;
+  }
+  bool bad = false;
+  const Place p = find_place(cache, seq, positions, b, t, table, max_pos, &bad);
+  if (lane < n) places[lane] = p;
+  if (bad && blockIdx.x == 0) atomicOr(err, DERR_BOUNDS);
+}
+
 struct AppendArgs {
   Kv4View cache;
   SeqView seq;
@@ -128,7 +161,7 @@ struct AppendArgs {
   int64_t max_pos;
   int q_heads;  // 0: no queries
   HeadRows q, k, v, q_out;
-  int tokens;  // of a block
+  int shift, each;  // 2^shift groups of lanes take a token of the block, each of them that many of its vectors
   int* err;
 };
 
@@ -156,107 +189,113 @@ __device__ __forceinline__ uint32_t codes8(const float* x, float m, float s) {
   return near ? exact_codes(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), m, s) : w;
 }
 
-// One group of D / 8 lanes per head vector, 8 dims per lane: a block's groups
-// take 16 (D = 128) or 32 head vectors, q heads then k then v, of up to four
-// tokens, two tokens' loads in flight at once.  All traffic is the vectors
-// themselves: memory bounds it for prompts, the chain of dependent loads
-// (sequence, page and position, vector) for one token.
+// A group of D / 8 lanes takes the head vectors of one token one by one, 8 dims
+// per lane, so that the token's row of the table is loaded once; a block's 16
+// (D = 128) or 32 groups are dealt to one or more tokens.  Each thread's 16 bytes
+// of a vector come through a ring of its own in shared memory, three vectors
+// ahead, which keeps the registers for four blocks an SM.
+// 8000 tokens of 48 heads of 128, half of each turned: 51 us, 3.4 TB/s; what is
+// left is the latency of a block's chain (sequence, page, table, vectors).  A head
+// vector of several tokens to a group, table rows loaded again for each: 20% to
+// 35% slower; without the ring, two tokens in registers: 15% more.
 template <int D, int MODE>
-__global__ void __launch_bounds__(AP_NT, 3) kv4_append_kernel(AppendArgs a) {
-  constexpr int L = D / 8;        // lanes per vector
-  constexpr int PER = AP_NT / L;  // vectors per block
-  constexpr int U = 2;            // tokens in flight
-  __shared__ Place places[AP_TOKENS];
+__global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs a) {
+  constexpr int L = D / 8;  // lanes of a group
+  __shared__ uint4 ring[AP_RING][AP_NT];
+  __shared__ Place places[AP_NT / L];
   const int kh = a.cache.kv_heads, items = a.q_heads + 2 * kh;
-  const int l = threadIdx.x % L, item = blockIdx.x * PER + threadIdx.x / L;
-  const int t0 = (int)(((int64_t)blockIdx.z * 65535 + blockIdx.y) * a.tokens);
-  const int n = min(a.tokens, a.seq.num_tokens - t0);
-  if ((int)(threadIdx.x >> 5) < n) {
-    bool bad = false;
-    const Place p = find_place(a.cache, a.seq, a.positions, t0 + (threadIdx.x >> 5), MODE != TURN_NONE, a.max_pos, &bad);
-    if ((threadIdx.x & 31) == 0) places[threadIdx.x >> 5] = p;
-    if (bad && (threadIdx.x & 31) == 0 && blockIdx.x == 0) atomicOr(a.err, DERR_BOUNDS);
-  }
-  const bool is_q = item < a.q_heads, is_k = !is_q && item < a.q_heads + kh;
-  const int head = is_q ? item : is_k ? item - a.q_heads : item - a.q_heads - kh;
-  const HeadRows& in = is_q ? a.q : is_k ? a.k : a.v;
-  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(in.p) + (int64_t)t0 * in.token + head * in.head;
-  const int64_t stride = in.token;
-  const bool vec = in.vec;
+  const int l = threadIdx.x % L, per = 1 << a.shift, tokens = (AP_NT / L) >> a.shift;
+  const int t0 = (int)(((int64_t)blockIdx.z * 65535 + blockIdx.y) * tokens), here = min(tokens, a.seq.num_tokens - t0);
+  const int mine = (threadIdx.x / L) >> a.shift, t = t0 + mine;
+  const int first = blockIdx.x * per * a.each + (threadIdx.x / L & (per - 1));  // then every per-th: q heads, k, v
+  const int n = mine < here && first < items ? min(a.each, (items - first + per - 1) >> a.shift) : 0;
+  auto vector_of = [&](int item, bool* vec) {
+    const bool is_q = item < a.q_heads, is_k = item < a.q_heads + kh;
+    const HeadRows& in = is_q ? a.q : is_k ? a.k : a.v;
+    const int head = item - (is_q ? 0 : is_k ? a.q_heads : a.q_heads + kh);
+    *vec = in.vec;
+    return static_cast<const __nv_bfloat16*>(in.p) + (int64_t)t * in.token + head * in.head;
+  };
+  auto fetch = [&](int i) {  // into a slot that was read a vector ago
+    if (i < n) {
+      bool vec;
+      const __nv_bfloat16* p = vector_of(first + (i << a.shift), &vec) + 8 * l;
+      uint4* to = &ring[i % AP_RING][threadIdx.x];
+      if (vec) async_copy16(to, p);
+      else *to = load8_raw(p, false);
+    }
+    async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < AP_RING - 1; ++i) fetch(i);  // before their places are known
+  find_places(a.cache, a.seq, a.positions, t0, here, MODE != TURN_NONE, a.max_pos, places, a.err);
   const unsigned group = (L == 16 ? 0xffffu : 0xffu) << ((threadIdx.x & 31) / L * L);
-  const bool turned = MODE != TURN_NONE && (is_q || is_k);
-  uint4 raw[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)  // the first ones before their places are known
-    if (item < items && u < n) raw[u] = load8_raw(row + u * stride + 8 * l, vec);
   __syncthreads();
-  if (item >= items) return;
+  if (n == 0) return;
+  const Place pl = places[mine];
+  const int kind = pl.kind, tok = pl.off & 15;
+  if (kind == 0) {
+    async_wait<0>();
+    return;
+  }
+  Turn turn;
+  if (MODE != TURN_NONE && kind == 2 && first < a.q_heads + kh)
+    load_turn<MODE>(turn, a.table + (int64_t)pl.pos * (a.rot >> 1), l, a.rot, a.interleaved);
 
-  for (int u0 = 0; u0 < n; u0 += U) {
-    Turn turn[U];
-    if (u0 > 0) {
+  for (int i = 0; i < n; ++i) {
+    fetch(i + AP_RING - 1);
+    async_wait<AP_RING - 1>();
+    const int item = first + (i << a.shift);
+    const bool is_q = item < a.q_heads, is_k = !is_q && item < a.q_heads + kh;
+    if (!is_q && (kind != 2 || pl.page < 0)) continue;
+    const uint4 raw = ring[i % AP_RING][threadIdx.x];
+    const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
+    float x[8];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u0 + u < n) raw[u] = load8_raw(row + (u0 + u) * stride + 8 * l, vec);
+    for (int e = 0; e < 4; ++e) {
+      x[2 * e] = __uint_as_float(w4[e] << 16);
+      x[2 * e + 1] = __uint_as_float(w4[e] & 0xffff0000u);
     }
-    if (turned) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u0 + u < n && places[u0 + u].kind == 2)
-          load_turn<MODE>(turn[u], a.table + (int64_t)places[u0 + u].pos * (a.rot >> 1), l, a.rot, a.interleaved);
+    if (MODE != TURN_NONE && kind == 2 && (is_q || is_k)) {
+      bool vec;
+      turn8<MODE>(x, turn, MODE == TURN_ANY ? vector_of(item, &vec) : nullptr, l, a.rot, a.interleaved, group);
     }
+    if (is_q) {
+      if (kind != 2) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (u0 + u >= n) break;
-      const Place& pl = places[u0 + u];
-      const int kind = pl.kind;
-      if (kind == 0 || (!is_q && (kind != 2 || pl.page < 0))) continue;
-      float x[8];
-      const uint32_t w4[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+      }
+      __syncwarp(group);  // q_out may be q: every lane has read its partners
+      store8_bf16(static_cast<__nv_bfloat16*>(a.q_out.p) + (int64_t)t * a.q_out.token + item * a.q_out.head + 8 * l,
+                  a.q_out.vec, x);
+      continue;
+    }
+    float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
+    float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    // 0 * x is 0 for a finite x, else NaN
+    const float z = 0.f * x[0] + 0.f * x[1] + 0.f * x[2] + 0.f * x[3] + 0.f * x[4] + 0.f * x[5] + 0.f * x[6] + 0.f * x[7];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w4[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w4[i] & 0xffff0000u);
-      }
-      if (turned && kind == 2) turn8<MODE>(x, turn[u], row + (u0 + u) * stride, l, a.rot, a.interleaved, group);
-      if (is_q) {
-        if (kind != 2) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        }
-        __syncwarp(group);  // q_out may be q: every lane has read its partners
-        store8_bf16(static_cast<__nv_bfloat16*>(a.q_out.p) + (int64_t)(t0 + u0 + u) * a.q_out.token + head * a.q_out.head +
-                        8 * l,
-                    a.q_out.vec, x);
-        continue;
-      }
-      float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
-      float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      // 0 * x is 0 for a finite x, else NaN
-      const float z = 0.f * x[0] + 0.f * x[1] + 0.f * x[2] + 0.f * x[3] + 0.f * x[4] + 0.f * x[5] + 0.f * x[6] + 0.f * x[7];
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(group, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(group, hi, o));
-      }
-      const bool fin = __all_sync(group, z == 0.f);
-      // 8 bits for step and minimum: the codes are taken against the rounded values
-      __nv_bfloat16 st = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.f)), mn = __float2bfloat16_rn(lo);
-      float sf = to_f(st), mf = to_f(mn);
-      if (!fin || !finite_f(sf) || !finite_f(mf)) {
-        st = __ushort_as_bfloat16(0);
-        mn = __ushort_as_bfloat16(0x7fff);
-        sf = 0.f;
-      }
-      const uint32_t w = sf > 0.f ? codes8(x, mf, sf) : 0u;
-      const int tok = pl.off & 15;
-      unsigned char* tile = kv4_tile(a.cache, kv4_tile_bytes(D), pl.page, head, pl.off >> 4);
-      const int code = is_k ? kv4_k_off<D>(tok, l) : kv4_codes(D) + kv4_v_off<D>(tok, l);
-      *reinterpret_cast<uint32_t*>(tile + code) = w;
-      if (l == 0) {
-        const uint32_t pr = (uint32_t)__bfloat16_as_ushort(st) | ((uint32_t)__bfloat16_as_ushort(mn) << 16);
-        *reinterpret_cast<uint32_t*>(tile + 2 * kv4_codes(D) + tok * 8 + (is_k ? 0 : 4)) = pr;
-      }
+    for (int o = L / 2; o > 0; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(group, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(group, hi, o));
+    }
+    const bool fin = __all_sync(group, z == 0.f);
+    // 8 bits for step and minimum: the codes are taken against the rounded values
+    __nv_bfloat16 st = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.f)), mn = __float2bfloat16_rn(lo);
+    float sf = to_f(st), mf = to_f(mn);
+    if (!fin || !finite_f(sf) || !finite_f(mf)) {
+      st = __ushort_as_bfloat16(0);
+      mn = __ushort_as_bfloat16(0x7fff);
+      sf = 0.f;
+    }
+    const uint32_t w = sf > 0.f ? codes8(x, mf, sf) : 0u;
+    const int head = item - a.q_heads - (is_k ? 0 : kh);
+    unsigned char* tile = kv4_tile(a.cache, kv4_tile_bytes(D), pl.page, head, pl.off >> 4);
+    const int code = is_k ? kv4_k_off<D>(tok, l) : kv4_codes(D) + kv4_v_off<D>(tok, l);
+    *reinterpret_cast<uint32_t*>(tile + code) = w;
+    if (l == 0) {
+      const uint32_t pr = (uint32_t)__bfloat16_as_ushort(st) | ((uint32_t)__bfloat16_as_ushort(mn) << 16);
+      *reinterpret_cast<uint32_t*>(tile + 2 * kv4_codes(D) + tok * 8 + (is_k ? 0 : 4)) = pr;
     }
   }
 }
@@ -274,17 +313,12 @@ struct ReadArgs {
 template <int D>
 __global__ void __launch_bounds__(AP_NT) kv4_read_kernel(ReadArgs a) {
   constexpr int L = D / 8, PER = AP_NT / L, U = 4;
-  __shared__ Place places[AP_TOKENS];
+  __shared__ Place places[RD_TOKENS];
   const int kh = a.cache.kv_heads;
   const int l = threadIdx.x % L, item = blockIdx.x * PER + threadIdx.x / L;
   const int t0 = (int)(((int64_t)blockIdx.z * 65535 + blockIdx.y) * a.tokens);
   const int n = min(a.tokens, a.seq.num_tokens - t0);
-  if ((int)(threadIdx.x >> 5) < n) {
-    bool bad = false;
-    const Place p = find_place(a.cache, a.seq, nullptr, t0 + (threadIdx.x >> 5), false, 0, &bad);
-    if ((threadIdx.x & 31) == 0) places[threadIdx.x >> 5] = p;
-    if (bad && (threadIdx.x & 31) == 0 && blockIdx.x == 0) atomicOr(a.err, DERR_BOUNDS);
-  }
+  find_places(a.cache, a.seq, nullptr, t0, n, false, 0, places, a.err);
   __syncthreads();
   if (item >= 2 * kh) return;
   const bool is_k = item < kh;
@@ -314,8 +348,8 @@ __global__ void __launch_bounds__(AP_NT) kv4_read_kernel(ReadArgs a) {
   }
 }
 
-// Four tokens a block where there are blocks enough, one where latency counts.
-int block_tokens(int items, int per, int tokens) { return ceil_div(items, per) * tokens >= 4 * 1184 ? AP_TOKENS : 1; }
+// Reading: four tokens a block where one each would be more blocks than the machine holds at once.
+int block_tokens(int items, int per, int tokens) { return ceil_div(items, per) * tokens >= 8 * 148 ? RD_TOKENS : 1; }
 dim3 token_grid(int items, int per, int tokens, int each) {
   const int64_t n = ceil_div(tokens, each);
   return dim3((unsigned)ceil_div(items, per), (unsigned)std::min<int64_t>(n, 65535), (unsigned)ceil_div(n, 65535));
@@ -339,9 +373,16 @@ void launch_rope_table(const double* inv_freq, int pairs, int64_t n, float facto
 void launch_kv4_append(const Kv4View& cache, int D, const SeqView& seq, const int32_t* positions, const float2* table,
                        int rot, int interleaved, int64_t max_pos, int q_heads, const HeadRows& q, const HeadRows& k,
                        const HeadRows& v, const HeadRows& q_out, int* err, cudaStream_t st) {
-  const int items = q_heads + 2 * cache.kv_heads, per = AP_NT / (D / 8), each = block_tokens(items, per, seq.num_tokens);
-  const AppendArgs a{cache, seq, positions, table, rot, interleaved, max_pos, q_heads, q, k, v, q_out, each, err};
-  const dim3 grid = token_grid(items, per, seq.num_tokens, each);
+  // One vector a group while that gives each processor two blocks at most, up to AP_EACH for more.  48 heads of 128:
+  // 64 tokens take 8.3 us with one or four each and 10.4 with eight, 500 tokens 14.2, 10.4 and 12.5, 8000 tokens 108,
+  // 74 and 66 and with twelve 63.
+  const int items = q_heads + 2 * cache.kv_heads, groups = AP_NT / (D / 8);
+  const int64_t turns = (int64_t)items * seq.num_tokens / ((int64_t)groups * 2 * 148);
+  const int each = (int)std::min<int64_t>(AP_EACH, std::max<int64_t>(1, turns));
+  int shift = 0;
+  while ((1 << shift) < groups && (each << shift) < items) ++shift;
+  const AppendArgs a{cache, seq, positions, table, rot, interleaved, max_pos, q_heads, q, k, v, q_out, shift, each, err};
+  const dim3 grid = token_grid(items, each << shift, seq.num_tokens, groups >> shift);
   if (D == 128) launch_append<128>(a, grid, st);
   else launch_append<64>(a, grid, st);
   count_launch();

@@ -707,9 +707,11 @@ static Q8Plan q8_plan(const Q8Args& a) {
 
 template <int OUT>
 static bool launch_q8(const Q8Args& a, cudaStream_t st) {
-  // two rows at most (three take as long as a tile of 16), their codes within the 48 KB of shared memory that leave an SM four blocks
+  // Two rows at most (three take as long as a tile of 16), and 16 KB of their codes, which each block loads first: one
+  // row of 4096 on 12288 channels takes 12.4 us (the ring 17.2), two 14.5 (17.6); one of 16384 on 4096 16.5 (18.6), of
+  // 22016 26.9 (22.7), two of 8192 12.4 (12.8), of 11008 18.6 (14.9).
   const int kc = (int)ceil_div(a.k, Q8_KB);
-  if (a.m <= 2 && a.m * kc * Q8_KB <= 48 * 1024) {
+  if (a.m <= 2 && a.m * kc * Q8_KB <= 16 * 1024) {
     const unsigned grid = (unsigned)ceil_div(a.n, 2 * Q8_VW);
     const size_t sm = (size_t)(a.m * kc * Q8_KB);
     if (a.m == 1) q8_vector_kernel<OUT, 1><<<grid, Q8_VW * 32, sm, st>>>(a);

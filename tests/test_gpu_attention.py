@@ -518,3 +518,50 @@ def test_handles_outlive_their_context():
     ctx.close()
     assert lib.kl_kv4_destroy(cache.h) == 0 and lib.kl_rope_destroy(rope.h) == 0
     cache.h = rope.h = None
+
+
+@pytest.mark.parametrize("heads,kv_heads,tokens", [(1, 1, 700), (3, 1, 5000), (60, 20, 300), (60, 20, 2), (128, 128, 40)])
+def test_append_head_counts(gpu_ctx, heads, kv_heads, tokens):
+    """Few and many heads on few and many tokens: every way of dealing them to the machine."""
+    for dim in (64, 128):
+        batch, pages = make_batch([tokens], [tokens], 16)
+        cache = Kv4Cache(pages, 16, kv_heads, dim, ctx=gpu_ctx)
+        q, k, v = (randn(tokens, h, dim, seed=s) for h, s in ((heads, 1), (kv_heads, 2), (kv_heads, 3)))
+        assert torch.equal(cache.append(k, v, batch, q=q), q)
+        got_k, got_v = cache.read(batch, tokens)
+        assert torch.equal(got_k, R.held(k).float().bfloat16())
+        assert torch.equal(got_v, R.held(v).float().bfloat16())
+
+
+def test_rows_in_front_of_the_first_sequence(gpu_ctx):
+    """cu_q that starts at 3: the rows before it belong to nobody, and nothing of theirs is written."""
+    batch, pages = make_batch([6], [6], 16)
+    cache = Kv4Cache(pages, 16, 2, 64, ctx=gpu_ctx)
+    k, v = randn(6, 2, 64, seed=1), randn(6, 2, 64, seed=2)
+    cache.append(k, v, batch)
+    late = SeqBatch(i32([3, 5]), i32([8]), batch.page_table, max_q=2)
+    k2, v2, q2 = randn(6, 2, 64, seed=3), randn(6, 2, 64, seed=4), randn(6, 4, 64, seed=5)
+    q_out = torch.full_like(q2, 7.0)
+    cache.append(k2, v2, late, q=q2, q_out=q_out)
+    assert (q_out[:3] == 7).all() and (q_out[5] == 7).all() and torch.equal(q_out[3:5], q2[3:5])
+    every = SeqBatch(i32([0, 8]), i32([8]), batch.page_table, max_q=8)
+    got, _ = cache.read(every, 8)
+    assert torch.equal(got, R.held(torch.cat([k, k2[3:5]])).float().bfloat16())
+    out = cache.attend(q2, late, out=torch.full_like(q2, 7.0))
+    assert (out[:3] == 7).all() and (out[5] == 7).all()
+
+
+def test_many_empty_sequences_between(gpu_ctx):
+    """Tokens whose sequences lie far apart in the batch, with thousands of empty ones between."""
+    n = 9000
+    q_len = [0] * n
+    for b, x in ((0, 2), (1, 1), (4500, 5), (4504, 1), (8999, 3)):
+        q_len[b] = x
+    kv_len = [x if x else 0 for x in q_len]
+    batch, pages = make_batch(q_len, kv_len, 16)
+    t = sum(q_len)
+    cache = Kv4Cache(pages, 16, 8, 64, ctx=gpu_ctx)
+    k, v = randn(t, 8, 64, seed=1), randn(t, 8, 64, seed=2)
+    cache.append(k, v, batch)
+    got_k, got_v = cache.read(batch, t)
+    assert torch.equal(got_k, R.held(k).float().bfloat16()) and torch.equal(got_v, R.held(v).float().bfloat16())
