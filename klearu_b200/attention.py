@@ -140,6 +140,8 @@ class SeqBatch:
         """A reference to the C struct for a call with so many rows."""
         got = self._c.get(num_tokens)
         if got is None:
+            if len(self._c) >= 64:
+                self._c.clear()
             cu_q, kv_len, table = self._tensors
             wide = table.shape[1]
             got = self._c[num_tokens] = C.byref(SeqBatchC(
@@ -269,6 +271,8 @@ class Kv4Cache:
         if need is None:
             n = C.c_size_t()
             launch(self.ctx, "kl_kv4_attend_workspace", self.h, c, heads, window, C.byref(n))
+            if len(self._workspace) >= 4096:
+                self._workspace.clear()
             need = self._workspace[key] = n.value
         # from torch's allocator in stream order: a captured graph keeps one of its own
         space = q.new_empty((need + 1) // 2) if need else None
