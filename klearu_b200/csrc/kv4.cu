@@ -161,6 +161,7 @@ struct AppendArgs {
   int64_t max_pos;
   int q_heads;  // 0: no queries
   HeadRows q, k, v, q_out;
+  int vec;          // all vectors start on 16 bytes
   int shift, each;  // 2^shift groups of lanes take a token of the block, each of them that many of its vectors
   int* err;
 };
@@ -175,18 +176,41 @@ __device__ __noinline__ uint32_t exact_codes(float4 a, float4 b, float m, float 
   return w;
 }
 // By a reciprocal: quotients off by at most 2^-23 of 15 decide unless one is
-// within 1e-5 of a border between two codes (or the reciprocal is none to use).
+// within 1e-5 of a border between two codes; there the sign of x - m - border * s
+// does, which one fused operation gives exactly, and on the border the even code.
+// (Values of 8 bits are often on one: a call with divisions for those took as
+// long as all the rest.)
 __device__ __forceinline__ uint32_t codes8(const float* x, float m, float s) {
+  if (!(s > 1e-30f && s < 1e30f)) return exact_codes(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), m, s);
   const float inv = __frcp_rn(s);
-  uint32_t w = 0;
-  bool near = !(s > 1e-30f && s < 1e30f);
+  float c[8], off = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float y = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f), c = y + 8388608.f;  // 2^23: rounds to a whole number
-    near = near || fabsf(y - (c - 8388608.f)) > 0.49999f;
-    w |= (__float_as_uint(c) & 15u) << (4 * kv4_nibble(i));
+    const float y = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
+    c[i] = (y + 8388608.f) - 8388608.f;  // 2^23: to a whole number
+    off = fmaxf(off, fabsf(y - c[i]));
   }
-  return near ? exact_codes(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), m, s) : w;
+  if (off > 0.49999f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = (x[i] - m) * inv, t = y - c[i];
+      if (fabsf(t) > 0.49999f && fabsf(t) < 0.6f) {  // a clamped quotient may be far off
+        const float below = t > 0.f ? c[i] : c[i] - 1.f, r = fmaf(-(below + 0.5f), s, x[i] - m);
+        const bool odd = (int)below & 1;
+        c[i] = fminf(fmaxf(r > 0.f || (r == 0.f && odd) ? below + 1.f : below, 0.f), 15.f);
+      }
+    }
+  }
+  uint32_t w = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // four codes as one number below 2^16
+    float sum = 8388608.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (kv4_nibble(i) >> 2 == h) sum = fmaf(c[i], (float)(1 << (4 * (kv4_nibble(i) & 3))), sum);
+    w |= (__float_as_uint(sum) & 0xffffu) << (16 * h);
+  }
+  return w;
 }
 
 // A group of D / 8 lanes takes the head vectors of one token one by one, 8 dims
@@ -209,19 +233,18 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
   const int mine = (threadIdx.x / L) >> a.shift, t = t0 + mine;
   const int first = blockIdx.x * per * a.each + (threadIdx.x / L & (per - 1));  // then every per-th: q heads, k, v
   const int n = mine < here && first < items ? min(a.each, (items - first + per - 1) >> a.shift) : 0;
-  auto vector_of = [&](int item, bool* vec) {
-    const bool is_q = item < a.q_heads, is_k = item < a.q_heads + kh;
-    const HeadRows& in = is_q ? a.q : is_k ? a.k : a.v;
-    const int head = item - (is_q ? 0 : is_k ? a.q_heads : a.q_heads + kh);
-    *vec = in.vec;
-    return static_cast<const __nv_bfloat16*>(in.p) + (int64_t)t * in.token + head * in.head;
+  // vector item of token t is at the base of its kind + item * its head stride
+  const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(a.q.p) + t * a.q.token + 8 * l;
+  const __nv_bfloat16* kb = static_cast<const __nv_bfloat16*>(a.k.p) + t * a.k.token - a.q_heads * a.k.head + 8 * l;
+  const __nv_bfloat16* vb = static_cast<const __nv_bfloat16*>(a.v.p) + t * a.v.token - (a.q_heads + kh) * a.v.head + 8 * l;
+  auto vector_of = [&](int item) {
+    return item < a.q_heads ? qb + item * a.q.head : item < a.q_heads + kh ? kb + item * a.k.head : vb + item * a.v.head;
   };
   auto fetch = [&](int i) {  // into a slot that was read a vector ago
     if (i < n) {
-      bool vec;
-      const __nv_bfloat16* p = vector_of(first + (i << a.shift), &vec) + 8 * l;
+      const __nv_bfloat16* p = vector_of(first + (i << a.shift));
       uint4* to = &ring[i % AP_RING][threadIdx.x];
-      if (vec) async_copy16(to, p);
+      if (a.vec) async_copy16(to, p);
       else *to = load8_raw(p, false);
     }
     async_commit();
@@ -238,6 +261,10 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
     async_wait<0>();
     return;
   }
+  __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(a.q_out.p) + t * a.q_out.token + 8 * l;
+  unsigned char* tile0 = pl.page < 0 ? nullptr : kv4_tile(a.cache, kv4_tile_bytes(D), pl.page, 0, pl.off >> 4);
+  const int k_off = kv4_k_off<D>(tok, l), v_off = kv4_codes(D) + kv4_v_off<D>(tok, l);
+  const int head_bytes = a.cache.tiles_per_page * kv4_tile_bytes(D);
   Turn turn;
   if (MODE != TURN_NONE && kind == 2 && first < a.q_heads + kh)
     load_turn<MODE>(turn, a.table + (int64_t)pl.pos * (a.rot >> 1), l, a.rot, a.interleaved);
@@ -257,8 +284,7 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
       x[2 * e + 1] = __uint_as_float(w4[e] & 0xffff0000u);
     }
     if (MODE != TURN_NONE && kind == 2 && (is_q || is_k)) {
-      bool vec;
-      turn8<MODE>(x, turn, MODE == TURN_ANY ? vector_of(item, &vec) : nullptr, l, a.rot, a.interleaved, group);
+      turn8<MODE>(x, turn, MODE == TURN_ANY ? vector_of(item) - 8 * l : nullptr, l, a.rot, a.interleaved, group);
     }
     if (is_q) {
       if (kind != 2) {
@@ -266,8 +292,7 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
         for (int e = 0; e < 8; ++e) x[e] = 0.f;
       }
       __syncwarp(group);  // q_out may be q: every lane has read its partners
-      store8_bf16(static_cast<__nv_bfloat16*>(a.q_out.p) + (int64_t)t * a.q_out.token + item * a.q_out.head + 8 * l,
-                  a.q_out.vec, x);
+      store8_bf16(ob + item * a.q_out.head, a.q_out.vec, x);
       continue;
     }
     float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
@@ -289,10 +314,8 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
       sf = 0.f;
     }
     const uint32_t w = sf > 0.f ? codes8(x, mf, sf) : 0u;
-    const int head = item - a.q_heads - (is_k ? 0 : kh);
-    unsigned char* tile = kv4_tile(a.cache, kv4_tile_bytes(D), pl.page, head, pl.off >> 4);
-    const int code = is_k ? kv4_k_off<D>(tok, l) : kv4_codes(D) + kv4_v_off<D>(tok, l);
-    *reinterpret_cast<uint32_t*>(tile + code) = w;
+    unsigned char* tile = tile0 + (int64_t)(item - a.q_heads - (is_k ? 0 : kh)) * head_bytes;
+    *reinterpret_cast<uint32_t*>(tile + (is_k ? k_off : v_off)) = w;
     if (l == 0) {
       const uint32_t pr = (uint32_t)__bfloat16_as_ushort(st) | ((uint32_t)__bfloat16_as_ushort(mn) << 16);
       *reinterpret_cast<uint32_t*>(tile + 2 * kv4_codes(D) + tok * 8 + (is_k ? 0 : 4)) = pr;
@@ -381,7 +404,8 @@ void launch_kv4_append(const Kv4View& cache, int D, const SeqView& seq, const in
   const int each = (int)std::min<int64_t>(AP_EACH, std::max<int64_t>(1, turns));
   int shift = 0;
   while ((1 << shift) < groups && (each << shift) < items) ++shift;
-  const AppendArgs a{cache, seq, positions, table, rot, interleaved, max_pos, q_heads, q, k, v, q_out, shift, each, err};
+  const AppendArgs a{cache, seq, positions, table, rot, interleaved, max_pos, q_heads, q, k, v, q_out,
+                     (q_heads == 0 || q.vec) && k.vec && v.vec, shift, each, err};
   const dim3 grid = token_grid(items, each << shift, seq.num_tokens, groups >> shift);
   if (D == 128) launch_append<128>(a, grid, st);
   else launch_append<64>(a, grid, st);
