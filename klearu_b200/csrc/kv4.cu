@@ -175,42 +175,25 @@ __device__ __noinline__ uint32_t exact_codes(float4 a, float4 b, float m, float 
     w |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[i] - m, s)), 0.f), 15.f) << (4 * kv4_nibble(i));
   return w;
 }
-// By a reciprocal: quotients off by at most 2^-23 of 15 decide unless one is
-// within 1e-5 of a border between two codes; there the sign of x - m - border * s
-// does, which one fused operation gives exactly, and on the border the even code.
-// (Values of 8 bits are often on one: a call with divisions for those took as
-// long as all the rest.)
+// The same by a reciprocal: y = d inv, and y + (d - y s) inv, the bracket in one
+// fused operation, is the quotient d / s rounded correctly (Markstein, 1990),
+// since inv is 1 / s rounded correctly.
+__device__ __forceinline__ float quotient(float d, float s, float inv) {
+  const float y = d * inv;
+  return fmaf(fmaf(-y, s, d), inv, y);
+}
 __device__ __forceinline__ uint32_t codes8(const float* x, float m, float s) {
   if (!(s > 1e-30f && s < 1e30f)) return exact_codes(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), m, s);
   const float inv = __frcp_rn(s);
-  float c[8], off = 0.f;
+  // + 2^23 rounds to a whole number, which stands in the low bits of 0x4b000000 + c
+  uint32_t w = 0u, over = 0u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float y = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
-    c[i] = (y + 8388608.f) - 8388608.f;  // 2^23: to a whole number
-    off = fmaxf(off, fabsf(y - c[i]));
+    const float y = fminf(fmaxf(quotient(x[i] - m, s, inv), 0.f), 15.f) + 8388608.f;
+    w += __float_as_uint(y) << (4 * kv4_nibble(i));
+    over += 0x4b000000u << (4 * kv4_nibble(i));
   }
-  if (off > 0.49999f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = (x[i] - m) * inv, t = y - c[i];
-      if (fabsf(t) > 0.49999f && fabsf(t) < 0.6f) {  // a clamped quotient may be far off
-        const float below = t > 0.f ? c[i] : c[i] - 1.f, r = fmaf(-(below + 0.5f), s, x[i] - m);
-        const bool odd = (int)below & 1;
-        c[i] = fminf(fmaxf(r > 0.f || (r == 0.f && odd) ? below + 1.f : below, 0.f), 15.f);
-      }
-    }
-  }
-  uint32_t w = 0;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {  // four codes as one number below 2^16
-    float sum = 8388608.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (kv4_nibble(i) >> 2 == h) sum = fmaf(c[i], (float)(1 << (4 * (kv4_nibble(i) & 3))), sum);
-    w |= (__float_as_uint(sum) & 0xffffu) << (16 * h);
-  }
-  return w;
+  return w - over;
 }
 
 // A group of D / 8 lanes takes the head vectors of one token one by one, 8 dims
@@ -218,10 +201,11 @@ __device__ __forceinline__ uint32_t codes8(const float* x, float m, float s) {
 // (D = 128) or 32 groups are dealt to one or more tokens.  Each thread's 16 bytes
 // of a vector come through a ring of its own in shared memory, three vectors
 // ahead, which keeps the registers for four blocks an SM.
-// 8000 tokens of 48 heads of 128, half of each turned: 51 us, 3.4 TB/s; what is
-// left is the latency of a block's chain (sequence, page, table, vectors).  A head
-// vector of several tokens to a group, table rows loaded again for each: 20% to
-// 35% slower; without the ring, two tokens in registers: 15% more.
+// 8000 tokens of 32 + 16 heads of 128, half of each turned: 45 us, 3.9 TB/s, with
+// three of four issue slots taken: the codes of a key or value cost 250
+// instructions a warp, a query 115.  A head vector of several tokens to a group,
+// the table rows loaded again for each, was 20% to 35% slower; two tokens in
+// registers instead of the ring 15%; quotients on a border taken as divisions 10%.
 template <int D, int MODE>
 __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs a) {
   constexpr int L = D / 8;  // lanes of a group
@@ -233,19 +217,29 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
   const int mine = (threadIdx.x / L) >> a.shift, t = t0 + mine;
   const int first = blockIdx.x * per * a.each + (threadIdx.x / L & (per - 1));  // then every per-th: q heads, k, v
   const int n = mine < here && first < items ? min(a.each, (items - first + per - 1) >> a.shift) : 0;
-  // vector item of token t is at the base of its kind + item * its head stride
-  const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(a.q.p) + t * a.q.token + 8 * l;
-  const __nv_bfloat16* kb = static_cast<const __nv_bfloat16*>(a.k.p) + t * a.k.token - a.q_heads * a.k.head + 8 * l;
-  const __nv_bfloat16* vb = static_cast<const __nv_bfloat16*>(a.v.p) + t * a.v.token - (a.q_heads + kh) * a.v.head + 8 * l;
-  auto vector_of = [&](int item) {
-    return item < a.q_heads ? qb + item * a.q.head : item < a.q_heads + kh ? kb + item * a.k.head : vb + item * a.v.head;
+  auto vector_of = [&](int item, int64_t* head, int* end) {  // and its kind's head stride and first item after
+    const bool is_q = item < a.q_heads, is_k = item < a.q_heads + kh;
+    const HeadRows& in = is_q ? a.q : is_k ? a.k : a.v;
+    const int from = is_q ? 0 : is_k ? a.q_heads : a.q_heads + kh;
+    *head = in.head;
+    *end = is_q ? a.q_heads : from + kh;
+    return static_cast<const __nv_bfloat16*>(in.p) + t * in.token + (item - from) * in.head + 8 * l;
   };
-  auto fetch = [&](int i) {  // into a slot that was read a vector ago
-    if (i < n) {
-      const __nv_bfloat16* p = vector_of(first + (i << a.shift));
-      uint4* to = &ring[i % AP_RING][threadIdx.x];
-      if (a.vec) async_copy16(to, p);
-      else *to = load8_raw(p, false);
+  // what is fetched next: its address moves on by a step while the kind stays the same
+  int coming = first, kind_end = 0;
+  const int stop = first + (n << a.shift);
+  int64_t step = 0;
+  const __nv_bfloat16* from = nullptr;
+  auto fetch = [&](int slot) {  // into a slot that was read a vector ago
+    if (coming < stop) {
+      if (coming >= kind_end) {
+        from = vector_of(coming, &step, &kind_end);
+        step <<= a.shift;
+      }
+      if (a.vec) async_copy16(&ring[slot][threadIdx.x], from);
+      else ring[slot][threadIdx.x] = load8_raw(from, false);
+      coming += per;
+      from += step;
     }
     async_commit();
   };
@@ -257,25 +251,29 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
   if (n == 0) return;
   const Place pl = places[mine];
   const int kind = pl.kind, tok = pl.off & 15;
-  if (kind == 0) {
+  __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(a.q_out.p) + t * a.q_out.token + first * a.q_out.head + 8 * l;
+  const int64_t out_step = a.q_out.head << a.shift;
+  if (kind != 2) {
     async_wait<0>();
+    const float none[8] = {};
+    if (kind == 1)
+      for (int item = first; item < min(stop, a.q_heads); item += per, ob += out_step) store8_bf16(ob, a.q_out.vec, none);
     return;
   }
-  __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(a.q_out.p) + t * a.q_out.token + 8 * l;
   unsigned char* tile0 = pl.page < 0 ? nullptr : kv4_tile(a.cache, kv4_tile_bytes(D), pl.page, 0, pl.off >> 4);
   const int k_off = kv4_k_off<D>(tok, l), v_off = kv4_codes(D) + kv4_v_off<D>(tok, l);
   const int head_bytes = a.cache.tiles_per_page * kv4_tile_bytes(D);
   Turn turn;
-  if (MODE != TURN_NONE && kind == 2 && first < a.q_heads + kh)
+  if (MODE != TURN_NONE && first < a.q_heads + kh)
     load_turn<MODE>(turn, a.table + (int64_t)pl.pos * (a.rot >> 1), l, a.rot, a.interleaved);
 
-  for (int i = 0; i < n; ++i) {
-    fetch(i + AP_RING - 1);
+  int slot = 0;
+  for (int item = first; item < stop; item += per) {
+    fetch((slot + AP_RING - 1) % AP_RING);
     async_wait<AP_RING - 1>();
-    const int item = first + (i << a.shift);
+    const uint4 raw = ring[slot][threadIdx.x];
+    slot = (slot + 1) % AP_RING;
     const bool is_q = item < a.q_heads, is_k = !is_q && item < a.q_heads + kh;
-    if (!is_q && (kind != 2 || pl.page < 0)) continue;
-    const uint4 raw = ring[i % AP_RING][threadIdx.x];
     const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
     float x[8];
 #pragma unroll
@@ -283,18 +281,19 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
       x[2 * e] = __uint_as_float(w4[e] << 16);
       x[2 * e + 1] = __uint_as_float(w4[e] & 0xffff0000u);
     }
-    if (MODE != TURN_NONE && kind == 2 && (is_q || is_k)) {
-      turn8<MODE>(x, turn, MODE == TURN_ANY ? vector_of(item) - 8 * l : nullptr, l, a.rot, a.interleaved, group);
+    if (MODE != TURN_NONE && (is_q || is_k)) {
+      int64_t head;
+      int end;
+      const __nv_bfloat16* p = MODE == TURN_ANY ? vector_of(item, &head, &end) - 8 * l : nullptr;
+      turn8<MODE>(x, turn, p, l, a.rot, a.interleaved, group);
     }
     if (is_q) {
-      if (kind != 2) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f;
-      }
-      __syncwarp(group);  // q_out may be q: every lane has read its partners
-      store8_bf16(ob + item * a.q_out.head, a.q_out.vec, x);
+      if (MODE == TURN_ANY) __syncwarp(group);  // q_out may be q: every lane has read its partners
+      store8_bf16(ob, a.q_out.vec, x);
+      ob += out_step;
       continue;
     }
+    if (pl.page < 0) break;  // no place in the cache for this and what follows
     float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
     float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     // 0 * x is 0 for a finite x, else NaN
@@ -306,7 +305,9 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
     }
     const bool fin = __all_sync(group, z == 0.f);
     // 8 bits for step and minimum: the codes are taken against the rounded values
-    __nv_bfloat16 st = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.f)), mn = __float2bfloat16_rn(lo);
+    const float range = hi - lo;
+    __nv_bfloat16 st = __float2bfloat16_rn(range > 1e-30f ? quotient(range, 15.f, 1.f / 15.f) : __fdiv_rn(range, 15.f));
+    __nv_bfloat16 mn = __float2bfloat16_rn(lo);
     float sf = to_f(st), mf = to_f(mn);
     if (!fin || !finite_f(sf) || !finite_f(mf)) {
       st = __ushort_as_bfloat16(0);
@@ -321,6 +322,7 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
       *reinterpret_cast<uint32_t*>(tile + 2 * kv4_codes(D) + tok * 8 + (is_k ? 0 : 4)) = pr;
     }
   }
+  async_wait<0>();  // rows that were not taken
 }
 
 struct ReadArgs {
@@ -397,8 +399,8 @@ void launch_kv4_append(const Kv4View& cache, int D, const SeqView& seq, const in
                        int rot, int interleaved, int64_t max_pos, int q_heads, const HeadRows& q, const HeadRows& k,
                        const HeadRows& v, const HeadRows& q_out, int* err, cudaStream_t st) {
   // One vector a group while that gives each processor two blocks at most, up to AP_EACH for more.  48 heads of 128:
-  // 64 tokens take 8.3 us with one or four each and 10.4 with eight, 500 tokens 14.2, 10.4 and 12.5, 8000 tokens 108,
-  // 74 and 66 and with twelve 63.
+  // 64 tokens and reading them back take 8.3 us with one or four each and 10.4 with eight, 500 tokens 14.2, 10.4 and
+  // 12.5, 8000 tokens 108, 74 and 66 and with twelve 63.
   const int items = q_heads + 2 * cache.kv_heads, groups = AP_NT / (D / 8);
   const int64_t turns = (int64_t)items * seq.num_tokens / ((int64_t)groups * 2 * 148);
   const int each = (int)std::min<int64_t>(AP_EACH, std::max<int64_t>(1, turns));
