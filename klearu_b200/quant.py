@@ -29,9 +29,10 @@ class Q8Rows(NamedTuple):
 
 def _two(t: torch.Tensor, what: str) -> int:
     """The row stride of a 2-D tensor that is contiguous in its last dimension."""
-    if t.dim() != 2 or (t.stride(1) != 1 and t.numel()):
+    stride, shape = t.stride(), t.shape
+    if len(shape) != 2 or (stride[1] != 1 and t.numel()):
         raise ValueError(f"{what} must be 2-D, contiguous in its last dimension")
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+    return stride[0] if shape[0] > 1 else max(shape[1], stride[0])
 
 
 def _rows_q8(x, weight, residual, eps, norm, one_plus, hidden, ctx) -> Q8Rows:
@@ -80,8 +81,8 @@ def add_rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tenso
     ``one_plus_weight``).  ``hidden`` receives h; pass ``residual`` itself to
     update the residual stream in place; by default, with a residual, a new
     tensor.  A row that is not finite gets scale NaN."""
-    if hidden is None and residual is not None:
-        hidden = x.new_empty(x.shape, dtype=torch.float32)
+    if hidden is None and isinstance(residual, torch.Tensor):
+        hidden = torch.empty_like(residual, memory_format=torch.contiguous_format)
     return _rows_q8(x, weight, residual, eps, 1, one_plus_weight, hidden, ctx)
 
 
@@ -148,10 +149,12 @@ class Q8Linear:
             if out_dtype not in (torch.float32, torch.bfloat16):
                 raise ValueError("out_dtype must be float32 or bfloat16")
             out = codes.new_empty((rows, self.out_features), dtype=out_dtype)
-        want(self.ctx, out, "out", torch.float32 if accumulate else (torch.float32, torch.bfloat16))
-        ldo = _two(out, "out")
-        if out.shape != (rows, self.out_features):
-            raise ValueError("out must be [rows][out_features]")
+            ldo = self.out_features
+        else:
+            want(self.ctx, out, "out", torch.float32 if accumulate else (torch.float32, torch.bfloat16))
+            ldo = _two(out, "out")
+            if out.shape != (rows, self.out_features):
+                raise ValueError("out must be [rows][out_features]")
         if rows:
             launch(self.ctx, "kl_q8_linear_forward", self.h, codes.data_ptr(), ld, scales.data_ptr(), rows,
                    out.data_ptr(), _lib.DTYPE_BF16 if out.dtype == torch.bfloat16 else _lib.DTYPE_F32, ldo,
