@@ -73,9 +73,10 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // keeps the largest so far within f16, rounded to 11 bits (2^-12), and what is
 // 2^-25 below the largest to none.  Sums, maxima and O are f32.
 //
-// Bound by memory, D + 8 bytes a token and key head; per 16 tokens a warp
-// spends about 90 logic instructions on the nibbles, half the rate at which
-// the memory delivers them.
+// D + 8 bytes a token and key head.  64 sequences of up to 16384 tokens, D = 128,
+// 8 key heads of 4 rows: 147 us, 4.0 TB/s of 6.4; one of 131071: 43 us, 3.3 TB/s.
+// Not the memory but the work on the nibbles bounds it: about 300 instructions a
+// warp for 16 tokens, half of them logic, which has half the issue rate.
 template <int D, int NR>
 __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kernel(AttendArgs a, SplitPlan p) {
   constexpr int TB = kv4_tile_bytes(D), CODES = kv4_codes(D);
