@@ -759,7 +759,7 @@ KL_API kl_status kl_kv4_read(kl_kv4_t cache, const kl_seq_batch* seqs_host, cons
  * tokens j <= i of its sequence, and with window > 0 only i - window < j.
  * Query head h reads key head h / (q_heads / kv_heads).  A token that sees
  * nothing gets zeros; keys that a token does not see have no effect on it, be
- * they NaN.  workspace: kl_kv4_attend_workspace bytes for the same arguments,
+ * they NaN.  out may be q itself.  workspace: kl_kv4_attend_workspace bytes for the same arguments,
  * 16-byte aligned, used until the launched work is done (graphs that may run at
  * the same time need one each). */
 KL_API kl_status kl_kv4_attend_workspace(kl_kv4_t cache, const kl_seq_batch* seqs_host, int q_heads, int window,

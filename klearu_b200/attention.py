@@ -179,6 +179,16 @@ class Kv4Cache:
             raise ValueError(f"{what} has shape {tuple(shape)}, expected {tokens} tokens and {heads} heads")
         return C.byref(HeadRowsC(t.data_ptr(), stride[0], stride[1]))
 
+    def _out(self, t: torch.Tensor, what: str, tokens: int, heads: int):
+        """``_rows`` of a tensor to be written, whose rows must lie apart."""
+        r = self._rows(t, what, tokens, heads)
+        reach = self.head_dim  # of the rows so far, from the closest together to the farthest apart
+        for step, n in sorted((s, n) for s, n in zip(t.stride(), t.shape[:2]) if n > 1):
+            if step < reach:
+                raise ValueError(f"{what}'s rows overlap")
+            reach += step * (n - 1)
+        return r
+
     def _new(self, like: torch.Tensor, tokens: int, heads: int):
         """A new [tokens][heads][head_dim] tensor and its C rows."""
         d = self.head_dim
@@ -198,8 +208,9 @@ class Kv4Cache:
         the cache; returns the turned q [tokens][q_heads][head_dim] (``q_out`` if
         given, which may be q).  Rows of no sequence are left as they are.  Two
         rows must not name the same token of the same page."""
-        t = k.shape[0] if k.dim() else 0
-        rk, rv = self._rows(k, "k", heads=self.kv_heads), self._rows(v, "v", t, self.kv_heads)
+        rk = self._rows(k, "k", heads=self.kv_heads)
+        t = k.shape[0]
+        rv = self._rows(v, "v", t, self.kv_heads)
         heads, rq, ro = 0, None, None
         if q is not None:
             rq = self._rows(q, "q", t)
@@ -207,7 +218,7 @@ class Kv4Cache:
             if q_out is None:
                 q_out, ro = self._new(q, t, heads)
             else:
-                ro = self._rows(q_out, "q_out", t, heads)
+                ro = self._out(q_out, "q_out", t, heads)
         elif q_out is not None:
             raise ValueError("q_out without q")
         if positions is not None:
@@ -243,7 +254,7 @@ class Kv4Cache:
                 k_out = torch.empty_like(v_out)
             elif v_out is None:
                 v_out = torch.empty_like(k_out)
-            rk, rv = self._rows(k_out, "k_out", num_tokens, heads), self._rows(v_out, "v_out", num_tokens, heads)
+            rk, rv = self._out(k_out, "k_out", num_tokens, heads), self._out(v_out, "v_out", num_tokens, heads)
         if num_tokens:
             launch(self.ctx, "kl_kv4_read", self.h, c, rk, rv)
         return k_out, v_out
@@ -255,17 +266,18 @@ class Kv4Cache:
         h // (q_heads / kv_heads)).  A token sees the tokens up to its own number
         in its sequence, and with ``window`` only the last ``window`` of those;
         one that sees nothing gets zeros.  ``scale`` defaults to
-        head_dim ** -0.5.  Returns ``out`` (allocated if None), rows of no
-        sequence left as they are."""
+        head_dim ** -0.5.  Returns ``out`` (allocated if None; it may be q), rows
+        of no sequence left as they are."""
         rq = self._rows(q, "q")
         t, heads = q.shape[0], q.shape[1]
         if out is None:
             out, ro = self._new(q, t, heads)
         else:
-            ro = self._rows(out, "out", t, heads)
+            ro = self._out(out, "out", t, heads)
         c = self._batch(batch, t)
         if t == 0 or heads == 0:
             return out
+        window = min(window, 2**31 - 1)
         key = (batch.sizes, t, heads, window)
         need = self._workspace.get(key)
         if need is None:

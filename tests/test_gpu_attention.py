@@ -207,8 +207,8 @@ def test_append_of_many_tokens(gpu_ctx, dim, interleaved, rot):
     assert (off > R.HALF * step).double().mean() < 1e-3
 
 
-def test_more_tokens_than_a_grid_is_high(gpu_ctx):
-    t = 4 * 65535 + 77
+@pytest.mark.parametrize("t", [4 * 65535 + 77, 32 * 65535 + 77])
+def test_more_tokens_than_a_grid_is_high(gpu_ctx, t):
     batch, pages = make_batch([t], [t], 1024)
     cache = Kv4Cache(pages, 1024, 1, 64, ctx=gpu_ctx)
     k, v = randn(t, 1, 64, seed=1), randn(t, 1, 64, seed=2)

@@ -6,6 +6,9 @@ same stream; prompts, single tokens, captured graphs and streams.
 Each part is compared with its plain 64-bit form on the inputs that it got."""
 
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -254,3 +257,71 @@ def test_c_entry_points_refuse(gpu_ctx):
     with pytest.raises(KlError):
         check(lib.kl_kv4_append(cache.h, None, C.byref(s), None, 0, None, None, C.byref(rows), None), gpu_ctx.h)
     gpu_ctx.sync()
+
+
+FIRST = """
+import torch
+from klearu_b200.attention import Kv4Cache, RopeTable, SeqBatch
+from klearu_b200.quant import Q8Linear, add_rms_norm_q8
+dev = "cuda:0"
+i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+x, w = torch.randn(600, 256, device=dev), torch.ones(256, device=dev)
+wide = Q8Linear(torch.ones(9000, 256, dtype=torch.int8, device=dev), torch.ones(9000, device=dev))
+cache, rope = Kv4Cache(64, 64, 8, 64), RopeTable(64, 4096)
+qkv = torch.randn(600, 24, 64, device=dev, dtype=torch.bfloat16)
+table = torch.arange(64, dtype=torch.int32, device=dev).view(1, 64)
+prompt = SeqBatch(i32([0, 600]), i32([600]), table, max_q=600, max_kv=600)
+token = SeqBatch(i32([0, 1]), i32([600]), table, max_q=1, max_kv=4096)
+
+def run():
+    r = add_rms_norm_q8(x, w)
+    y = [wide.forward(r.codes[:n], r.scales[:n]) for n in (1, 40, 600)]
+    q = cache.append(qkv[:, 8:16], qkv[:, 16:], prompt, q=qkv[:, :8], rope=rope)
+    k, v = cache.read(prompt, 600)
+    o = [cache.attend(q, prompt), cache.attend(q[:1], token), cache.attend(torch.cat([q] * 4, 1), prompt)]
+    return [r.codes, r.scales, *y, q, k, v, *o]
+
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = run()
+g.replay()
+want = run()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("captured first")
+"""
+
+
+def test_first_calls_can_be_captured(gpu_ctx):
+    """In a process of its own: no call needs to have run before it is captured."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=root)
+    done = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=240, env=env)
+    assert done.returncode == 0 and "captured first" in done.stdout, done.stderr[-2000:]
+
+
+def test_outputs_that_overlap_and_in_place(gpu_ctx):
+    cache = Kv4Cache(64, 16, 2, 64, ctx=gpu_ctx)
+    table = i32([list(range(64))])
+    every = SeqBatch(i32([0, 1000]), i32([1000]), table, max_q=1000)
+    k, v = randn(1000, 2, 64, seed=1, dtype=torch.bfloat16), randn(1000, 2, 64, seed=2, dtype=torch.bfloat16)
+    cache.append(k, v, every)
+    for n in (1, 5, 200):
+        batch = SeqBatch(i32([0, n]), i32([1000]), table, max_q=n)
+        q = randn(n, 4, 64, seed=3, dtype=torch.bfloat16)
+        want = cache.attend(q, batch)
+        assert torch.equal(cache.attend(q, batch, window=2**40), want)
+        assert cache.attend(q, batch, out=q) is q and torch.equal(q, want)
+    q = randn(8, 4, 64, dtype=torch.bfloat16)
+    batch = SeqBatch(i32([0, 8]), i32([1000]), table, max_q=8)
+    flat = torch.zeros(8 * 4 * 64, dtype=torch.bfloat16, device=DEV)
+    for bad in (flat[:256].view(1, 4, 64).expand(8, 4, 64), flat[:512].view(8, 1, 64).expand(8, 4, 64),
+                flat.as_strided((8, 4, 64), (128, 64, 1)), flat.as_strided((8, 4, 64), (64, 64, 1))):
+        with pytest.raises(ValueError):
+            cache.attend(q, batch, out=bad)
+        with pytest.raises(ValueError):
+            cache.append(k[:8], v[:8], batch, q=q, q_out=bad)
+    fine = flat.as_strided((8, 4, 64), (64, 512, 1))  # heads outside, tokens inside
+    assert torch.equal(cache.attend(q, batch, out=fine), cache.attend(q, batch))
+    with pytest.raises(ValueError):
+        cache.append("k", v, batch)
