@@ -7,6 +7,7 @@
 // engine's own.
 #include "engine.h"
 #include "kv4.cuh"
+#include "pdl.cuh"
 
 namespace kl {
 namespace {
@@ -243,6 +244,8 @@ __global__ void __launch_bounds__(AP_NT, AP_BLOCKS) kv4_append_kernel(AppendArgs
     }
     async_commit();
   };
+  begin_next();
+  after_before();
 #pragma unroll
   for (int i = 0; i < AP_RING - 1; ++i) fetch(i);  // before their places are known
   find_places(a.cache, a.seq, a.positions, t0, here, MODE != TURN_NONE, a.max_pos, places, a.err);
@@ -343,6 +346,8 @@ __global__ void __launch_bounds__(AP_NT) kv4_read_kernel(ReadArgs a) {
   const int l = threadIdx.x % L, item = blockIdx.x * PER + threadIdx.x / L;
   const int t0 = (int)(((int64_t)blockIdx.z * 65535 + blockIdx.y) * a.tokens);
   const int n = min(a.tokens, a.seq.num_tokens - t0);
+  begin_next();
+  after_before();
   find_places(a.cache, a.seq, nullptr, t0, n, false, 0, places, a.err);
   __syncthreads();
   if (item >= 2 * kh) return;
@@ -382,10 +387,10 @@ dim3 token_grid(int items, int per, int tokens, int each) {
 
 template <int D>
 void launch_append(const AppendArgs& a, dim3 grid, cudaStream_t st) {
-  if (!a.table) kv4_append_kernel<D, TURN_NONE><<<grid, AP_NT, 0, st>>>(a);
-  else if (a.interleaved && a.rot % 8 == 0) kv4_append_kernel<D, TURN_PAIRS><<<grid, AP_NT, 0, st>>>(a);
-  else if (!a.interleaved && a.rot % 16 == 0) kv4_append_kernel<D, TURN_HALVES><<<grid, AP_NT, 0, st>>>(a);
-  else kv4_append_kernel<D, TURN_ANY><<<grid, AP_NT, 0, st>>>(a);
+  auto* kernel = !a.table ? kv4_append_kernel<D, TURN_NONE>
+                 : a.interleaved ? a.rot % 8 == 0 ? kv4_append_kernel<D, TURN_PAIRS> : kv4_append_kernel<D, TURN_ANY>
+                 : a.rot % 16 == 0 ? kv4_append_kernel<D, TURN_HALVES> : kv4_append_kernel<D, TURN_ANY>;
+  launch_next(kernel, grid, AP_NT, 0, st, a);
 }
 
 }  // namespace
@@ -419,8 +424,7 @@ void launch_kv4_read(const Kv4View& cache, int D, const SeqView& seq, const Head
   const int items = 2 * cache.kv_heads, per = AP_NT / (D / 8), each = block_tokens(items, per, seq.num_tokens);
   const ReadArgs a{cache, seq, k, v, each, err};
   const dim3 grid = token_grid(items, per, seq.num_tokens, each);
-  if (D == 128) kv4_read_kernel<128><<<grid, AP_NT, 0, st>>>(a);
-  else kv4_read_kernel<64><<<grid, AP_NT, 0, st>>>(a);
+  launch_next(D == 128 ? kv4_read_kernel<128> : kv4_read_kernel<64>, grid, AP_NT, 0, st, a);
   count_launch();
 }
 

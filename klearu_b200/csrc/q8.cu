@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "engine.h"
+#include "pdl.cuh"
 #include "tcgen05.cuh"
 
 namespace kl {
@@ -70,6 +71,8 @@ template <int NV, class T>
 __global__ void __launch_bounds__(1024) norm_q8_vec_kernel(NormQ8Args a) {
   __shared__ float2 tmp[32];
   __shared__ unsigned long long top_s;
+  begin_next();
+  after_before();
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const float* r = a.residual ? a.residual + row * a.ldr : nullptr;
@@ -198,6 +201,8 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const float* r = a.residual ? a.residual + row * a.ldr : nullptr;
   float* ho = a.hidden ? a.hidden + row * a.ldh : nullptr;
+  begin_next();
+  after_before();
   if (threadIdx.x == 0) top_s = 0ull;
   float ss = 0.f, mx = 0.f;
   bool fin = true;
@@ -327,22 +332,28 @@ struct Q8Ring {
     }
   }
 };
+// One chunk of K of a tile: its weights, announcing both, and its rows.
+__device__ __forceinline__ void q8_load_w(const int8_t* tile, const Q8Tile& t, unsigned char* sm, uint64_t* full, int stage) {
+  const int size = Q8_WTILE + t.nt * Q8_KB;
+  mbar_arrive_expect_tx(full + stage, (uint32_t)size);
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(sm + stage * size)),
+      "l"(tile), "r"(Q8_WTILE), "r"(smem_u32(full + stage))
+      : "memory");
+}
+__device__ __forceinline__ void q8_load_a(const CUtensorMap* am, const Q8Tile& t, unsigned char* sm, uint64_t* full, int c,
+                                          int row, int stage) {
+  tma_load_2d(sm + stage * (Q8_WTILE + t.nt * Q8_KB) + Q8_WTILE, am, c * Q8_KB, row, full + stage);
+}
 // The loading side of a tile: K chunks [c0, c1) through the ring.  False when a
 // wait gave up.
 __device__ __forceinline__ bool q8_load(const int8_t* w, const CUtensorMap* am, const Q8Tile& t, unsigned char* sm,
                                         uint64_t* full, uint64_t* empty, int ch, int row, int c0, int c1, Q8Ring& q) {
   const int8_t* tile = w + ((int64_t)(ch >> 7) * t.kc + c0) * Q8_WTILE;
-  const int size = Q8_WTILE + t.nt * Q8_KB;
   for (int c = c0; c < c1; ++c, q.next(t.stages), tile += Q8_WTILE) {
-    uint64_t* bar = full + q.stage;
-    unsigned char* to = sm + q.stage * size;
     if (q.round > 0 && !mbar_wait(&empty[q.stage], (q.round - 1) & 1u)) return false;
-    mbar_arrive_expect_tx(bar, (uint32_t)size);
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(to)),
-        "l"(tile), "r"(Q8_WTILE), "r"(smem_u32(bar))
-        : "memory");
-    tma_load_2d(to + Q8_WTILE, am, c * Q8_KB, row, bar);
+    q8_load_w(tile, t, sm, full, q.stage);
+    q8_load_a(am, t, sm, full, c, row, q.stage);
   }
   return true;
 }
@@ -398,16 +409,21 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
     mbar_init(&done, 1);
     fail = 0;
     fence_mbar_init();
-    // the ring's first fills go out before anything else is ready
-    q8_load(a.w, &am, t, sm, full, empty, ch, row, c0, first, q);
+    // the ring's first fills go out before anything else is ready, the weights before the rows are
+    const int8_t* tile = a.w + ((int64_t)(ch >> 7) * t.kc + c0) * Q8_WTILE;
+    for (int i = c0; i < first; ++i, tile += Q8_WTILE) q8_load_w(tile, t, sm, full, i - c0);
+    after_before();
+    for (int i = c0; i < first; ++i, q.next(t.stages)) q8_load_a(&am, t, sm, full, i, row, q.stage);
   }
   // what the end needs, while the ring fills
   const float sw = c < a.n ? a.w_scale[c] : 0.f, bias = a.bias && c < a.n ? a.bias[c] : 0.f;
+  after_before();
   for (int j = threadIdx.x; j < t.nt; j += 128) sa[j] = row + j < a.m ? a.a_scale[row + j] : 0.f;
   if (warp == 1) tc5_alloc(&tmem_s, t.tmem_cols);
   tc5_fence_before();
   __syncthreads();
   tc5_fence_after();
+  begin_next();  // not before this block has its tensor memory, which the next one's may wait for
   const uint32_t tmem = tmem_s;
   if (warp == 0 && lane == 0) {
     if (!q8_load(a.w, &am, t, sm, full, empty, ch, row, first, c1, q)) atomicExch(&fail, 1);
@@ -586,7 +602,9 @@ __global__ void __launch_bounds__(Q8_VW * 32) q8_vector_kernel(Q8Args a) {
       x[1][u] = in ? __ldcs(reinterpret_cast<const uint4*>(p + Q8_KB + (((i & 7) ^ (s0 + 1)) << 4))) : make_uint4(0, 0, 0, 0);
     }
   };
+  begin_next();
   load(0);  // the first weights on their way while the rows are staged
+  after_before();
   for (int i = threadIdx.x; i < M * words; i += Q8_VW * 32) {
     const int r = i / words, at = (i - r * words) * 16;
     uint4 v = make_uint4(0, 0, 0, 0);
@@ -659,11 +677,9 @@ void launch_norm_q8(const NormQ8Args& a, int rows, cudaStream_t st) {
     // The plain kernel takes 14.5, 21.2 and 247: rows that are not aligned, and more than 16384 columns.
     const bool two = a.cols > 8192 || rows > 296;
     const int threads = (int)round_up(ceil_div(a.cols, two ? 16 : 8), 32);
-    if (a.x_bf16)
-      two ? norm_q8_vec_kernel<2, __nv_bfloat16><<<rows, threads, 0, st>>>(a)
-          : norm_q8_vec_kernel<1, __nv_bfloat16><<<rows, threads, 0, st>>>(a);
-    else
-      two ? norm_q8_vec_kernel<2, float><<<rows, threads, 0, st>>>(a) : norm_q8_vec_kernel<1, float><<<rows, threads, 0, st>>>(a);
+    auto* kernel = a.x_bf16 ? two ? norm_q8_vec_kernel<2, __nv_bfloat16> : norm_q8_vec_kernel<1, __nv_bfloat16>
+                            : two ? norm_q8_vec_kernel<2, float> : norm_q8_vec_kernel<1, float>;
+    launch_next(kernel, dim3(rows), threads, 0, st, a);
     count_launch();
     return;
   }
@@ -674,8 +690,7 @@ void launch_norm_q8(const NormQ8Args& a, int rows, cudaStream_t st) {
                          NORM_Q8_MAX_COLS * 4);
   });
   const size_t sm = (size_t)a.cols * 4;
-  if (a.x_bf16) norm_q8_kernel<256, __nv_bfloat16><<<rows, 256, sm, st>>>(a);
-  else norm_q8_kernel<256, float><<<rows, 256, sm, st>>>(a);
+  launch_next(a.x_bf16 ? norm_q8_kernel<256, __nv_bfloat16> : norm_q8_kernel<256, float>, dim3(rows), 256, sm, st, a);
   count_launch();
 }
 
@@ -735,8 +750,7 @@ static bool launch_q8(const Q8Args& a, cudaStream_t st) {
   if (a.m <= 2 && a.m * kc * Q8_KB <= 16 * 1024) {
     const unsigned grid = (unsigned)ceil_div(a.n, 2 * Q8_VW);
     const size_t sm = (size_t)(a.m * kc * Q8_KB);
-    if (a.m == 1) q8_vector_kernel<OUT, 1><<<grid, Q8_VW * 32, sm, st>>>(a);
-    else q8_vector_kernel<OUT, 2><<<grid, Q8_VW * 32, sm, st>>>(a);
+    launch_next(a.m == 1 ? q8_vector_kernel<OUT, 1> : q8_vector_kernel<OUT, 2>, dim3(grid), Q8_VW * 32, sm, st, a);
     count_launch();
     return true;
   }
@@ -770,11 +784,13 @@ static bool launch_q8(const Q8Args& a, cudaStream_t st) {
   cfg.blockDim = 128;
   cfg.dynamicSmemBytes = bytes + 1024;
   cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim = {(unsigned)p.splits, 1, 1};
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)p.splits, 1, 1};
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
   cfg.gridDim = dim3((unsigned)(ch * p.splits), (unsigned)row_tiles, 1);
   cudaLaunchKernelEx(&cfg, q8_split_kernel<OUT>, am, a, t, p.splits);
   count_launch();

@@ -186,6 +186,43 @@ def test_streams_and_graphs_at_once(gpu_ctx):
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
 
 
+def test_kernels_that_begin_early(gpu_ctx):
+    """Calls one behind the other, where a kernel may begin while the one before ends, give what they give with a
+    wait after each; buffers are written again by the next call as soon as the last has read them."""
+    layer, twin = Layer(gpu_ctx, 4, 700), Layer(gpu_ctx, 4, 700)
+    wide = Q8Linear.from_weights(randn(700, layer.hidden, seed=20), ctx=gpu_ctx)
+    back = Q8Linear.from_weights(randn(layer.hidden, 700, seed=21) / 700, ctx=gpu_ctx)
+
+    def run(x, wait):
+        length, got = 0, []
+        hidden = None
+        for step in range(60):
+            n = 37 if step % 20 == 0 else 1
+            length += n
+            batch = SeqBatch(i32([0, n, 2 * n, 3 * n, 4 * n]), i32([length] * 4), x.table, max_q=n)
+            if hidden is None or hidden.shape[0] != 4 * n:
+                hidden = randn(4 * n, x.hidden, seed=step)
+            for _ in range(3):
+                rows = add_rms_norm_q8(hidden, x.norm, ctx=gpu_ctx)
+                wait()
+                up = wide.forward(rows.codes, rows.scales)
+                wait()
+                rows = quantize_rows_q8(up, ctx=gpu_ctx)
+                wait()
+                back.forward(rows.codes, rows.scales, out=hidden, accumulate=True)
+                wait()
+            x(hidden, batch)
+            wait()
+            hidden /= hidden.abs().amax()
+            got.append(hidden.clone())
+        return got
+
+    slow = run(twin, torch.cuda.synchronize)
+    for _ in range(3):
+        fast = run(layer, lambda: None)
+        assert all(torch.equal(a, b) for a, b in zip(fast, slow))
+
+
 def test_calls_allocate_nothing(gpu_ctx):
     """Apart from torch's own tensors: a second call of every kind adds no allocation of the library's."""
     layer = Layer(gpu_ctx, 1, 400)
