@@ -192,7 +192,7 @@ class Kv4Cache:
     def _new(self, like: torch.Tensor, tokens: int, heads: int):
         """A new [tokens][heads][head_dim] tensor and its C rows."""
         d = self.head_dim
-        t = like.new_empty((tokens, heads, d))
+        t = torch.empty_like(like) if like.is_contiguous() else like.new_empty((tokens, heads, d))
         return t, C.byref(HeadRowsC(t.data_ptr(), heads * d, d))
 
     def _batch(self, batch: SeqBatch, tokens: int):
@@ -244,7 +244,7 @@ class Kv4Cache:
         c = self._batch(batch, num_tokens)
         heads = self.kv_heads
         if k_out is None and v_out is None:
-            both = torch.empty((2, num_tokens, heads, self.head_dim), dtype=_BF16, device=batch.kv_len.device)
+            both = batch.kv_len.new_empty((2, num_tokens, heads, self.head_dim), dtype=_BF16)
             k_out, v_out = both.unbind()
             at, d = both.data_ptr(), heads * self.head_dim
             rk = C.byref(HeadRowsC(at, d, self.head_dim))

@@ -59,9 +59,10 @@ def _rows_q8(x, weight, residual, eps, norm, one_plus, hidden, ctx) -> Q8Rows:
     if (ldr and residual.shape != x.shape) or (ldh and hidden.shape != x.shape):
         raise ValueError("residual and hidden must have x's shape")
     ld = -(-cols // 16) * 16
-    codes = x.new_empty((rows, ld), dtype=torch.int8)
-    if ld != cols:
-        codes = codes[:, :cols]
+    if ld == cols and x.is_contiguous():
+        codes = torch.empty_like(x, dtype=torch.int8)
+    else:
+        codes = x.new_empty((rows, ld), dtype=torch.int8)[:, :cols]
     scales = x.new_empty(rows, dtype=torch.float32)
     if rows:
         launch(ctx, "kl_norm_q8", ctx.h, x.data_ptr(),
@@ -82,7 +83,7 @@ def add_rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tenso
     update the residual stream in place; by default, with a residual, a new
     tensor.  A row that is not finite gets scale NaN."""
     if hidden is None and isinstance(residual, torch.Tensor):
-        hidden = torch.empty_like(residual, memory_format=torch.contiguous_format)
+        hidden = torch.empty_like(residual) if residual.is_contiguous() else residual.new_empty(residual.shape)
     return _rows_q8(x, weight, residual, eps, 1, one_plus_weight, hidden, ctx)
 
 
