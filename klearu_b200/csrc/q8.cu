@@ -444,14 +444,20 @@ __global__ void __launch_bounds__(128) q8_split_kernel(const __grid_constant__ C
     const int each = t.join;
     cluster_wait();  // all blocks have begun, their shared memory is there
     const uint32_t at = smem_u32(part + (rank * 128 + (int)threadIdx.x) * each);
+    int to = 0, off = 0;  // whose rows these are, and where in its share
 #pragma unroll 1
     for (int j = 0; j < rows; j += 16) {
       uint32_t v[16];
       tc5_ld16_async(mine + j, v);
       tc5_ld_wait();
 #pragma unroll
-      for (int u = 0; u < 16; u += 4)
-        if (j + u < rows) st_cluster4(at + 4 * (uint32_t)((j + u) % each), (uint32_t)((j + u) / each), v + u);
+      for (int u = 0; u < 16; u += 4) {
+        if (j + u < rows) st_cluster4(at + 4 * (uint32_t)off, (uint32_t)to, v + u);
+        if ((off += 4) == each) {
+          off = 0;
+          ++to;
+        }
+      }
     }
     __syncwarp();
     cluster_arrive();
