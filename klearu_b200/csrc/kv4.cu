@@ -370,15 +370,21 @@ __global__ void __launch_bounds__(AP_NT) kv4_read_kernel(ReadArgs a) {
     for (int u = 0; u < U; ++u) {
       if (u0 + u >= n || places[u0 + u].kind == 0) continue;
       const float sf = __uint_as_float(pr[u] << 16), mf = __uint_as_float(pr[u] & 0xffff0000u);
+      const uint32_t even = w[u] & 0x0f0f0f0fu, odd = (w[u] >> 4) & 0x0f0f0f0fu;
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((w[u] >> (4 * kv4_nibble(i))) & 15u), sf, mf);
+      for (int i = 0; i < 8; ++i) {  // a byte under 2^23's exponent is that number and a code
+        const int n = kv4_nibble(i);
+        const uint32_t c = __byte_perm(n & 1 ? odd : even, 0x4b000000u, 0x7540 | (n >> 1));
+        x[i] = fmaf(__uint_as_float(c) - 8388608.f, sf, mf);
+      }
       store8_bf16(static_cast<__nv_bfloat16*>(o.p) + (int64_t)(t0 + u0 + u) * o.token + head * o.head + 8 * l, o.vec, x);
     }
   }
 }
 
-// Reading: four tokens a block where one each would be more blocks than the machine holds at once.
+// Reading: four tokens a block where one each would be more blocks than the machine holds at once (8 key heads: 8000
+// tokens 10.3 us against 17.6, 600 3.3 both, 256 2.9 against 2.7).
 int block_tokens(int items, int per, int tokens) { return ceil_div(items, per) * tokens >= 8 * 148 ? RD_TOKENS : 1; }
 dim3 token_grid(int items, int per, int tokens, int each) {
   const int64_t n = ceil_div(tokens, each);
