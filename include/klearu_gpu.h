@@ -706,7 +706,7 @@ KL_API kl_status kl_rope_destroy(kl_rope_t rope);
 /* A paged cache of keys and values in 4 bits.  A head vector x is held as codes
  * c of 4 bits, a step s and a minimum m: x ~ s c + m with m = bf16(min x),
  * s = bf16((max x - min x) / 15), c = clamp(rint((x - m) / s), 0, 15) (0 where
- * s is 0); a vector with a value that is not finite reads back as NaN.
+ * s is 0), difference and quotient rounded to f32; a vector with a value that is not finite reads back as NaN.
  * page_size: tokens per page, a multiple of 16; head_dim: 64 or 128
  * (KL_EUNSUPPORTED otherwise).  head_dim + 8 bytes per token and head. */
 KL_API kl_status kl_kv4_create(kl_ctx_t ctx, int64_t num_pages, int page_size, int kv_heads, int head_dim,

@@ -2,7 +2,8 @@
 64-bit forms (attention_ref.py).
 
 Inputs are bf16, so without a rotation a code is decided exactly: x - m and the
-quotient's distance from a border need fewer bits than f32 has.  With one, a
+quotient's distance from a border need fewer bits than f32 has, unless a value
+2^16 times smaller than m stands where 0 would be on the border.  With one, a
 32-bit rotated value may fall on the other side of a border than the 64-bit one
 (off by 3 roundings of 2^-24 against steps of at least 2^-9 of the minimum and
 range): then a cached value is one step off, and a step or minimum one step of
