@@ -588,7 +588,8 @@ struct AttendPlan {
 
 // Which kernel.  Per key of a sequence and key head the split kernel takes 30 ps and 30 more for each tile of 16 rows;
 // the tensor-core kernel 2.4 us for 128 keys and 256 rows on each of 148 processors.  Where its blocks leave
-// processors idle it gets chunks of the keys, of 256 at least (one sequence of 2000, 64 new tokens: 25 us, 29 with 512).
+// processors idle it gets chunks of the keys, of 256 at least (one sequence of 2000, 64 new tokens: 25 us, 29 with 512;
+// of 60000, 1280 tokens, 160 blocks: 2234 us whole, 1398 in eight; of 2000: 73 whole, 102 in two).
 // Both sides, split and tensor core, 4 query heads on each of 8 key heads, us:
 //   new tokens                4          12         16         32         64         500
 //   1 sequence of 60000    37   80    74   81    96   82   186   86   351   93   2467  581
@@ -598,8 +599,20 @@ struct AttendPlan {
 AttendPlan attend_plan(const AttendShape& s) {
   const int64_t rows = (int64_t)s.max_q * (s.q_heads / s.kv_heads), heads = (int64_t)s.num_seqs * s.kv_heads;
   const int64_t span = plan_span(s, 256), steps = ceil_div(span, 128), blocks = heads * ceil_div(rows, 256);
-  const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(148 / blocks, steps / 2));
-  const double tc = 2.4 * (double)ceil_div(blocks * chunks, 148) * (double)ceil_div(steps, chunks);
+  // A turn of blocks takes 12 us beside its steps; chunks 5 us for the join and 2.5 ps for each of the D values that a
+  // row of a chunk writes and the join reads.  Several sequences are ragged, which evens out their turns: they are cut
+  // for one turn at most.
+  const int64_t rows_all = std::min<int64_t>(s.num_tokens, (int64_t)s.num_seqs * s.max_q) * s.q_heads;
+  int64_t chunks = 1;
+  double tc = 0.0, least = 1e30;
+  for (int64_t t = 0; t <= (s.num_seqs > 1 ? 1 : 16); ++t) {  // whole, or as many chunks as t turns hold
+    int64_t c = std::min<int64_t>(148 * t / blocks, steps / 2);
+    c = c > 1 ? ceil_div(steps, ceil_div(steps, c)) : 1;
+    const int64_t turns = ceil_div(blocks * c, 148);
+    const double work = 2.4 * (double)(turns * ceil_div(steps, c));
+    const double all = work + 12.0 * (double)turns + (c > 1 ? 5.0 + 2.5e-6 * (double)(rows_all * s.D * c) : 0.0);
+    if (all < least) chunks = c, tc = work, least = all;
+  }
   const double split = 30e-6 * (double)heads * (double)span * (double)(1 + ceil_div(rows, 16));
   AttendPlan p{tc < split, (int)chunks, {}};
   // hints may be far off: the workspace stays below half a gigabyte
