@@ -18,8 +18,12 @@
 // f16, not bf16, for its 11 bits: with keys, values and probabilities at 2^-12
 // the output is as exact as its own bf16 rounding.  Its range is made up for by
 // powers of two: of each row of Q, of each step's K (both into the score's
-// factor) and V (the step's probabilities are taken times 2^(ev - ev of the
-// first step), which the running reference follows and the row sum takes out).
+// factor) and V.  V is held times 2^-ev, a row's O in units of 2^(unit - 6) of
+// its own, and P is 2^(6 + ev - unit) times the probability (to the reference),
+// 2^15 at most and with full precision down to 2^-14: the unit follows ev where
+// it grows by more than 1 or falls by more than 7 (O is rescaled with it), so
+// that neither zeros nor larger values in front leave later probabilities among
+// f16's subnormals.  (Following every growth: 502 us in place of 498.)
 // Tensor memory: S_0, S_1 (128 columns each), O_0, O_1 (D columns each).
 // Where the rows make fewer blocks than the device has processors (a chunk of
 // one long prompt), each row's steps are shared out to several blocks, whose
@@ -150,8 +154,10 @@ struct TcSmem {
 // A step's powers of two and missing pages.
 struct TcStep {
   unsigned char hole[8];  // 16-token tiles whose page does not exist
-  float ek2, ev;          // K is held times 1 / ek2, V times 2^-ev
+  float ek2;              // K is held times 1 / ek2
+  float ev;               // V times 2^-ev; TC_NONE: nothing but zeros
 };
+constexpr float TC_NONE = -10000.f;
 struct TcShared {
   uint64_t q_full, k_full[2], v_full[2], done;
   uint64_t s_full[2], p_full[2], o_full[2];  // by tile, one phase a step: scores there; P there; O has taken P
@@ -283,14 +289,20 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
     const int jhi = (w.first + (w.r0 + i * 128) / group - w.lo + 1) / TC_KV;
     const int jlo = a.window > 0 ? (w.first + (min(w.r0 + i * 128 + 128, w.rows) - 1) / group - a.window - w.lo + TC_KV) / TC_KV - 1
                                  : -1;
-    float ref = 0.f, lift = -INFINITY, l = 0.f, ev0 = 0.f;
+    float ref = 0.f, lift = -INFINITY, l = 0.f;  // l: the sum of 2^(score - ref)
+    float unit = TC_NONE;
     for (int j = 0; j < w.steps; ++j) {
       if (!warp_wait(&sh.s_full[i], (kq + j) & 1u)) return false;
       tc5_fence_after();
       const TcStep& st = sh.step[(kq + j) & 3u];
       const uint2 holes = *reinterpret_cast<const uint2*>(st.hole);
-      if (j == 0) ev0 = st.ev;
-      const float ev = st.ev - ev0;
+      float off = st.ev - unit;  // P is 2^(6 + off) times the probability
+      float grow = 1.f;          // of O by a change of its unit
+      if (!(off <= 1.f && off >= -7.f)) {
+        if (unit != TC_NONE && lift != -INFINITY) grow = st.ev == TC_NONE ? 1.f : pow2(max(-126, (int)-off));  // else O is zero
+        if (st.ev != TC_NONE) unit = st.ev;
+        off = 0.f;
+      }
       const float f = fmaxf(worth * st.ek2, 1.2e-38f);  // never 0, which an unseen score's -inf would make NaN
       uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll 1
@@ -321,8 +333,8 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
 #pragma unroll
           for (int c = 0; c < 4; ++c) tops[c] = fmaxf(tops[c], fmaxf(s[u + c], s[u + c + 4]));
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        if (top != -INFINITY) top = fmaf(top, f, ev);
-        if (__any_sync(FULL, top > lift)) {
+        if (top != -INFINITY) top *= f;
+        if (__any_sync(FULL, top > lift || grow != 1.f)) {
           const bool first = lift == -INFINITY;
           const float now = top > lift - 8.f || first ? top : ref;
           float keep = 1.f;
@@ -355,12 +367,13 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
               tc5_ld16_async(tO + 16 * c, v);
               tc5_ld_wait();
 #pragma unroll
-              for (int u = 0; u < 16; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * keep);
+              for (int u = 0; u < 16; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * (keep * grow));
               tc5_st16(tO + 16 * c, v);
             }
           }
+          grow = 1.f;
         }
-        const uint64_t f2 = pair(f, f), less2 = pair(ev - ref, ev - ref);
+        const uint64_t f2 = pair(f, f), less2 = pair(6.f + off - ref, 6.f + off - ref);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
@@ -380,7 +393,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
       }
       float x, y;
       unpair(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), x, y);
-      l = ev == 0.f ? l + (x + y) : fmaf(x + y, exp2f(-ev), l);
+      l = fmaf(x + y, off == 0.f ? 0.015625f : exp2f(-6.f - off), l);
       tc5_st_wait();
       tc5_fence_before();
       __syncwarp();
@@ -395,7 +408,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
       kq += (uint32_t)w.steps;
       if (!warp_wait(&sh.o_full[i], (kq - 1) & 1u)) return false;
       tc5_fence_after();
-      const float inv = 1.f / l, up = exp2f(ev0);
+      const float inv = 0.015625f / l, up = unit == TC_NONE ? 0.f : pow2((int)unit);
       float* to = join_rows(a, chunks) + at * D;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -418,7 +431,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
       kq += (uint32_t)w.steps;
       if (!warp_wait(&sh.o_full[i], (kq - 1) & 1u)) return false;
       tc5_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l, up = exp2f(ev0);
+      const float inv = l == 0.f ? 0.f : 0.015625f / l, up = unit == TC_NONE ? 0.f : pow2((int)unit);
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t v[32];
@@ -461,9 +474,9 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
   const int lane = threadIdx.x & 31, tid = threadIdx.x - 256, sub = tid & 15;
   const int kvh = blockIdx.y;
   uint32_t kq = 0;
-  int ev_before = 0;
   bool alive = true;
   tc_each(a, chunks, sh, bad, [&](const TcWork& w) {
+    int ev_top = -126;
     const int32_t* table = a.seq.table + w.b * a.seq.table_ld;
     uint4 kc[D / 32], vc[D / 32], vp[2];
     uint2 kp;
@@ -536,11 +549,12 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
       const uint4 mv = *reinterpret_cast<const uint4*>(sh.reach[st][1]);
       const uint32_t tk = max(max(mk.x, mk.y), max(mk.z, mk.w)), tv = max(max(mv.x, mv.y), max(mv.z, mv.w));
       const int ek = tk ? max(-126, (int)(tk >> 23) - 127 - 13) : 0;
-      const int ev = tv ? max(-126, (int)(tv >> 23) - 127 - 13) : ev_before;  // nothing but zeros: as it was
-      ev_before = ev;
+      // values 2^60 smaller than those of a step before lose bits: O, which grows as its unit falls, stays finite
+      const int ev = max(max(-126, (int)(tv >> 23) - 127 - 13), ev_top - 60);
+      if (tv) ev_top = max(ev_top, ev);
       if (tid == 0) {
         sh.step[q & 3u].ek2 = pow2(ek);
-        sh.step[q & 3u].ev = (float)ev;
+        sh.step[q & 3u].ev = tv ? (float)ev : TC_NONE;
       }
       const float fk = pow2(-ek), fv = pow2(-ev);
       {  // ---- K: this thread's token, D contiguous ----
