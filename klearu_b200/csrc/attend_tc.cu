@@ -23,7 +23,11 @@
 // 2^15 at most and with full precision down to 2^-14: the unit follows ev where
 // it grows by more than 1 or falls by more than 7 (O is rescaled with it), so
 // that neither zeros nor larger values in front leave later probabilities among
-// f16's subnormals.  (Following every growth: 502 us in place of 498.)
+// f16's subnormals.  (Following every growth: 502 us in place of 498.)  A step
+// whose keys or values are more than 2^16 apart in size is "wide": there every
+// token has powers of two of its own, and each row takes its scores and its unit
+// from the tokens that it sees, so that those that it does not see cost it no
+// bits; tokens that no row of the block sees are zeros.
 // Tensor memory: S_0, S_1 (128 columns each), O_0, O_1 (D columns each).
 // Where the rows make fewer blocks than the device has processors (a chunk of
 // one long prompt), each row's steps are shared out to several blocks, whose
@@ -154,18 +158,24 @@ struct TcSmem {
 // A step's powers of two and missing pages.
 struct TcStep {
   unsigned char hole[8];  // 16-token tiles whose page does not exist
-  float ek2;              // K is held times 1 / ek2
+  float ek2;              // K is held times 1 / ek2; negative: a wide step
   float ev;               // V times 2^-ev; TC_NONE: nothing but zeros
 };
+// Of a token of a wide step: K is held times 2^-ek, V times 2^-ev.
+struct TcPowers {
+  signed char ek, ev;  // ev -128: its value is zero
+};
+constexpr int TC_SPREAD = 16;  // of a step that is not wide, as a power of two
 constexpr float TC_NONE = -10000.f;
 struct TcShared {
   uint64_t q_full, k_full[2], v_full[2], done;
   uint64_t s_full[2], p_full[2], o_full[2];  // by tile, one phase a step: scores there; P there; O has taken P
   uint32_t tmem;
   int fail;
-  alignas(16) uint32_t reach[2][2][4];  // by step & 1: largest |K|, |V| of each decoding warp
+  alignas(16) uint32_t reach[2][4][4];  // by step & 1: largest |K|, |V|, smallest of each but 0, of each decoding warp
   // by step & 3: a step's is written again when the step two on has its scores, after this one's softmax
   alignas(16) TcStep step[4];
+  alignas(16) TcPowers powers[4][TC_KV];  // of a wide step
 };
 static_assert(offsetof(TcShared, reach) % 16 == 0 && offsetof(TcShared, step) % 16 == 0 && sizeof(TcStep) == 16,
               "read as 16- and 8-byte vectors");
@@ -191,6 +201,7 @@ struct TcWork {
   SeqSpan s;
   int b, rows, r0, first;  // row r is token first + r / group
   int lo, steps;           // keys [lo, lo + 128 steps) cover what the rows see (there); lo a multiple of 16
+  int from;                // no row sees a key in front of it
   int hi;                  // no row sees hi or later (the chunk ends there)
 };
 
@@ -210,7 +221,8 @@ __device__ __forceinline__ void tc_each(const AttendArgs& a, int chunks, TcShare
       w.r0 = rt * TC_ROWS;
       const int pos0 = w.first + w.r0 / group;
       w.hi = w.first + (min(w.r0 + TC_ROWS, w.rows) - 1) / group + 1;
-      w.lo = (a.window > 0 ? max(0, pos0 - a.window + 1) : 0) & ~15;
+      w.from = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+      w.lo = w.from & ~15;
       w.steps = w.hi > w.lo ? (w.hi - w.lo + TC_KV - 1) / TC_KV : 0;
       if (chunks > 1) {  // the rows' own steps in equal shares
         const int each = (w.steps + chunks - 1) / chunks, from = min(w.steps, chunk * each);
@@ -224,6 +236,89 @@ __device__ __forceinline__ void tc_each(const AttendArgs& a, int chunks, TcShare
       }
     }
   }
+}
+
+// What a row's softmax has so far.
+struct TcRow {
+  float ref, lift, l;  // l: the sum of 2^(score - ref); a score above lift moves ref
+  float unit, peak;    // of O; the largest so far: O stays finite while the unit is above peak - 64
+};
+// A wide step's probabilities, for a row that sees its keys [from, to].  Not inlined: beside the ordinary step's its code
+// costs that one 16 us of 507 (7416 prompt tokens).
+template <int D>
+__device__ __noinline__ TcRow tc_wide_step(TcRow row, const TcStep& st, const TcPowers* powers, float worth, int from, int to,
+                                           uint32_t tS, uint32_t tO, bool rescale) {
+  auto score = [&](float s, int u, TcPowers x) {
+    const float f = fminf(fmaxf(worth * pow2(x.ek), 1.2e-38f), 3.4e38f);
+    return u <= to && u >= from && !st.hole[u >> 4] ? s * f : -INFINITY;
+  };
+  float top = -INFINITY, most = -INFINITY;  // the largest score, and with its value's exponent
+#pragma unroll 1
+  for (int c = 0; c < TC_KV; c += 16) {
+    uint32_t s[16];
+    tc5_ld16_async(tS + c, s);
+    tc5_ld_wait();
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const TcPowers x = powers[c + u];
+      const float t = score(__uint_as_float(s[u]), c + u, x);
+      top = fmaxf(top, t);
+      if (x.ev != -128) most = fmaxf(most, t + (float)x.ev);
+    }
+  }
+  float by = 1.f;  // of O
+  const bool first = row.lift == -INFINITY;
+  if (top != -INFINITY && (first || top > row.ref)) {
+    if (!first) by = exp2_fast(row.ref - top);
+    row.ref = top;
+    row.lift = top + 8.f;
+    row.l *= by;
+  }
+  if (most != -INFINITY) {  // the unit by what counts most
+    float need = ceilf(fminf(fmaxf(most - row.ref, -126.f), 126.f));
+    if (row.unit == TC_NONE || first) {
+      row.unit = need;
+    } else {
+      need = fmaxf(need, row.peak - 64.f);
+      if (need > row.unit + 1.f || need < row.unit - 7.f) {
+        by *= pow2(max(-126, (int)(row.unit - need)));
+        row.unit = need;
+      }
+    }
+    row.peak = fmaxf(row.peak, row.unit);
+  }
+  if (rescale && __any_sync(FULL, by != 1.f)) {
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+      uint32_t v[16];
+      tc5_ld16_async(tO + c, v);
+      tc5_ld_wait();
+#pragma unroll
+      for (int u = 0; u < 16; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * by);
+      tc5_st16(tO + c, v);
+    }
+  }
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < TC_KV; c += 32) {  // P's columns [c / 2, c / 2 + 16) have been read
+    uint32_t s[32], pk[16];
+    tc5_ld16_async(tS + c, s);
+    tc5_ld16_async(tS + c + 16, s + 16);
+    tc5_ld_wait();
+#pragma unroll
+    for (int u = 0; u < 32; ++u) {
+      const TcPowers x = powers[c + u];
+      const float t = score(__uint_as_float(s[u]), c + u, x) - row.ref;
+      sum += exp2_fast(t);
+      s[u] = __float_as_uint(exp2_fast(t + (x.ev == -128 ? 0.f : 6.f + (float)x.ev - row.unit)));
+    }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) pk[u] = pack_f16(__uint_as_float(s[2 * u]), __uint_as_float(s[2 * u + 1]));
+    tc5_st16(tS + c / 2, pk);
+  }
+  row.l += sum;
+  tc5_st_wait();
+  return row;
 }
 
 // ---- warps 0-7: one row per thread ----
@@ -289,18 +384,26 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
     const int jhi = (w.first + (w.r0 + i * 128) / group - w.lo + 1) / TC_KV;
     const int jlo = a.window > 0 ? (w.first + (min(w.r0 + i * 128 + 128, w.rows) - 1) / group - a.window - w.lo + TC_KV) / TC_KV - 1
                                  : -1;
-    float ref = 0.f, lift = -INFINITY, l = 0.f;  // l: the sum of 2^(score - ref)
-    float unit = TC_NONE;
+    float ref = 0.f, lift = -INFINITY, l = 0.f, unit = TC_NONE, peak = -126.f;  // a TcRow
     for (int j = 0; j < w.steps; ++j) {
       if (!warp_wait(&sh.s_full[i], (kq + j) & 1u)) return false;
       tc5_fence_after();
       const TcStep& st = sh.step[(kq + j) & 3u];
       const uint2 holes = *reinterpret_cast<const uint2*>(st.hole);
+      if (st.ek2 < 0.f) {
+        const int to = seen - TC_KV * j, from = a.window > 0 ? max(0, to - a.window + 1) : 0;
+        const TcRow row = tc_wide_step<D>({ref, lift, l, unit, peak}, st, sh.powers[(kq + j) & 3u], worth, from, to, tS, tO, j > 0);
+        ref = row.ref, lift = row.lift, l = row.l, unit = row.unit, peak = row.peak;
+        tc5_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[i]);
+        continue;
+      }
       float off = st.ev - unit;  // P is 2^(6 + off) times the probability
       float grow = 1.f;          // of O by a change of its unit
       if (!(off <= 1.f && off >= -7.f)) {
         if (unit != TC_NONE && lift != -INFINITY) grow = st.ev == TC_NONE ? 1.f : pow2(max(-126, (int)-off));  // else O is zero
-        if (st.ev != TC_NONE) unit = st.ev;
+        if (st.ev != TC_NONE) unit = st.ev, peak = fmaxf(peak, unit);
         off = 0.f;
       }
       const float f = fmaxf(worth * st.ek2, 1.2e-38f);  // never 0, which an unseen score's -inf would make NaN
@@ -361,13 +464,14 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
             }
           }
           if (j > 0) {  // O: these scores were not begun before it had taken the step before
+            const float by = keep * grow;
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t v[16];
               tc5_ld16_async(tO + 16 * c, v);
               tc5_ld_wait();
 #pragma unroll
-              for (int u = 0; u < 16; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * (keep * grow));
+              for (int u = 0; u < 16; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) * by);
               tc5_st16(tO + 16 * c, v);
             }
           }
@@ -494,14 +598,16 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
                  ? nullptr
                  : kv4_tile(a.cache, TB, page, kvh, n - kv4_column(a.cache, n) * a.cache.tiles_per_page);
     };
-    auto fetch_k = [&](const unsigned char* tile) {
+    // tokens that no row sees are zeros, whatever is left in their places
+    auto live = [&](int n) { return n >= w.from && n < w.hi; };
+    auto fetch_k = [&](const unsigned char* tile, int j) {
       kp = make_uint2(0, 0);
       if (!tile) {
 #pragma unroll
         for (int u = 0; u < D / 32; ++u) kc[u] = make_uint4(0, 0, 0, 0);
         return;
       }
-      kp = *reinterpret_cast<const uint2*>(tile + 2 * CODES + sub * 8);
+      if (live(w.lo + j * TC_KV + tid)) kp = *reinterpret_cast<const uint2*>(tile + 2 * CODES + sub * 8);
 #pragma unroll
       for (int u = 0; u < D / 32; ++u) {
         if (D == 128) {
@@ -513,7 +619,7 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
         }
       }
     };
-    auto fetch_v = [&](const unsigned char* tile) {
+    auto fetch_v = [&](const unsigned char* tile, int j) {
       if (!tile) {
 #pragma unroll
         for (int u = 0; u < D / 32; ++u) vc[u] = make_uint4(0, 0, 0, 0);
@@ -525,18 +631,34 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         vp[h] = *reinterpret_cast<const uint4*>(tile + 2 * CODES + (8 * h + 2 * (sub & 3)) * 8);
+      const int n = w.lo + j * TC_KV;
+      if (!live(n) || !live(n + TC_KV - 1)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int m = n + (tid & ~15) + 8 * h + 2 * (sub & 3);
+          if (!live(m)) vp[h].x = vp[h].y = 0;
+          if (!live(m + 1)) vp[h].z = vp[h].w = 0;
+        }
+      }
     };
     int32_t page = page_of(0), next = page_of(1);
     const unsigned char* tile = tile_of(0, page);
-    fetch_k(tile);
-    fetch_v(tile);
+    fetch_k(tile, 0);
+    fetch_v(tile, 0);
     for (int j = 0; j < w.steps; ++j) {
       const uint32_t q = kq + j, st = q & 1u;
       // ---- the step's powers of two: the largest |K| and |V| to [2^13, 2^14) ----
-      const uint32_t rk = __reduce_max_sync(FULL, reach(kp.x)), rv = __reduce_max_sync(FULL, reach(kp.y));
+      // a vector that is not finite: the key becomes NaN for whoever sees it, the value zero, since a
+      // product with it reaches rows that do not
+      const bool nan = bf_high(kp.x) != bf_high(kp.x) || bf_high(kp.y) != bf_high(kp.y);
+      const uint32_t my_k = nan ? 0u : reach(kp.x), my_v = nan ? 0u : reach(kp.y);
+      const uint32_t rk = __reduce_max_sync(FULL, my_k), rv = __reduce_max_sync(FULL, my_v);
+      const uint32_t nk = __reduce_min_sync(FULL, my_k ? my_k : ~0u), nv = __reduce_min_sync(FULL, my_v ? my_v : ~0u);
       if (lane == 0) {
         sh.reach[st][0][tid >> 5] = rk;
         sh.reach[st][1][tid >> 5] = rv;
+        sh.reach[st][2][tid >> 5] = nk;
+        sh.reach[st][3][tid >> 5] = nv;
       }
       // tile 1's scores of the step before are there: K's and V's stages of two steps before are free (its O had
       // taken P before them), and so is the step's slot.  The four warps give up as one.
@@ -547,20 +669,22 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
       if (!all_of_128(alive)) return false;
       const uint4 mk = *reinterpret_cast<const uint4*>(sh.reach[st][0]);
       const uint4 mv = *reinterpret_cast<const uint4*>(sh.reach[st][1]);
+      const uint4 sk = *reinterpret_cast<const uint4*>(sh.reach[st][2]);
+      const uint4 sv = *reinterpret_cast<const uint4*>(sh.reach[st][3]);
       const uint32_t tk = max(max(mk.x, mk.y), max(mk.z, mk.w)), tv = max(max(mv.x, mv.y), max(mv.z, mv.w));
-      const int ek = tk ? max(-126, (int)(tk >> 23) - 127 - 13) : 0;
-      // values 2^60 smaller than those of a step before lose bits: O, which grows as its unit falls, stays finite
-      const int ev = max(max(-126, (int)(tv >> 23) - 127 - 13), ev_top - 60);
-      if (tv) ev_top = max(ev_top, ev);
+      const uint32_t bk = min(min(sk.x, sk.y), min(sk.z, sk.w)), bv = min(min(sv.x, sv.y), min(sv.z, sv.w));
+      auto power = [](uint32_t r) { return max(-126, (int)(r >> 23) - 127 - 13); };  // -126 for 0
+      const int ek = power(tk), ev = power(tv);
+      // also where values fall so far below those before that the rows' units could not follow
+      const bool wide = (tk >> 23) > (bk >> 23) + TC_SPREAD || (tv >> 23) > (bv >> 23) + TC_SPREAD || (tv && ev < ev_top - 60);
+      ev_top = max(ev_top, ev);
+      if (wide) sh.powers[q & 3u][tid] = TcPowers{(signed char)power(my_k), (signed char)(my_v ? power(my_v) : -128)};
       if (tid == 0) {
-        sh.step[q & 3u].ek2 = pow2(ek);
+        sh.step[q & 3u].ek2 = wide ? -1.f : pow2(ek);
         sh.step[q & 3u].ev = tv ? (float)ev : TC_NONE;
       }
-      const float fk = pow2(-ek), fv = pow2(-ev);
+      const float fk = pow2(wide ? -power(my_k) : -ek), fv = pow2(-ev);
       {  // ---- K: this thread's token, D contiguous ----
-        // a vector that is not finite: the key becomes NaN for whoever sees it, the value zero, since a
-        // product with it reaches rows that do not
-        const bool nan = bf_high(kp.x) != bf_high(kp.x) || bf_high(kp.y) != bf_high(kp.y);
         const uint32_t s2 = nan ? 0u : twice_f16(bf_low(kp.x) * fk);
         const uint32_t m2 = nan ? 0x7fff7fffu : twice_f16(bf_high(kp.x) * fk);
         unsigned char* to = sK + st * KVB + tid * 128;
@@ -577,7 +701,7 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
       // the next step's loads go out as soon as their registers are free
       page = next;
       tile = tile_of(j + 1, page);
-      fetch_k(tile);
+      fetch_k(tile, j + 1);
       next = page_of(j + 2);
       // ---- V: 16-byte chunks of the codes; two tokens each ----
       uint32_t s2[2][2], m2[2][2];  // of tokens 2t + o of half h
@@ -587,8 +711,9 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
         for (int o = 0; o < 2; ++o) {
           const uint32_t k = o ? vp[h].z : vp[h].x, v = o ? vp[h].w : vp[h].y;
           const bool nan = bf_high(k) != bf_high(k) || bf_high(v) != bf_high(v);
-          s2[h][o] = nan ? 0u : twice_f16(bf_low(v) * fv);
-          m2[h][o] = nan ? 0u : twice_f16(bf_high(v) * fv);
+          const float fo = wide ? pow2(-power(reach(v))) : fv;
+          s2[h][o] = nan ? 0u : twice_f16(bf_low(v) * fo);
+          m2[h][o] = nan ? 0u : twice_f16(bf_high(v) * fo);
         }
 #pragma unroll
       for (int u = 0; u < D / 32; ++u) {
@@ -608,7 +733,7 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.v_full[st]);
-      fetch_v(tile);
+      fetch_v(tile, j + 1);
     }
     kq += (uint32_t)w.steps;
     return true;

@@ -127,7 +127,7 @@ def test_zero_values_first_whole_rows(gpu_ctx):
 
 @pytest.mark.parametrize("kernel", ["many", "whole"])
 @pytest.mark.parametrize("big,size", [(1e6, 1.0), (1e6, 1e-3), (1e10, 1.0), (1e2, 1e-4)])
-@pytest.mark.parametrize("keys", [128, 256])
+@pytest.mark.parametrize("keys", [1, 16, 128, 300])
 def test_large_values_that_hardly_count(gpu_ctx, kernel, big, size, keys):
     """The first keys' scores are 60 and more below the others', and their values far larger."""
     n, rows = 900, 70
@@ -178,3 +178,63 @@ def test_a_long_flat_tail(gpu_ctx, kernel):
         total = top + others
         assert ((out[r, :, 1] / (15 * others / total) - 1).abs() <= B.BF16 + tail + 1e-3).all(), r
         assert ((out[r, :, 2] / (15 * top / total) - 1).abs() <= B.BF16 + B.F16 + 1e-3).all(), r
+
+
+# ---------------------------------------------------------------------------
+# tokens that a row does not see
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("garbage", [1e6, 1e10, 1e30])
+def test_stale_tokens_behind_the_sequence(gpu_ctx, kernel, garbage):
+    """Another use of the page left large finite keys and values behind the sequence's end."""
+    dim, page, rows = 128, 128, 70
+    table = torch.full((1, 512 if kernel == "many" else 2), -7, dtype=torch.int32, device=DEV)
+    table[0, 0], table[0, 1] = 1, 0
+    for n in (90, 129, 250):
+        k, v = randn(256, 2, dim, seed=1), randn(256, 2, dim, seed=2)
+        k[n:] = (k[n:].float() * garbage).bfloat16()
+        v[n:] = (v[n:].float() * garbage).bfloat16()
+        cache = Kv4Cache(2, page, 2, dim, ctx=gpu_ctx)
+        cache.append(k, v, SeqBatch(i32([0, 256]), i32([256]), table, max_q=256))
+        now = SeqBatch(i32([0, rows]), i32([n]), table, max_q={"few": 1, "many": 200, "whole": 2**30}[kernel], max_kv=65536)
+        q = randn(rows, 8, dim, seed=3)
+        B.check(attend(kernel, cache, q, now), q, R.held(k[:n]), R.held(v[:n]), [rows], [n], rms=False)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("large", [1e5, 1e8, 1e30])
+@pytest.mark.parametrize("window", [0, 150])
+def test_large_tokens_that_some_rows_do_not_see(gpu_ctx, kernel, large, window):
+    """Later tokens for the rows before them, and tokens in front of a window: large values there change nothing."""
+    n, rows = 500, 140
+    q, k, v = inputs([rows], [n], 4, 2, 64)
+    at = [3, 230, 419, n - 20, n - 1]
+    for j in at:
+        v[j] = (v[j].float() * large).bfloat16()
+    out = run(gpu_ctx, kernel, q, k, v, [rows], [n], window=window, rms=False)
+    if not window:
+        return
+    # rows 20 to 55 (tokens 380 to 415) see tokens from 231 on and none of the large ones: small errors of their own
+    want, _ = B.attend(q[20:56], R.held(k)[:416], R.held(v)[:416], 380, window, 64**-0.5)
+    off = out[20:56].double() - want
+    assert float(off.square().mean().sqrt()) <= B.RMS * float(want.square().mean().sqrt())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("large", [1e5, 1e8, 1e20])
+def test_large_keys_that_some_rows_do_not_see(gpu_ctx, kernel, large):
+    n, rows = 500, 140
+    q, k, v = inputs([rows], [n], 4, 2, 64)
+    for j in (3, 430, n - 1):
+        k[j] = (k[j].float() * large).bfloat16()
+    # tokens 380 to 429: none of the large keys but the first, which a window of 300 leaves out
+    run_rows, first = 50, 380
+    batch, pages = batch_for(kernel, [rows], [n], 16)
+    cache = Kv4Cache(pages, 16, 2, 64, ctx=gpu_ctx)
+    cache.append(k, v, SeqBatch(i32([0, n]), batch.kv_len, batch.page_table, max_q=n))
+    out = attend(kernel, cache, q, batch, window=300)
+    i = first - (n - rows)
+    want, tol = B.attend(q[i : i + run_rows], R.held(k)[:430], R.held(v)[:430], first, 300, 64**-0.5)
+    off = (out[i : i + run_rows].double() - want).abs()
+    assert float((off / tol).max()) <= 1.0
+    assert float(off.square().mean().sqrt()) <= B.RMS * float(want.square().mean().sqrt())
