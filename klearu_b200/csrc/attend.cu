@@ -71,8 +71,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // word of 8 codes costs five logic instructions.  q is scaled by a power of two
 // into f16's range, which loses what is below 2^-37 of the row's largest;
 // probabilities go in times their value's step and a power of two 2^-E that
-// keeps the largest so far within f16, rounded to 11 bits (2^-12), and what is
-// 2^-25 below the largest to none.  Sums, maxima and O are f32.
+// keeps the largest so far within f16, rounded to 11 bits (2^-11 at most), and
+// what is 2^-25 below the largest to none.  References are whole numbers: where
+// one rises, E falls as much and O stays as it is, so that large values whose
+// keys have been outdone leave the range to what counts.  Sums, maxima and O are
+// f32.
 //
 // D + 8 bytes a token and key head.  64 sequences of up to 16384 tokens, D = 128,
 // 8 key heads of 4 rows: 147 us, 4.0 TB/s of 6.4; one of 131071: 43 us, 3.3 TB/s.
@@ -320,16 +323,22 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) top[r][u] = fmaxf(top[r][u], __shfl_xor_sync(FULL, top[r][u], d));
               const bool none = lift[r][u] == -INFINITY;
+              top[r][u] = ceilf(top[r][u]);
               if ((top[r][u] > ref[r][u] || none) && top[r][u] != -INFINITY) {
                 // sums taken with no finite score so far are NaN or zero: both stay what they are
-                const float keep = none ? 1.f : exp2f(ref[r][u] - top[r][u]);
+                const float rise = none ? 0.f : fminf(top[r][u] - ref[r][u], 253.f), keep = exp2f(-rise);
                 l[r][u] *= keep;
                 vb[r][u] *= keep;
+                const int room = 253 - (int)(__float_as_uint(down[r][u]) >> 23);  // to 2^126
+                if ((int)rise > room) {  // O with what is left of it
+                  const float less = exp2f((float)room - rise);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                  o[m][r][u] *= keep;
-                  o[m][r][2 + u] *= keep;
+                  for (int m = 0; m < MT; ++m) {
+                    o[m][r][u] *= less;
+                    o[m][r][2 + u] *= less;
+                  }
                 }
+                down[r][u] = __uint_as_float(__float_as_uint(down[r][u]) + ((uint32_t)min((int)rise, room) << 23));
                 ref[r][u] = top[r][u];
                 lift[r][u] = top[r][u] + 8.f;
               }

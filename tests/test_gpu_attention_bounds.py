@@ -125,7 +125,7 @@ def test_zero_values_first_whole_rows(gpu_ctx):
         run(gpu_ctx, "many", q, k, v, q_len, kv_len, rms=False)
 
 
-@pytest.mark.parametrize("kernel", ["many", "whole"])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("big,size", [(1e6, 1.0), (1e6, 1e-3), (1e10, 1.0), (1e2, 1e-4)])
 @pytest.mark.parametrize("keys", [1, 16, 128, 300])
 def test_large_values_that_hardly_count(gpu_ctx, kernel, big, size, keys):
