@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
     for (int r0 = (blockIdx.x % p.row_tiles) * 8 * NR; r0 < rows; r0 += p.row_tiles * 8 * NR) {
       // tokens that some row of this tile sees: [lo, hi), this block's share [k0, k1)
       const int pos0 = first + r0 / group, hi = first + (min(r0 + 8 * NR, rows) - 1) / group + 1;
-      const int lo = (a.window > 0 ? max(0, pos0 - a.window + 1) : 0) & ~15;
+      const int lo = window_from(a.window, pos0) & ~15;
       const int span = max(0, hi - lo);
       const int chunk = max(p.chunk, (int)round_up(ceil_div(span, p.chunks), 16 * AT_W));
       const int k0 = min(hi, lo + chunk_id * chunk), k1 = max(k0, min(hi, k0 + chunk));
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
         }
       }
       const int see_all_to = pos0;  // every row of the tile sees tokens up to here ..
-      const int see_all_from = a.window > 0 ? hi - a.window : 0;  // .. from here
+      const int see_all_from = window_from(a.window, hi - 1);  // .. from here
 
       float o[MT][NR][4], l[NR][2], vb[NR][2], ref[NR][2], lift[NR][2];
 #pragma unroll
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
 #pragma unroll
               for (int u = 0; u < 4; ++u) {
                 const int j = j0 + c * 16 * AT_W + g + 8 * (u >> 1), q = pos[r][u & 1];
-                if (!ok[c] || j > q || (a.window > 0 && j <= q - a.window)) x[c][r][u] = -INFINITY;
+                if (!ok[c] || j > q || (a.window > 0 && q - j >= a.window)) x[c][r][u] = -INFINITY;
               }
         }
         float top[NR][2];

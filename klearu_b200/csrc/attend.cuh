@@ -15,6 +15,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// The first token that token pos sees (0 where pos is a row in front of its sequence); a window may be as large as a
+// number gets, a position as small, so the difference is not taken where it would be negative.
+__device__ __forceinline__ int window_from(int window, int pos) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
+
 // The workspace: (reference, sum) of [chunk][token][query head], then their rows of D.
 __device__ __forceinline__ float* join_rows(const AttendArgs& a, int chunks) {
   const int64_t n = (int64_t)chunks * a.seq.num_tokens * a.q_heads * 2;

@@ -238,3 +238,13 @@ def test_large_keys_that_some_rows_do_not_see(gpu_ctx, kernel, large):
     off = (out[i : i + run_rows].double() - want).abs()
     assert float((off / tol).max()) <= 1.0
     assert float(off.square().mean().sqrt()) <= B.RMS * float(want.square().mean().sqrt())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("window", [2**40, 2**31 - 1, 2**31 - 2, 10**6])
+@pytest.mark.parametrize("q_len,kv_len", [([9], [4]), ([300], [30]), ([70, 9], [3, 900])])
+def test_padding_and_a_window_that_reaches_all(gpu_ctx, kernel, window, q_len, kv_len):
+    """Rows in front of the first token beside rows that see keys, and a window as large as a number gets."""
+    q, k, v = inputs(q_len, kv_len, 4, 2, 64)
+    out = run(gpu_ctx, kernel, q, k, v, q_len, kv_len, window=window, rms=False)
+    assert torch.equal(out, run(gpu_ctx, kernel, q, k, v, q_len, kv_len, rms=False))
