@@ -106,10 +106,10 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
     bool bad = false;
     const SeqSpan s = seq_span(a.seq, b, ps, &bad);
     if (bad && threadIdx.x == 0) atomicOr(a.err, DERR_BOUNDS);
-    const int rows = s.q_len * group, first = s.kv_len - s.q_len;  // row r is token first + r / group
+    const int rows = s.q_len * group, first = s.first;  // row r is token first + r / group
     for (int r0 = (blockIdx.x % p.row_tiles) * 8 * NR; r0 < rows; r0 += p.row_tiles * 8 * NR) {
       // tokens that some row of this tile sees: [lo, hi), this block's share [k0, k1)
-      const int pos0 = first + r0 / group, hi = first + (min(r0 + 8 * NR, rows) - 1) / group + 1;
+      const int pos0 = first + r0 / group, pos1 = first + (min(r0 + 8 * NR, rows) - 1) / group, hi = min(pos1 + 1, s.kv_len);
       const int lo = window_from(a.window, pos0) & ~15;
       const int span = max(0, hi - lo);
       const int chunk = max(p.chunk, (int)round_up(ceil_div(span, p.chunks), 16 * AT_W));
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
         }
       }
       const int see_all_to = pos0;  // every row of the tile sees tokens up to here ..
-      const int see_all_from = window_from(a.window, hi - 1);  // .. from here
+      const int see_all_from = window_from(a.window, pos1);  // .. from here
 
       float o[MT][NR][4], l[NR][2], vb[NR][2], ref[NR][2], lift[NR][2];
 #pragma unroll

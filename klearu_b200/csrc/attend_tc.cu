@@ -215,12 +215,12 @@ __device__ __forceinline__ void tc_each(const AttendArgs& a, int chunks, TcShare
   for (w.b = blockIdx.z; w.b < a.seq.num_seqs; w.b += gridDim.z) {
     w.s = seq_span(a.seq, w.b, a.cache.page_size, bad);
     w.rows = w.s.q_len * group;
-    w.first = w.s.kv_len - w.s.q_len;
+    w.first = w.s.first;
     const int tiles = (w.rows + TC_ROWS - 1) / TC_ROWS;
     for (int rt = height - 1 - ((int)blockIdx.x - chunk * height); rt < tiles; rt += height) {
       w.r0 = rt * TC_ROWS;
       const int pos0 = w.first + w.r0 / group;
-      w.hi = w.first + (min(w.r0 + TC_ROWS, w.rows) - 1) / group + 1;
+      w.hi = min(w.first + (min(w.r0 + TC_ROWS, w.rows) - 1) / group + 1, w.s.kv_len);
       w.from = window_from(a.window, pos0);
       w.lo = w.from & ~15;
       w.steps = w.hi > w.lo ? (w.hi - w.lo + TC_KV - 1) / TC_KV : 0;
@@ -379,9 +379,9 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
     }
-    const int seen = w.first + row / group - w.lo;  // the row sees keys up to its own, counted from w.lo
+    const int own = w.first + row / group - w.lo, seen = min(own, w.s.kv_len - 1 - w.lo);  // counted from w.lo, as what follows
     // every row of the tile sees all of the steps in (jlo, jhi)
-    const int jhi = (w.first + (w.r0 + i * 128) / group - w.lo + 1) / TC_KV;
+    const int jhi = (min(w.first + (w.r0 + i * 128) / group, w.s.kv_len - 1) - w.lo + 1) / TC_KV;
     const int last = w.first + (min(w.r0 + i * 128 + 128, w.rows) - 1) / group - w.lo;
     const int jlo = a.window > 0 && last >= a.window ? (last - a.window + TC_KV) / TC_KV - 1 : -1;
     float ref = 0.f, lift = -INFINITY, l = 0.f, unit = TC_NONE, peak = -126.f;  // a TcRow
@@ -391,7 +391,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
       const TcStep& st = sh.step[(kq + j) & 3u];
       const uint2 holes = *reinterpret_cast<const uint2*>(st.hole);
       if (st.ek2 < 0.f) {
-        const int to = seen - TC_KV * j, from = window_from(a.window, to);
+        const int to = seen - TC_KV * j, from = window_from(a.window, own - TC_KV * j);
         const TcRow row = tc_wide_step<D>({ref, lift, l, unit, peak}, st, sh.powers[(kq + j) & 3u], worth, from, to, tS, tO, j > 0);
         ref = row.ref, lift = row.lift, l = row.l, unit = row.unit, peak = row.peak;
         tc5_fence_before();
@@ -416,7 +416,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
         tc5_ld_wait();
         const uint32_t hole4 = h ? holes.y : holes.x;
         if (j >= jhi || j <= jlo) {
-          const int to = seen - TC_KV * j - 64 * h, from = window_from(a.window, to);  // columns seen
+          const int at0 = TC_KV * j + 64 * h, to = seen - at0, from = window_from(a.window, own - at0);  // columns seen
           const unsigned span = to >= from ? (unsigned)(to - from) : 0u, at = to >= from ? (unsigned)from : 0x40000000u;
 #pragma unroll
           for (int u = 0; u < 64; ++u)

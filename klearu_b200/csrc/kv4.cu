@@ -111,13 +111,15 @@ __device__ __forceinline__ Place find_place(const Kv4View& cache, const SeqView&
   if (b >= seq.num_seqs) return r;
   const SeqSpan s = seq_span(seq, b, cache.page_size, bad);
   if (t < s.row) return r;  // in front of the first sequence
-  const int index = s.kv_len - s.q_len + (t - s.row);
+  const int index = s.first + (t - s.row);
   r.pos = positions ? positions[t] : index;
   r.kind = 1;
   if (index < 0) return r;  // in front of its sequence's first token: padding
-  const int col = kv4_column(cache, index >> 4);
-  r.off = index - col * cache.page_size;
-  r.page = seq.table[b * seq.table_ld + col];
+  if (index < s.kv_len) {
+    const int col = kv4_column(cache, index >> 4);
+    r.off = index - col * cache.page_size;
+    r.page = seq.table[b * seq.table_ld + col];
+  }
   if (r.page < 0 || r.page >= cache.num_pages) {
     *bad = true;
     r.page = -1;

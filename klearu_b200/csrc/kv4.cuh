@@ -123,16 +123,18 @@ __device__ __forceinline__ int find_seq(const int32_t* cu, int n, int t) {
   return lo;
 }
 
-// A sequence's rows and length, held to what the call's arrays have room for;
-// *bad where they had to be.
+// A sequence's rows and tokens, held to what the call's arrays have room for;
+// *bad where they had to be.  Row `row` is token `first`, whatever was cut off;
+// tokens from kv_len on have no place.
 struct SeqSpan {
-  int row, q_len, kv_len;
+  int row, q_len, first, kv_len;
 };
 __device__ __forceinline__ SeqSpan seq_span(const SeqView& s, int b, int page_size, bool* bad) {
   SeqSpan r;
   const int a = s.cu_q[b], e = s.cu_q[b + 1], n = s.kv_len[b];
   r.row = max(0, min(a, s.num_tokens));
   r.q_len = max(0, min(e, s.num_tokens) - r.row);
+  r.first = (int)((uint32_t)max(0, n) - ((uint32_t)e - (uint32_t)r.row));  // a number where there are rows: 0 <= row < e
   r.kv_len = (int)max((int64_t)0, min((int64_t)n, (int64_t)s.width * page_size));
   *bad = r.row != a || r.q_len != e - a || r.kv_len != n;
   return r;

@@ -1,0 +1,110 @@
+"""What the calls of the attention half do at the edges of their arguments: lengths beyond the table, streams other than
+the context's, tiny rows, tangents."""
+
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import attention_bound as B
+import attention_ref as R
+from klearu_b200._lib import KL_EBOUNDS, KlError
+from klearu_b200.attention import Kv4Cache, RopeTable, SeqBatch
+from klearu_b200.core import Context
+from klearu_b200.dejavu import FfnStack, SparseMlp, SparsityPredictor
+from klearu_b200.quant import Q8Linear, add_rms_norm_q8, quantize_rows_q8
+from test_gpu_attention import DEV, i32, randn
+from test_gpu_q8 import check_norm
+
+pytestmark = pytest.mark.gpu
+
+
+def reported(ctx):
+    with pytest.raises(KlError) as e:
+        ctx.sync()
+    return e.value.status == KL_EBOUNDS
+
+
+# ---------------------------------------------------------------------------
+# lengths and rows beyond what the call's arrays hold
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("q_len", [1, 5, 60])
+def test_tokens_beyond_the_table(q_len):
+    """A sequence longer than its row of the table: its tokens keep their numbers, those that have a page are written and
+    attended to, the others are not, and nothing of the tokens before them changes.  60: the kernel for many rows."""
+    ctx = Context(0)
+    page, heads, kv_heads, dim, held = 1024, 32, 8, 64, 8192
+    n = held + 10  # ten tokens more than the table has room for
+    table = i32([[5, 2, 7, 0, 1, 6, 3, 4]])
+    cache = Kv4Cache(8, page, kv_heads, dim, ctx=ctx)
+    k, v = randn(n, kv_heads, dim, seed=1), randn(n, kv_heads, dim, seed=2)
+    old = SeqBatch(i32([0, held]), i32([held]), table, max_q=held)
+    cache.append(k[:held], v[:held], old)
+    ctx.sync()
+    first = n - q_len
+    new = SeqBatch(i32([0, q_len]), i32([n]), table, max_q=q_len)
+    k2, v2, q = randn(q_len, kv_heads, dim, seed=3), randn(q_len, kv_heads, dim, seed=4), randn(q_len, heads, dim, seed=5)
+    rope = RopeTable(dim, 16384, ctx=ctx)
+    turned = cache.append(k2, v2, new, q=q, rope=rope)
+    assert reported(ctx)
+    pos = torch.arange(first, n, device=DEV)
+    want = R.rotate(q, pos, rope.inv_freq, False)
+    assert ((turned.double() - want).abs() <= R.HALF * want.abs() + 1e-5).all()
+    fit = max(0, held - first)  # of the new tokens
+    hk, hv = R.held(k[:held]), R.held(v[:held])
+    gk, gv = cache.read(old, held)
+    assert torch.equal(gk[: held - fit], hk[: held - fit].float().bfloat16())
+    assert torch.equal(gv[: held - fit], hv[: held - fit].float().bfloat16())
+    assert torch.equal(gv[held - fit :], R.held(v2[:fit]).float().bfloat16())
+    rk, rv = cache.read(new, q_len)
+    assert reported(ctx)
+    assert torch.equal(rv[:fit], gv[held - fit :]) and torch.equal(rk[:fit], gk[held - fit :])
+    assert (rk[fit:] == 0).all() and (rv[fit:] == 0).all()
+    # every row sees the tokens up to its own that there are; with a window the last of its own numbers
+    for window in (0, 25, 8):
+        out = cache.attend(q, new, window=window)
+        assert reported(ctx)
+        for r in range(q_len):
+            p = first + r
+            low, high = max(0, p - window + 1) if window else 0, min(p + 1, held)
+            if low >= high:
+                assert (out[r] == 0).all()
+                continue
+            want, _ = B.attend(q[r : r + 1], gk[low:high].double(), gv[low:high].double(), high - low - 1, 0, dim**-0.5)
+            # read() rounds the held keys and values to bf16: 2^-7 / sqrt(12) of each, and a score's error from its keys
+            # (scale sqrt(sum q^2 K^2) of that, about 2.5) moves the output as much again
+            size = float(want.square().mean().sqrt())
+            assert float((out[r].double() - want[0]).square().mean().sqrt()) <= 0.01 * size + 1e-4, (window, r)
+
+
+@pytest.mark.parametrize("rows", [5, 60])
+def test_rows_beyond_the_tensor(rows):
+    """A batch with more rows than the call's tensors: the rows that there are keep their tokens' numbers."""
+    ctx = Context(0)
+    page, heads, kv_heads, dim, n, lost = 1024, 32, 8, 64, 8000, 7
+    table = i32([list(range(8))])
+    cache = Kv4Cache(8, page, kv_heads, dim, ctx=ctx)
+    k, v = randn(n, kv_heads, dim, seed=1), randn(n, kv_heads, dim, seed=2)
+    cache.append(k, v, SeqBatch(i32([0, n]), i32([n]), table, max_q=n))
+    ctx.sync()
+    first = n - rows - lost  # the call says rows + 7 new tokens and has only so many rows
+    batch = SeqBatch(i32([0, rows + lost]), i32([n]), table, max_q=rows + lost)
+    k2, v2, q = randn(rows, kv_heads, dim, seed=3), randn(rows, kv_heads, dim, seed=4), randn(rows, heads, dim, seed=5)
+    cache.append(k2, v2, batch)
+    assert reported(ctx)
+    k[first : first + rows], v[first : first + rows] = k2, v2
+    every = SeqBatch(i32([0, n]), i32([n]), table, max_q=n)
+    gk, gv = cache.read(every, n)
+    assert torch.equal(gk, R.held(k).float().bfloat16()) and torch.equal(gv, R.held(v).float().bfloat16())
+    out = cache.attend(q, batch)
+    assert reported(ctx)
+    want, tol = B.attend(q, R.held(k), R.held(v), first, 0, dim**-0.5)
+    assert ((out.double() - want).abs() <= tol).all()
+
+
+def ffn(ctx, h=192, layers=1):
+    rng = np.random.default_rng(3)
+    w = lambda *s: (rng.standard_normal(s) * 0.05).astype(np.float32)  # noqa: E731
+    pred = [SparsityPredictor(w(40, h), w(40), w(256, 40), w(256), ctx=ctx) for _ in range(layers)]
+    mlp = [SparseMlp(w(256, h), w(256, h), w(h, 256), ctx=ctx) for _ in range(layers)]
+    return FfnStack(pred, mlp, np.ones((layers, h), np.float32), ctx=ctx)
