@@ -36,14 +36,19 @@ __device__ __forceinline__ void norm_weights8(const NormQ8Args& a, int c, float*
 // rint(127 u / top) for u = h * w in 64 bits.  The f32 quotient decides unless
 // it is within 1e-4 of a border between two codes (its own error is below
 // 3 roundings of 127, 2.3e-5): only then are the 64-bit product and quotient
-// taken, so the codes are those of the definition.
+// taken, so the codes are those of the definition.  Where the row's largest is so
+// small that 127 / top is no f32 (below 3.7e-37), every code is taken so.
 __device__ __noinline__ int q8_exact(float h, float w, double top) {
   return (int)rint((double)h * (double)w * 127.0 / top);
+}
+// A row's scale; mx, the largest product in f32, has lost bits where it is among the smallest numbers.
+__device__ __forceinline__ float q8_scale(float mx, float rinv, double top) {
+  return mx < 1e-30f ? (float)(top * (double)rinv / 127.0) : mx * rinv / 127.f;
 }
 __device__ __forceinline__ int q8_code(float h, float w, float p, float inv, double top) {
   const float t = p * inv;
   const float r = rintf(t);
-  if (fabsf(fabsf(t - r) - 0.5f) < 1e-4f) return q8_exact(h, w, top);
+  if (!(fabsf(fabsf(t - r) - 0.5f) >= 1e-4f)) return q8_exact(h, w, top);  // NaN where inv is infinite
   return (int)r;
 }
 
@@ -157,7 +162,7 @@ __global__ void __launch_bounds__(1024) norm_q8_vec_kernel(NormQ8Args a) {
   const bool good = finite32(mx) && finite32(ss);
   if (threadIdx.x == 0) {
     const float rinv = a.norm ? 1.f / sqrtf(ss / (float)a.cols + a.eps) : 1.f;
-    a.scales[row] = good ? mx * rinv / 127.f : __int_as_float(0x7fffffff);
+    a.scales[row] = good ? q8_scale(mx, rinv, top) : __int_as_float(0x7fffffff);
   }
   const float inv = good && mx > 0.f ? 127.f / mx : 0.f;
   int8_t* co = a.codes + row * a.ldc;
@@ -175,10 +180,10 @@ __global__ void __launch_bounds__(1024) norm_q8_vec_kernel(NormQ8Args a) {
         off = fmaxf(off, fabsf(t - (y - 12582912.f)));
         b[i] = __float_as_uint(y);
       }
-      if (off > 0.4999f) {  // a border between two codes is near
+      if (off > 0.4999f || inv == INFINITY) {  // a border between two codes is near
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (fabsf(p[v][i] * inv - (__uint_as_float(b[i]) - 12582912.f)) > 0.4999f)
+          if (!(fabsf(p[v][i] * inv - (__uint_as_float(b[i]) - 12582912.f)) <= 0.4999f))
             b[i] = (uint32_t)q8_exact(h[v][i], norm_weight(a, c + i), top);
       }
 #pragma unroll
@@ -229,7 +234,7 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
   const double top = __longlong_as_double((long long)top_s);
   const float rinv = a.norm ? 1.f / sqrtf(ss / (float)a.cols + a.eps) : 1.f;
   const bool good = finite32(mx) && finite32(ss);
-  if (threadIdx.x == 0) a.scales[row] = good ? mx * rinv / 127.f : __int_as_float(0x7fffffff);
+  if (threadIdx.x == 0) a.scales[row] = good ? q8_scale(mx, rinv, top) : __int_as_float(0x7fffffff);
   const float inv = good && mx > 0.f ? 127.f / mx : 0.f;
   int8_t* co = a.codes + row * a.ldc;
   for (int i = threadIdx.x; i < a.cols; i += NT) {

@@ -108,3 +108,27 @@ def ffn(ctx, h=192, layers=1):
     pred = [SparsityPredictor(w(40, h), w(40), w(256, 40), w(256), ctx=ctx) for _ in range(layers)]
     mlp = [SparseMlp(w(256, h), w(256, h), w(h, 256), ctx=ctx) for _ in range(layers)]
     return FfnStack(pred, mlp, np.ones((layers, h), np.float32), ctx=ctx)
+
+
+# ---------------------------------------------------------------------------
+# rows of extreme sizes
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("cols", [256, 77])
+@pytest.mark.parametrize("size", [3e-37, 1e-37, 1e-38, 1e-40, 3e-44])
+def test_codes_of_tiny_rows(gpu_ctx, cols, size):
+    """Rows so small that 127 over their largest value is no 32-bit number."""
+    x = (randn(5, cols, seed=1, dtype=torch.float32).double() * size).float()
+    x[1] = 0
+    x[2, 3] = size * 40
+    x[3, ::2] = 0
+    ones = torch.ones(cols, device=DEV)
+    r = quantize_rows_q8(x, ctx=gpu_ctx)
+    u = x.double()
+    top = u.abs().amax(-1, keepdim=True)
+    assert torch.equal(r.codes.double(), torch.where(top > 0, (u * 127 / top).round(), 0.0))
+    # a scale below the normal numbers has steps of 2^-149
+    assert ((r.scales.double() - top[:, 0] / 127).abs() <= 2.0**-149 + 4 * 2.0**-24 * top[:, 0] / 127).all()
+    r = add_rms_norm_q8(x, ones, eps=1e-5, ctx=gpu_ctx)
+    assert torch.equal(r.codes.double(), torch.where(top > 0, (u * 127 / top).round(), 0.0))
+    want = top[:, 0] / (u.square().mean(-1) + 1e-5).sqrt() / 127
+    assert ((r.scales.double() - want).abs() <= 2.0**-149 + 8 * 2.0**-24 * want).all()
