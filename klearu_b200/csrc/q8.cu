@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(1024) norm_q8_vec_kernel(NormQ8Args a) {
   }
   __syncthreads();
   const double top = __longlong_as_double((long long)top_s);
-  const bool good = finite32(mx) && finite32(ss);
+  const bool good = finite32(mx) && (!a.norm || finite32(ss));
   if (threadIdx.x == 0) {
     const float rinv = a.norm ? 1.f / sqrtf(ss / (float)a.cols + a.eps) : 1.f;
     a.scales[row] = good ? q8_scale(mx, rinv, top) : __int_as_float(0x7fffffff);
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
   __syncthreads();
   const double top = __longlong_as_double((long long)top_s);
   const float rinv = a.norm ? 1.f / sqrtf(ss / (float)a.cols + a.eps) : 1.f;
-  const bool good = finite32(mx) && finite32(ss);
+  const bool good = finite32(mx) && (!a.norm || finite32(ss));
   if (threadIdx.x == 0) a.scales[row] = good ? q8_scale(mx, rinv, top) : __int_as_float(0x7fffffff);
   const float inv = good && mx > 0.f ? 127.f / mx : 0.f;
   int8_t* co = a.codes + row * a.ldc;

@@ -132,3 +132,13 @@ def test_codes_of_tiny_rows(gpu_ctx, cols, size):
     assert torch.equal(r.codes.double(), torch.where(top > 0, (u * 127 / top).round(), 0.0))
     want = top[:, 0] / (u.square().mean(-1) + 1e-5).sqrt() / 127
     assert ((r.scales.double() - want).abs() <= 2.0**-149 + 8 * 2.0**-24 * want).all()
+
+
+@pytest.mark.parametrize("cols", [256, 77])
+def test_codes_of_large_rows(gpu_ctx, cols):
+    """Without a norm the sum of squares is nobody's business: rows whose squares pass 32 bits have codes."""
+    x = randn(4, cols, seed=1, dtype=torch.float32) * 1e25
+    x[1] *= 1e12
+    check_norm(quantize_rows_q8(x, ctx=gpu_ctx), x, torch.ones(cols, device=DEV), 0, False)
+    r = add_rms_norm_q8(x, torch.ones(cols, device=DEV), ctx=gpu_ctx)
+    assert torch.isnan(r.scales).all() and (r.codes == 0).all()
