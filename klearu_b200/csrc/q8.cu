@@ -41,9 +41,15 @@ __device__ __forceinline__ void norm_weights8(const NormQ8Args& a, int c, float*
 __device__ __noinline__ int q8_exact(float h, float w, double top) {
   return (int)rint((double)h * (double)w * 127.0 / top);
 }
-// A row's scale; mx, the largest product in f32, has lost bits where it is among the smallest numbers.
-__device__ __forceinline__ float q8_scale(float mx, float rinv, double top) {
-  return mx < 1e-30f ? (float)(top * (double)rinv / 127.0) : mx * rinv / 127.f;
+// Where eps is too small to matter beside them: squares of values below 2^-40, many of which are no normal numbers, are
+// summed once more times 2^200.
+__host__ __device__ __forceinline__ bool q8_small_eps(const NormQ8Args& a) { return a.norm && a.eps < 0x1p-75f; }
+__device__ __forceinline__ bool q8_small(const NormQ8Args& a, float ss) { return q8_small_eps(a) && ss < 0x1p-80f; }
+// A row's scale.  mx, the largest product in f32, has lost bits where it is among the smallest numbers; top has not.
+__device__ __forceinline__ float q8_scale(const NormQ8Args& a, float mx, double top, float ss, bool small) {
+  if (small) return (float)(top * (0x1p100 / 127.0) * (double)(1.f / sqrtf(ss / (float)a.cols + a.eps * 0x1p100f * 0x1p100f)));
+  const float rinv = a.norm ? 1.f / sqrtf(ss / (float)a.cols + a.eps) : 1.f;
+  return mx < 1e-30f ? (float)(top * (1.0 / 127.0) * (double)rinv) : mx * rinv / 127.f;
 }
 __device__ __forceinline__ int q8_code(float h, float w, float p, float inv, double top) {
   const float t = p * inv;
@@ -72,7 +78,9 @@ __device__ __forceinline__ float block_reduce(float v, float* tmp, bool is_max) 
 // more a load; one pass over memory.  8191 rows of 4096 bf16 columns and their
 // residual: 79 us, 4.7 TB/s; bound by each block's chain of load, two barriers
 // and store.  Resident blocks that fetch their next row meanwhile took 91.
-template <int NV, class T>
+// SMALL: eps may be too small for the squares of small rows; keeping h for that
+// costs registers (201 us with the values formed after it, 199 without).
+template <int NV, class T, bool SMALL>
 __global__ void __launch_bounds__(1024) norm_q8_vec_kernel(NormQ8Args a) {
   __shared__ float2 tmp[32];
   __shared__ unsigned long long top_s;
@@ -160,10 +168,10 @@ __global__ void __launch_bounds__(1024) norm_q8_vec_kernel(NormQ8Args a) {
   __syncthreads();
   const double top = __longlong_as_double((long long)top_s);
   const bool good = finite32(mx) && (!a.norm || finite32(ss));
-  if (threadIdx.x == 0) {
-    const float rinv = a.norm ? 1.f / sqrtf(ss / (float)a.cols + a.eps) : 1.f;
-    a.scales[row] = good ? q8_scale(mx, rinv, top) : __int_as_float(0x7fffffff);
-  }
+  auto put_scale = [&](bool small) {
+    if (threadIdx.x == 0) a.scales[row] = good ? q8_scale(a, mx, top, ss, small) : __int_as_float(0x7fffffff);
+  };
+  if (!SMALL) put_scale(false);
   const float inv = good && mx > 0.f ? 127.f / mx : 0.f;
   int8_t* co = a.codes + row * a.ldc;
 #pragma unroll
@@ -192,6 +200,23 @@ __global__ void __launch_bounds__(1024) norm_q8_vec_kernel(NormQ8Args a) {
     }
     *reinterpret_cast<uint2*>(co + c) = make_uint2(out[0], out[1]);
   }
+  if (!SMALL) return;
+  const bool small = q8_small(a, ss);
+  if (small) {
+    ss = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(h[v][i] * 0x1p100f, h[v][i] * 0x1p100f, ss);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
+    if ((threadIdx.x & 31) == 0) tmp[threadIdx.x >> 5].x = ss;
+    __syncthreads();
+    ss = (int)(threadIdx.x & 31) < warps ? tmp[threadIdx.x & 31].x : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
+  }
+  put_scale(small);
 }
 
 // The same for any alignment and width: the row's h waits in shared memory
@@ -232,9 +257,13 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
   }
   __syncthreads();
   const double top = __longlong_as_double((long long)top_s);
-  const float rinv = a.norm ? 1.f / sqrtf(ss / (float)a.cols + a.eps) : 1.f;
-  const bool good = finite32(mx) && (!a.norm || finite32(ss));
-  if (threadIdx.x == 0) a.scales[row] = good ? q8_scale(mx, rinv, top) : __int_as_float(0x7fffffff);
+  const bool good = finite32(mx) && (!a.norm || finite32(ss)), small = q8_small(a, ss);
+  if (small) {
+    ss = 0.f;
+    for (int i = threadIdx.x; i < a.cols; i += NT) ss = fmaf(nq_h[i] * 0x1p100f, nq_h[i] * 0x1p100f, ss);
+    ss = block_reduce<NT>(ss, tmp, false);
+  }
+  if (threadIdx.x == 0) a.scales[row] = good ? q8_scale(a, mx, top, ss, small) : __int_as_float(0x7fffffff);
   const float inv = good && mx > 0.f ? 127.f / mx : 0.f;
   int8_t* co = a.codes + row * a.ldc;
   for (int i = threadIdx.x; i < a.cols; i += NT) {
@@ -688,8 +717,12 @@ void launch_norm_q8(const NormQ8Args& a, int rows, cudaStream_t st) {
     // The plain kernel takes 14.5, 21.2 and 247: rows that are not aligned, and more than 16384 columns.
     const bool two = a.cols > 8192 || rows > 296;
     const int threads = (int)round_up(ceil_div(a.cols, two ? 16 : 8), 32);
-    auto* kernel = a.x_bf16 ? two ? norm_q8_vec_kernel<2, __nv_bfloat16> : norm_q8_vec_kernel<1, __nv_bfloat16>
-                            : two ? norm_q8_vec_kernel<2, float> : norm_q8_vec_kernel<1, float>;
+    auto pick = [&](auto small) {
+      constexpr bool S = decltype(small)::value;
+      return a.x_bf16 ? two ? norm_q8_vec_kernel<2, __nv_bfloat16, S> : norm_q8_vec_kernel<1, __nv_bfloat16, S>
+                      : two ? norm_q8_vec_kernel<2, float, S> : norm_q8_vec_kernel<1, float, S>;
+    };
+    auto* kernel = q8_small_eps(a) ? pick(std::true_type{}) : pick(std::false_type{});
     launch_next(kernel, dim3(rows), threads, 0, st, a);
     count_launch();
     return;

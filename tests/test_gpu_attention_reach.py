@@ -135,6 +135,15 @@ def test_codes_of_tiny_rows(gpu_ctx, cols, size):
 
 
 @pytest.mark.parametrize("cols", [256, 77])
+@pytest.mark.parametrize("size", [1e-15, 1e-19, 1e-22, 1e-25, 1e-33])
+def test_norm_of_small_rows_without_eps(gpu_ctx, cols, size):
+    """The squares of these rows are below the normal 32-bit numbers, their root mean square is not."""
+    x = (randn(5, cols, seed=1, dtype=torch.float32).double() * size).float()
+    w = 1 + 0.2 * randn(cols, seed=3, dtype=torch.float32)
+    check_norm(add_rms_norm_q8(x, w, eps=0.0, ctx=gpu_ctx), x, w, 0.0, True)
+
+
+@pytest.mark.parametrize("cols", [256, 77])
 def test_codes_of_large_rows(gpu_ctx, cols):
     """Without a norm the sum of squares is nobody's business: rows whose squares pass 32 bits have codes."""
     x = randn(4, cols, seed=1, dtype=torch.float32) * 1e25
