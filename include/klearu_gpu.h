@@ -701,6 +701,9 @@ typedef struct kl_q8_linear_s* kl_q8_linear_t;
  * interleaved, else (i, i + rot_dim / 2); dims from rot_dim on are not turned. */
 KL_API kl_status kl_rope_create(kl_ctx_t ctx, int rot_dim, int64_t max_positions, const double* inv_freq_host,
                                 float attention_factor, int interleaved, kl_rope_t* out);
+/* The same with a factor of 64 bits. */
+KL_API kl_status kl_rope_create_f64(kl_ctx_t ctx, int rot_dim, int64_t max_positions, const double* inv_freq_host,
+                                    double attention_factor, int interleaved, kl_rope_t* out);
 KL_API kl_status kl_rope_destroy(kl_rope_t rope);
 
 /* A paged cache of keys and values in 4 bits.  A head vector x is held as codes

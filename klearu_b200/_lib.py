@@ -174,6 +174,7 @@ _PROTOS = {
     "kl_ffn_stack_destroy": (_S, [_H]),
     "kl_ffn_stack_decode": (_S, [_H, _P, C.c_int, C.c_float]),
     "kl_rope_create": (_S, [_H, C.c_int, C.c_int64, _P, C.c_float, C.c_int, C.POINTER(_H)]),
+    "kl_rope_create_f64": (_S, [_H, C.c_int, C.c_int64, _P, C.c_double, C.c_int, C.POINTER(_H)]),
     "kl_rope_destroy": (_S, [_H]),
     "kl_kv4_create": (_S, [_H, C.c_int64, C.c_int, C.c_int, C.c_int, C.POINTER(_H)]),
     "kl_kv4_destroy": (_S, [_H]),

@@ -92,7 +92,7 @@ class RopeTable:
         self.rot_dim, self.max_positions, self.interleaved = rot_dim, max_positions, interleaved
         self.inv_freq = np.ascontiguousarray(f)
         h = C.c_void_p()
-        launch(self.ctx, "kl_rope_create", self.ctx.h, rot_dim, max_positions, self.inv_freq.ctypes.data,
+        launch(self.ctx, "kl_rope_create_f64", self.ctx.h, rot_dim, max_positions, self.inv_freq.ctypes.data,
                attention_factor, int(interleaved), C.byref(h))
         self.h = h
 

@@ -3740,13 +3740,14 @@ AttendShape attend_shape(kl_kv4_t c, const kl_seq_batch* s, int q_heads, int win
 }
 }  // namespace
 
-extern "C" kl_status kl_rope_create(kl_ctx_t ctx, int rot_dim, int64_t max_positions, const double* inv_freq_host,
-                                    float attention_factor, int interleaved, kl_rope_t* out) {
+extern "C" kl_status kl_rope_create_f64(kl_ctx_t ctx, int rot_dim, int64_t max_positions, const double* inv_freq_host,
+                                        double attention_factor, int interleaved, kl_rope_t* out) {
   if (!ctx || !out) return KL_EINVAL;
   KL_API_BEGIN(ctx)
   require(rot_dim >= 2 && rot_dim % 2 == 0, "rope: rot_dim must be even and >= 2");
   require(max_positions >= 1 && max_positions <= INT32_MAX, "rope: max_positions must be in [1, 2^31)");
   require(inv_freq_host != nullptr, "rope: inv_freq is required");
+  require(std::isfinite(attention_factor), "rope: attention_factor must be finite");
   auto r = std::make_unique<kl_rope_s>();
   r->ctx = ctx;
   r->device = ctx->device;
@@ -3762,6 +3763,10 @@ extern "C" kl_status kl_rope_create(kl_ctx_t ctx, int rot_dim, int64_t max_posit
   ck(cudaStreamSynchronize(ctx->stream), "sync");
   *out = r.release();
   KL_API_END
+}
+extern "C" kl_status kl_rope_create(kl_ctx_t ctx, int rot_dim, int64_t max_positions, const double* inv_freq_host,
+                                    float attention_factor, int interleaved, kl_rope_t* out) {
+  return kl_rope_create_f64(ctx, rot_dim, max_positions, inv_freq_host, attention_factor, interleaved, out);
 }
 extern "C" kl_status kl_rope_destroy(kl_rope_t r) { return destroy_handle(r); }
 

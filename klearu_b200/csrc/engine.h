@@ -403,7 +403,7 @@ struct SeqView;
 struct HeadRows;
 struct AttendArgs;
 struct AttendShape;
-void launch_rope_table(const double* inv_freq, int pairs, int64_t n, float factor, float2* table, cudaStream_t st);
+void launch_rope_table(const double* inv_freq, int pairs, int64_t n, double factor, float2* table, cudaStream_t st);
 void launch_kv4_append(const Kv4View& cache, int D, const SeqView& seq, const int32_t* positions, const float2* table,
                        int rot, int interleaved, int64_t max_pos, int q_heads, const HeadRows& q, const HeadRows& k,
                        const HeadRows& v, const HeadRows& q_out, int* err, cudaStream_t st);

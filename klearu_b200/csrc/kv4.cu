@@ -14,7 +14,7 @@ namespace {
 
 // table[p][i] = (cos, sin)(p * inv_freq[i]) * factor, angles and functions in
 // 64 bits (a far position's angle has no fraction bits left in 32), held in 32.
-__global__ void rope_table_kernel(const double* inv_freq, int pairs, int64_t n, float factor, float2* table) {
+__global__ void rope_table_kernel(const double* inv_freq, int pairs, int64_t n, double factor, float2* table) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= n * pairs) return;
   double s, c;
@@ -403,7 +403,7 @@ void launch_append(const AppendArgs& a, dim3 grid, cudaStream_t st) {
 
 }  // namespace
 
-void launch_rope_table(const double* inv_freq, int pairs, int64_t n, float factor, float2* table, cudaStream_t st) {
+void launch_rope_table(const double* inv_freq, int pairs, int64_t n, double factor, float2* table, cudaStream_t st) {
   rope_table_kernel<<<(unsigned)ceil_div(n * pairs, 256), 256, 0, st>>>(inv_freq, pairs, n, factor, table);
   count_launch();
 }

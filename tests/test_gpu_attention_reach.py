@@ -151,3 +151,23 @@ def test_codes_of_large_rows(gpu_ctx, cols):
     check_norm(quantize_rows_q8(x, ctx=gpu_ctx), x, torch.ones(cols, device=DEV), 0, False)
     r = add_rms_norm_q8(x, torch.ones(cols, device=DEV), ctx=gpu_ctx)
     assert torch.isnan(r.scales).all() and (r.codes == 0).all()
+
+
+# ---------------------------------------------------------------------------
+# the table of angles, tangents
+# ---------------------------------------------------------------------------
+def test_attention_factor_has_64_bits(gpu_ctx):
+    """A factor that is no 32-bit number: cosines times it are rounded once, and a turned query of ones shows them."""
+    factor, rot, t = 1 + 2.0**-24 * 0.99, 64, 65536
+    rope = RopeTable(rot, t, attention_factor=factor, ctx=gpu_ctx)
+    cache = Kv4Cache(t // 1024, 1024, 1, 64, ctx=gpu_ctx)
+    batch = SeqBatch(i32([0, t]), i32([t]), torch.arange(t // 1024, dtype=torch.int32, device=DEV).view(1, -1), max_q=t)
+    kv = torch.zeros(t, 1, 64, dtype=torch.bfloat16, device=DEV)
+    # a pair (1, 0) turns into the table's (cos, sin), shown in bf16; of four million numbers about forty lie so close to
+    # a border of bf16 that a factor rounded to 32 bits (here to 1) puts them on the other side
+    q = torch.zeros(t, 1, 64, dtype=torch.bfloat16, device=DEV)
+    q[..., : rot // 2] = 1.0
+    got = cache.append(kv, kv, batch, q=q, rope=rope)[:, 0]
+    z = torch.arange(t, dtype=torch.float64)[:, None] * torch.as_tensor(rope.inv_freq)
+    want = torch.cat([(z.cos() * factor).float(), (z.sin() * factor).float()], 1).bfloat16()
+    assert torch.equal(got.cpu(), want)
