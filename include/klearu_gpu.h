@@ -116,8 +116,11 @@ typedef struct kl_batch_iter_s* kl_batch_iter_t;
  * reference is single-process CPU code with no device state. */
 KL_API kl_status kl_ctx_create(int device, void* stream, kl_ctx_t* out);
 KL_API kl_status kl_ctx_destroy(kl_ctx_t ctx);
+/* Later calls run on another stream. */
 KL_API kl_status kl_ctx_set_stream(kl_ctx_t ctx, void* stream);
-/* Wait for all work issued on the context's stream; reports device errors. */
+/* Wait for all work issued on the context's stream (once the context has had
+ * more than one: for all work on its device, graphs that captured its calls
+ * among it); reports device errors. */
 KL_API kl_status kl_ctx_sync(kl_ctx_t ctx);
 /* Synchronise and report (then clear) the device-side error word. */
 KL_API kl_status kl_ctx_check(kl_ctx_t ctx);

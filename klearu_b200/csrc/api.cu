@@ -176,7 +176,8 @@ int bits_for(uint64_t n) {  // bits needed for values < n
 struct kl_ctx_s {
   int device = 0;
   cudaStream_t stream = nullptr;
-  DBuf err;  // int device error word
+  bool strayed = false;  // calls may have run, or graphs that captured them may run, on streams other than this one
+  DBuf err;              // int device error word
   std::string last_error;
 };
 
@@ -535,7 +536,8 @@ kl_status finish(kl_ctx_t ctx, const KlError& e) {
 namespace {
 // Read and clear the device error word (synchronises).
 void check_device_errors(kl_ctx_t ctx) {
-  ck(cudaStreamSynchronize(ctx->stream), "stream synchronize");
+  if (ctx->strayed) ck(cudaDeviceSynchronize(), "device synchronize");
+  else ck(cudaStreamSynchronize(ctx->stream), "stream synchronize");
   int e = 0;
   ck(cudaMemcpy(&e, ctx->err.p, 4, cudaMemcpyDeviceToHost), "read error word");
   if (e) {
@@ -590,6 +592,7 @@ extern "C" kl_status kl_ctx_destroy(kl_ctx_t ctx) {
 }
 extern "C" kl_status kl_ctx_set_stream(kl_ctx_t ctx, void* stream) {
   if (!ctx) return KL_EINVAL;
+  ctx->strayed = ctx->strayed || ctx->stream != static_cast<cudaStream_t>(stream);
   ctx->stream = static_cast<cudaStream_t>(stream);
   return KL_OK;
 }

@@ -102,6 +102,32 @@ def test_rows_beyond_the_tensor(rows):
     assert ((out.double() - want).abs() <= tol).all()
 
 
+# ---------------------------------------------------------------------------
+# streams
+# ---------------------------------------------------------------------------
+def test_errors_of_another_stream_are_reported():
+    """A call that runs on a stream which is not the context's: the next sync waits for it and reports what it saw."""
+    ctx = Context(0)
+    cache = Kv4Cache(3, 16, 2, 64, ctx=ctx)
+    bad = SeqBatch(i32([0, 40]), i32([40]), i32([[0, 3, 2]]), max_q=40)
+    cache.read(SeqBatch(i32([0, 40]), i32([40]), i32([[0, 1, 2]]), max_q=40), 40)
+    ctx.sync()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # about 50 ms of a busy stream in front
+        cache.read(bad, 40)
+    assert reported(ctx)
+    ctx.sync()  # and once only
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.read(bad, 40)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        graph.replay()
+    assert reported(ctx)
+
+
 def ffn(ctx, h=192, layers=1):
     rng = np.random.default_rng(3)
     w = lambda *s: (rng.standard_normal(s) * 0.05).astype(np.float32)  # noqa: E731
