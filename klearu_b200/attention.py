@@ -7,7 +7,9 @@ reference keeps f32 keys and values, crates/klearu-llm/src/model/kv_cache.rs).
 ``quant`` has the 8-bit projections around them.
 
 Every call launches on torch's current stream, like a torch operator, and can
-be captured in a CUDA graph; tensors have to be on the context's device.
+be captured in a CUDA graph; tensors have to be on the context's device.  As for
+all handles of the library, one host thread at a time calls a context and what
+was made with it.
 Nothing here has a backward pass: an input that requires a gradient is refused
 while gradients are recorded.
 """

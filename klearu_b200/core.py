@@ -42,7 +42,9 @@ class Context:
         if not torch.cuda.is_available():
             raise RuntimeError("klearu_b200 needs a CUDA device (there is no CPU fallback)")
         self.device = device
-        self.launch_lock = threading.Lock()  # held by calls that follow torch's current stream
+        # Keeps calls that follow torch's current stream from one another's while the context is switched to it.  All
+        # other calls of the context read its stream without the lock: one host thread at a time, as for every handle.
+        self.launch_lock = threading.Lock()
         self.stream = stream if stream is not None else torch.cuda.current_stream(device)
         h = C.c_void_p()
         check(self.lib.kl_ctx_create(device, C.c_void_p(self.stream.cuda_stream), C.byref(h)), None, "kl_ctx_create")

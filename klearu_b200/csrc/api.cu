@@ -3627,6 +3627,13 @@ extern "C" kl_status kl_ffn_stack_decode(kl_ffn_stack_t s, float* hidden, int n_
   support(k >= 1, "ffn stack decode: a sparsity that keeps no neuron is not supported");
   topk_check(s->pred[0], k);
   cudaStream_t st = ctx__->stream;
+  // a graph would keep scratch buffers that a larger call replaces
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) {
+    cudaGetLastError();  // the legacy stream while another one is captured
+    capture = cudaStreamCaptureStatusActive;
+  }
+  support(capture == cudaStreamCaptureStatusNone, "ffn stack decode: cannot be captured (it replays a graph of its own)");
   if (n_tokens > s->cap_T || k > s->cap_k) {
     s->cap_T = std::max(n_tokens, s->cap_T);
     s->cap_k = std::max(k, s->cap_k);

@@ -16,6 +16,7 @@ import numpy as np
 import torch
 
 from ._lib import check
+from .attention import _raw_stream, launch
 from .core import Context, default_context
 
 
@@ -119,7 +120,8 @@ class FfnStack:
     predictor top-k, the sparse SwiGLU MLP and the residual add, in one
     kl_ffn_stack_decode call (replayed as a CUDA graph for a repeated shape).
     ``predictors`` / ``mlps`` are lists of SparsityPredictor / SparseMlp on the
-    same context; ``norm_weights`` is [layers][hidden]."""
+    same context; ``norm_weights`` is [layers][hidden].  Where each layer has an
+    attention half (``attention``, ``quant``) in front, each has a stack of its own."""
 
     def __init__(self, predictors, mlps, norm_weights, eps: float = 1e-5, one_plus_weight: bool = False,
                  ctx: Context | None = None):
@@ -141,8 +143,22 @@ class FfnStack:
             self.lib.kl_ffn_stack_destroy(self.h)
 
     def decode(self, hidden: torch.Tensor, neuron_sparsity: float) -> torch.Tensor:
-        """Updates ``hidden`` [tokens][hidden] (a CUDA f32 tensor) in place and returns it."""
+        """Updates ``hidden`` [tokens][hidden] (a CUDA f32 tensor) in place and returns it.
+
+        Runs on torch's current stream, as the calls of ``attention`` and ``quant`` do, in order with the context's
+        own (behind what it holds, in front of what follows there).  It cannot be captured in a CUDA graph."""
         assert hidden.is_cuda and hidden.dtype == torch.float32 and hidden.is_contiguous()
-        check(self.lib.kl_ffn_stack_decode(self.h, hidden.data_ptr(), hidden.shape[0], float(neuron_sparsity)),
-              self.ctx.h, "kl_ffn_stack_decode")
+        args = ("kl_ffn_stack_decode", self.h, hidden.data_ptr(), hidden.shape[0], float(neuron_sparsity))
+        own = self.ctx.stream
+        if _raw_stream(self.ctx.device) == own.cuda_stream:
+            launch(self.ctx, *args)
+            return hidden
+        with torch.cuda.device(self.ctx.device):
+            now = torch.cuda.current_stream()
+            ordered = not torch.cuda.is_current_stream_capturing()
+            if ordered:
+                now.wait_stream(own)
+            launch(self.ctx, *args)
+            if ordered:
+                own.wait_stream(now)
         return hidden

@@ -136,6 +136,85 @@ def ffn(ctx, h=192, layers=1):
     return FfnStack(pred, mlp, np.ones((layers, h), np.float32), ctx=ctx)
 
 
+def test_both_halves_of_a_layer_on_another_stream(gpu_ctx):
+    """Norm, projection and the MLP stack on torch's current stream, in order, whichever stream the context has."""
+    stack = ffn(gpu_ctx)
+    w = randn(192, 192, seed=2, dtype=torch.float32) / 14
+    back = Q8Linear.from_weights(w, ctx=gpu_ctx)
+    norm = torch.ones(192, device=DEV)
+
+    def layer(hidden):
+        rows = add_rms_norm_q8(hidden, norm, ctx=gpu_ctx)
+        back.forward(rows.codes, rows.scales, out=hidden, accumulate=True)
+        stack.decode(hidden, 0.25)
+        rows = add_rms_norm_q8(hidden, norm, ctx=gpu_ctx)
+        back.forward(rows.codes, rows.scales, out=hidden, accumulate=True)
+
+    start = randn(3, 192, seed=1, dtype=torch.float32)
+    want = start.clone()
+    for _ in range(3):
+        layer(want)
+    torch.cuda.synchronize()
+    hidden = start.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)  # what is not ordered behind this runs too early
+        for _ in range(3):
+            layer(hidden)
+        got = hidden.clone()
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_the_mlp_half_is_not_captured(gpu_ctx):
+    """Refused with an error that leaves the capture as it is."""
+    stack = ffn(gpu_ctx, layers=2)
+    hidden, x = randn(3, 192, seed=1, dtype=torch.float32), torch.zeros(4, device=DEV)
+    for _ in range(3):
+        stack.decode(hidden, 0.25)
+    want = hidden.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        for _ in range(2):
+            with pytest.raises(KlError):
+                stack.decode(hidden, 0.25)
+        x.add_(1)
+    graph.replay()
+    assert torch.equal(hidden, want) and (x == 2).all()
+    stack.decode(hidden, 0.25)
+    gpu_ctx.sync()
+    assert not torch.equal(hidden, want)
+
+
+def test_a_context_with_a_stream_of_its_own():
+    """What the context's own stream holds and what torch's current stream holds both come before and after the stack."""
+    own = torch.cuda.Stream()
+    ctx = Context(0, stream=own)
+    stack, twin = ffn(ctx), ffn(Context(0))
+    start = randn(3, 192, seed=1, dtype=torch.float32)
+    want, hidden = start.clone(), torch.zeros_like(start)
+    for _ in range(3):
+        twin.decode(want, 0.25)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(own):
+        torch.cuda._sleep(50_000_000)
+        hidden.copy_(start)
+    for _ in range(3):
+        stack.decode(hidden, 0.25)  # behind what the context's stream holds
+    ctx.sync()
+    assert torch.equal(hidden, want)
+    with torch.cuda.stream(own):
+        torch.cuda._sleep(50_000_000)
+        hidden.copy_(start)
+    for _ in range(3):
+        stack.decode(hidden, 0.25)
+    got = hidden.clone()  # on the current stream
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
 # ---------------------------------------------------------------------------
 # rows of extreme sizes
 # ---------------------------------------------------------------------------
