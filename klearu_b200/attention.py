@@ -11,7 +11,7 @@ be captured in a CUDA graph; tensors have to be on the context's device.  As for
 all handles of the library, one host thread at a time calls a context and what
 was made with it.
 Nothing here has a backward pass: an input that requires a gradient is refused
-while gradients are recorded.
+while gradients are recorded, and so is one with a forward-mode tangent.
 """
 
 from __future__ import annotations
@@ -21,6 +21,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import HeadRowsC, SeqBatchC, check
 from .core import Context, default_context
@@ -56,6 +57,8 @@ def want(ctx: Context, t: torch.Tensor, what: str, dtype) -> None:
         raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires a gradient, and this call has no backward pass")
+    if forward_ad._current_level >= 0 and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what} has a tangent, which this call would drop; unpack it first")
 
 
 class RopeTable:

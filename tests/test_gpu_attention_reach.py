@@ -276,3 +276,19 @@ def test_attention_factor_has_64_bits(gpu_ctx):
     z = torch.arange(t, dtype=torch.float64)[:, None] * torch.as_tensor(rope.inv_freq)
     want = torch.cat([(z.cos() * factor).float(), (z.sin() * factor).float()], 1).bfloat16()
     assert torch.equal(got.cpu(), want)
+
+
+def test_tangents_are_refused(gpu_ctx):
+    cache = Kv4Cache(4, 16, 2, 64, ctx=gpu_ctx)
+    batch = SeqBatch(i32([0, 4]), i32([4]), i32([[0]]), max_q=4)
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device=DEV)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(ValueError):
+            cache.attend(dual, batch)
+        with pytest.raises(ValueError):
+            cache.append(dual, x, batch)
+        h = torch.ones(2, 64, device=DEV)
+        with pytest.raises(ValueError):
+            quantize_rows_q8(forward_ad.make_dual(h, h), ctx=gpu_ctx)
+        cache.attend(x, batch)  # a tensor without a tangent is welcome
