@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
       uint32_t qf[NR][2 * KW][2];
       float f[NR][2], qs[NR][2];  // of rows 2t, 2t + 1: what a product of codes is worth, and sum(q), in units of log2
       int pos[NR][2];
+      bool big = false;  // a row above 2^113: 2^12 of what its products are worth goes to the keys' steps and minima
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         const int row = r0 + 8 * r + g;
@@ -162,17 +163,19 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
 #pragma unroll
         for (int i = 0; i < D / 4; ++i) {
           top = fmaxf(top, fabsf(x[i]));
-          sum += x[i];
           fin = fin && finite_f(x[i]);
         }
         top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
         top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+        const int e = max(-114, min(126, 13 - ((int)(__float_as_uint(top) >> 23) - 127)));
+        const float up = __uint_as_float((uint32_t)(e + 127) << 23), up16 = up * 0.0625f;
+        big = big || e < -100;
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) sum = fmaf(x[i], up, sum);
         sum += __shfl_xor_sync(FULL, sum, 1);
         sum += __shfl_xor_sync(FULL, sum, 2);
         const unsigned bads = __ballot_sync(FULL, !fin);
         fin = ((bads >> (4 * g)) & 15u) == 0;
-        const int e = fin ? max(-100, min(126, 13 - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
-        const float up = __uint_as_float((uint32_t)(e + 127) << 23), up16 = up * 0.0625f;
 #pragma unroll
         for (int w = 0; w < KW; ++w)
 #pragma unroll
@@ -181,14 +184,23 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
             qf[r][2 * w + h][0] = fin ? pack_f16(y[0] * up, y[1] * up) : 0u;
             qf[r][2 * w + h][1] = fin ? pack_f16(y[2] * up16, y[3] * up16) : 0u;
           }
-        const float worth = __uint_as_float((uint32_t)(24 - e + 127) << 23) * (a.scale * log2e);
-        const float total = fin ? sum * (a.scale * log2e) : __int_as_float(0x7fffffff);
+        const float worth = __uint_as_float((uint32_t)(12 - e + 127) << 23) * (a.scale * log2e);
+        const float total = fin ? sum * (a.scale * log2e) * __uint_as_float((uint32_t)(127 - e) << 23) * 0x1p-12f
+                                : __int_as_float(0x7fffffff);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           f[r][i] = __shfl_sync(FULL, worth, 4 * (2 * t + i));
           qs[r][i] = __shfl_sync(FULL, total, 4 * (2 * t + i));
           pos[r][i] = first + (r0 + 8 * r + 2 * t + i) / group;
         }
+      }
+      big = __any_sync(FULL, big);
+      const float key_up = big ? 0x1p12f : 1.f;
+      if (!big) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) f[r][i] *= 0x1p12f, qs[r][i] *= 0x1p12f;
       }
       const int see_all_to = pos0;  // every row of the tile sees tokens up to here ..
       const int see_all_from = window_from(a.window, pos1);  // .. from here
@@ -267,8 +279,8 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
             }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float ks = __uint_as_float(pr[k].x << 16);
-            float km = __uint_as_float(pr[k].x & 0xffff0000u);
+            const float ks = __uint_as_float(pr[k].x << 16) * key_up;
+            float km = __uint_as_float(pr[k].x & 0xffff0000u) * key_up;
             vs[c][k] = __uint_as_float(pr[k].y << 16);
             vm[c][k] = __uint_as_float(pr[k].y & 0xffff0000u);
             // a value that is NaN makes the score NaN for whoever sees it, and is nothing to the others

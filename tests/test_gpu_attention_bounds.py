@@ -248,3 +248,13 @@ def test_padding_and_a_window_that_reaches_all(gpu_ctx, kernel, window, q_len, k
     q, k, v = inputs(q_len, kv_len, 4, 2, 64)
     out = run(gpu_ctx, kernel, q, k, v, q_len, kv_len, window=window, rms=False)
     assert torch.equal(out, run(gpu_ctx, kernel, q, k, v, q_len, kv_len, rms=False))
+
+
+@pytest.mark.parametrize("size", [2.0**114, 2.0**117, 2.0**125])
+def test_largest_queries(gpu_ctx, size):
+    """Queries up to the type's end and keys so small that the scores are ordinary."""
+    for kernel, rows in (("few", 3), ("many", 70), ("whole", 70)):
+        q, k, v = inputs([rows], [300], 4, 2, 64)
+        q = (q.clamp(-3, 3).double() * size).bfloat16()
+        k = (k.double() / size).bfloat16()
+        run(gpu_ctx, kernel, q, k, v, [rows], [300])
