@@ -21,7 +21,7 @@ constexpr int AT_W = 4;       // warps per block
 constexpr int AT_STAGES = 3;  // pairs of tiles of a warp's ring
 
 struct SplitPlan {
-  int chunk;      // tokens per block, a multiple of 16 AT_W
+  int least;      // fewest tokens per block, a multiple of 16 AT_W
   int chunks;     // blocks along a sequence
   int row_tiles;  // blocks along a sequence's rows
 };
@@ -101,20 +101,40 @@ __global__ void __launch_bounds__(AT_W * 32, NR == 1 ? 4 : 3) attend_split_kerne
   after_before();
   uint32_t used = 0;  // pairs of tiles that this warp has put through its ring
   const float log2e = 1.4426950408889634f;
+  // The longest sequence's tokens are shared out evenly, the others' cut alike.  Its length is looked up, since hints
+  // are the cache's whole capacity in a captured loop.  With exact hints and with such of 131072, us: one token of 777
+  // 7.9 and 9.9 (chunks by the hint alone 7.6 and 15.2), of 8000 11.0 and 13.5 (10.6 and 22.5), 64 sequences of 8000
+  // 126 and 126 (124 and 152), 8 of up to 30000 30 and 30 (30 and 137).
+  uint32_t share = p.chunks > 1 ? 0u : p.least;
+  const int some = p.chunks > 1 && lane < a.seq.num_seqs ? a.seq.kv_len[lane] : 0;
 
   for (int b = blockIdx.z; b < a.seq.num_seqs; b += gridDim.z) {
     bool bad = false;
     const SeqSpan s = seq_span(a.seq, b, ps, &bad);
     if (bad && threadIdx.x == 0) atomicOr(a.err, DERR_BOUNDS);
+    if (share == 0) {
+      int most = some;
+      for (int i = lane + 32; i < a.seq.num_seqs; i += 32) most = max(most, a.seq.kv_len[i]);
+      uint32_t longest = (uint32_t)max(0, __reduce_max_sync(FULL, most));
+      if (a.window > 0) longest = min(longest, (uint32_t)a.window + 8 * NR + 17);
+      share = max((uint32_t)p.least, ((longest + p.chunks - 1) / p.chunks + 16 * AT_W - 1) & ~(16 * AT_W - 1));
+    }
     const int rows = s.q_len * group, first = s.first;  // row r is token first + r / group
     for (int r0 = (blockIdx.x % p.row_tiles) * 8 * NR; r0 < rows; r0 += p.row_tiles * 8 * NR) {
       // tokens that some row of this tile sees: [lo, hi), this block's share [k0, k1)
       const int pos0 = first + r0 / group, pos1 = first + (min(r0 + 8 * NR, rows) - 1) / group, hi = min(pos1 + 1, s.kv_len);
       const int lo = window_from(a.window, pos0) & ~15;
       const int span = max(0, hi - lo);
-      const int chunk = max(p.chunk, (int)round_up(ceil_div(span, p.chunks), 16 * AT_W));
-      const int k0 = min(hi, lo + chunk_id * chunk), k1 = max(k0, min(hi, k0 + chunk));
+      // what does not fit is the last chunk's
+      const int64_t at0 = lo + (int64_t)chunk_id * share, at1 = chunk_id + 1 < p.chunks ? at0 + share : hi;
+      const int k0 = (int)min((int64_t)hi, at0), k1 = (int)max((int64_t)k0, min((int64_t)hi, at1));
       const int t0 = k0 >> 4, tiles = (k1 - k0 + 15) >> 4;  // k0 is a multiple of 16 wherever tiles > 0
+      if (tiles == 0 && p.chunks > 1) {  // a chunk behind the sequence's end, as hints make them
+        for (int r = r0 + threadIdx.x; r < min(r0 + 8 * NR, rows); r += AT_W * 32)
+          reinterpret_cast<float2*>(a.scratch)[((int64_t)chunk_id * a.seq.num_tokens + s.row + r / group) * a.q_heads + kvh * group +
+                                               r % group] = make_float2(-INFINITY, 0.f);
+        continue;
+      }
       // this warp's tiles are warp, warp + AT_W, ..; it takes them in pairs, for two chains of everything
       const int mine_n = tiles > warp ? (tiles - warp + AT_W - 1) / AT_W : 0, n = (mine_n + 1) / 2;
 
@@ -568,13 +588,12 @@ SplitPlan split_plan(const AttendShape& s) {
   // 58 us, 64 of them 108, 89, 85 and 96.
   const int64_t want = 148 * (nr == 1 ? 4 : 3) * std::min<int64_t>(4, std::max<int64_t>(1, items / 64));
   const int64_t chunks = std::max<int64_t>(1, want / items);
-  int64_t chunk = round_up(std::max<int64_t>(ceil_div(span, chunks), 16 * AT_W), 16 * AT_W);
+  const int64_t chunk = round_up(std::max<int64_t>(ceil_div(span, chunks), 16 * AT_W), 16 * AT_W);
   // Shorter chunks cost more in the join than they save: 64 sequences of up to 1000 take 23 us in one chunk each and
   // 31 in four, 32 of up to 2000 35 us in chunks of 256 and 26 in 512; where there are few, 256 keep the latency low
   // (one sequence of 2000: 10 us against 12 with 512).
-  chunk = std::max<int64_t>(chunk, std::min<int64_t>(round_up(span, 16 * AT_W), items >= 256 ? 1024 : items >= 128 ? 512 : 256));
-  p.chunk = (int)chunk;
-  p.chunks = (int)std::max<int64_t>(1, ceil_div(span, chunk));
+  p.least = items >= 256 ? 1024 : items >= 128 ? 512 : 256;
+  p.chunks = (int)std::max<int64_t>(1, ceil_div(span, std::max<int64_t>(chunk, p.least)));
   return p;
 }
 
