@@ -77,7 +77,7 @@ class RopeTable:
                  scaling: str | None = None, factor: float = 1.0, original_positions: int | None = None,
                  low_turns: float = 1.0, high_turns: float = 4.0, attention_factor: float = 1.0,
                  ctx: Context | None = None):
-        if rot_dim < 2 or rot_dim % 2:
+        if rot_dim < 2 or rot_dim % 2 or rot_dim >= 2**31:
             raise ValueError("rot_dim must be even and >= 2")
         if not (base > 0 and factor > 0 and math.isfinite(attention_factor)):
             raise ValueError("base and factor must be > 0, attention_factor finite")
@@ -163,6 +163,8 @@ class Kv4Cache:
     for a token's key and value in one head."""
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, ctx: Context | None = None):
+        if max(page_size, kv_heads, head_dim) >= 2**31 or min(page_size, kv_heads, head_dim) < 0:
+            raise ValueError("page_size, kv_heads and head_dim must be whole numbers of 31 bits")
         self.ctx = ctx or default_context()
         self.lib = self.ctx.lib
         self.num_pages, self.page_size, self.kv_heads, self.head_dim = num_pages, page_size, kv_heads, head_dim
@@ -244,8 +246,8 @@ class Kv4Cache:
         stand for, [num_tokens][kv_heads][head_dim] (bf16), num_tokens the rows of
         the call (cu_q's last entry, or more).  Rows of no sequence are left as
         they are."""
-        if num_tokens < 0:
-            raise ValueError("num_tokens must be >= 0")
+        if not 0 <= num_tokens < 2**31:
+            raise ValueError("num_tokens must be in [0, 2^31)")
         c = self._batch(batch, num_tokens)
         heads = self.kv_heads
         if k_out is None and v_out is None:
@@ -282,7 +284,7 @@ class Kv4Cache:
         c = self._batch(batch, t)
         if t == 0 or heads == 0:
             return out
-        window = min(window, 2**31 - 1)
+        window = max(-1, min(window, 2**31 - 1))  # a C int would take a number past 31 bits for another
         key = (batch.sizes, t, heads, window)
         need = self._workspace.get(key)
         if need is None:
