@@ -161,7 +161,7 @@ struct TcStep {
   float ek2;              // K is held times 1 / ek2; negative: a wide step
   float ev;               // V times 2^-ev; TC_NONE: nothing but zeros
 };
-// Of a token of a wide step: K is held times 2^-ek, V times 2^-ev.
+// Of a token: K is held times 2^-ek, V times 2^-ev, of the whole step alike where it is not wide.
 struct TcPowers {
   signed char ek, ev;  // ev -128: its value is zero
 };
@@ -175,7 +175,7 @@ struct TcShared {
   alignas(16) uint32_t reach[2][4][4];  // by step & 1: largest |K|, |V|, smallest of each but 0, of each decoding warp
   // by step & 3: a step's is written again when the step two on has its scores, after this one's softmax
   alignas(16) TcStep step[4];
-  alignas(16) TcPowers powers[4][TC_KV];  // of a wide step
+  alignas(16) TcPowers powers[4][TC_KV];
 };
 static_assert(offsetof(TcShared, reach) % 16 == 0 && offsetof(TcShared, step) % 16 == 0 && sizeof(TcStep) == 16,
               "read as 16- and 8-byte vectors");
@@ -248,23 +248,36 @@ struct TcRow {
 template <int D>
 __device__ __noinline__ TcRow tc_wide_step(TcRow row, const TcStep& st, const TcPowers* powers, float worth, int from, int to,
                                            uint32_t tS, uint32_t tO, bool rescale) {
-  auto score = [&](float s, int u, TcPowers x) {
-    const float f = fminf(fmaxf(worth * pow2(x.ek), 1.2e-38f), 3.4e38f);
-    return u <= to && u >= from && !st.hole[u >> 4] ? s * f : -INFINITY;
-  };
-  float top = -INFINITY, most = -INFINITY;  // the largest score, and with its value's exponent
-#pragma unroll 1
-  for (int c = 0; c < TC_KV; c += 16) {
+  // 16 keys' scores in units of log2, -inf for those that it does not see, and their values' powers
+  auto scores = [&](int c, float* t, float* ev) {
     uint32_t s[16];
     tc5_ld16_async(tS + c, s);
+    const uint4 x[2] = {*reinterpret_cast<const uint4*>(powers + c), *reinterpret_cast<const uint4*>(powers + c + 8)};
+    const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+    const bool hole = st.hole[c >> 4];
     tc5_ld_wait();
 #pragma unroll
     for (int u = 0; u < 16; ++u) {
-      const TcPowers x = powers[c + u];
-      const float t = score(__uint_as_float(s[u]), c + u, x);
-      top = fmaxf(top, t);
-      if (x.ev != -128) most = fmaxf(most, t + (float)x.ev);
+      const uint32_t y = w[u >> 1] >> (16 * (u & 1));
+      const float f = fminf(fmaxf(worth * pow2((signed char)(y & 0xff)), 1.2e-38f), 3.4e38f);
+      t[u] = c + u <= to && c + u >= from && !hole ? __uint_as_float(s[u]) * f : -INFINITY;
+      ev[u] = __int_as_float(0x4b400000 + (signed char)(y >> 8 & 0xff)) - 12582912.f;
     }
+  };
+  // the largest score, and the largest with its value's exponent, that one relative to the first: scores may be large
+  float top = -INFINITY, most = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < TC_KV; c += 16) {
+    float t[16], ev[16];
+    scores(c, t, ev);
+    float now = top;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) now = fmaxf(now, t[u]);
+    if (now > top) most -= now - top;
+    top = now;
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+      if (ev[u] != -128.f && t[u] != -INFINITY) most = fmaxf(most, t[u] - top + ev[u]);
   }
   float by = 1.f;  // of O
   const bool first = row.lift == -INFINITY;
@@ -275,7 +288,7 @@ __device__ __noinline__ TcRow tc_wide_step(TcRow row, const TcStep& st, const Tc
     row.l *= by;
   }
   if (most != -INFINITY) {  // the unit by what counts most
-    float need = ceilf(fminf(fmaxf(most - row.ref, -126.f), 126.f));
+    float need = ceilf(fminf(fmaxf(most + (top - row.ref), -126.f), 126.f));
     if (row.unit == TC_NONE || first) {
       row.unit = need;
     } else {
@@ -301,19 +314,19 @@ __device__ __noinline__ TcRow tc_wide_step(TcRow row, const TcStep& st, const Tc
   float sum = 0.f;
 #pragma unroll 1
   for (int c = 0; c < TC_KV; c += 32) {  // P's columns [c / 2, c / 2 + 16) have been read
-    uint32_t s[32], pk[16];
-    tc5_ld16_async(tS + c, s);
-    tc5_ld16_async(tS + c + 16, s + 16);
-    tc5_ld_wait();
+    uint32_t pk[16];
 #pragma unroll
-    for (int u = 0; u < 32; ++u) {
-      const TcPowers x = powers[c + u];
-      const float t = score(__uint_as_float(s[u]), c + u, x) - row.ref;
-      sum += exp2_fast(t);
-      s[u] = __float_as_uint(exp2_fast(t + (x.ev == -128 ? 0.f : 6.f + (float)x.ev - row.unit)));
+    for (int h = 0; h < 2; ++h) {
+      float t[16], ev[16];
+      scores(c + 16 * h, t, ev);
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        sum += exp2_fast(t[u] - row.ref);
+        t[u] = exp2_fast(t[u] - row.ref + (ev[u] == -128.f ? 0.f : 6.f + ev[u] - row.unit));
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) pk[8 * h + u] = pack_f16(t[2 * u], t[2 * u + 1]);
     }
-#pragma unroll
-    for (int u = 0; u < 16; ++u) pk[u] = pack_f16(__uint_as_float(s[2 * u]), __uint_as_float(s[2 * u + 1]));
     tc5_st16(tS + c / 2, pk);
   }
   row.l += sum;
@@ -363,7 +376,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
           top = max(top & 0xffffu, top >> 16);
 #pragma unroll
           for (int d = 1; d < LPR; d <<= 1) top = max(top, __shfl_xor_sync(FULL, top, d));
-          const int eq = max(-115, min(100, 13 - ((int)(top >> 7) - 127)));
+          const int eq = top < 0x7f80u ? max(-114, min(100, 13 - ((int)(top >> 7) - 127))) : 0;
           // the scale's sign goes into q, and a scale of zero makes it zero, so that a score's factor is positive
           const float up = a.scale == 0.f ? 0.f : a.scale < 0.f ? -pow2(eq) : pow2(eq);
 #pragma unroll
@@ -385,12 +398,14 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
     const int last = w.first + (min(w.r0 + i * 128 + 128, w.rows) - 1) / group - w.lo;
     const int jlo = a.window > 0 && last >= a.window ? (last - a.window + TC_KV) / TC_KV - 1 : -1;
     float ref = 0.f, lift = -INFINITY, l = 0.f, unit = TC_NONE, peak = -126.f;  // a TcRow
+    const float most_worth = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(worth)));
     for (int j = 0; j < w.steps; ++j) {
       if (!warp_wait(&sh.s_full[i], (kq + j) & 1u)) return false;
       tc5_fence_after();
       const TcStep& st = sh.step[(kq + j) & 3u];
       const uint2 holes = *reinterpret_cast<const uint2*>(st.hole);
-      if (st.ek2 < 0.f) {
+      // .. or scores that may pass 2^22, where the ordinary step's one rounding of a score and its reference would differ
+      if (st.ek2 < 0.f || most_worth * st.ek2 > 0x1p-13f) {
         const int to = seen - TC_KV * j, from = window_from(a.window, own - TC_KV * j);
         const TcRow row = tc_wide_step<D>({ref, lift, l, unit, peak}, st, sh.powers[(kq + j) & 3u], worth, from, to, tS, tO, j > 0);
         ref = row.ref, lift = row.lift, l = row.l, unit = row.unit, peak = row.peak;
@@ -678,7 +693,8 @@ __device__ __forceinline__ void tc_decode(const AttendArgs& a, int chunks, TcSha
       // also where values fall so far below those before that the rows' units could not follow
       const bool wide = (tk >> 23) > (bk >> 23) + TC_SPREAD || (tv >> 23) > (bv >> 23) + TC_SPREAD || (tv && ev < ev_top - 60);
       ev_top = max(ev_top, ev);
-      if (wide) sh.powers[q & 3u][tid] = TcPowers{(signed char)power(my_k), (signed char)(my_v ? power(my_v) : -128)};
+      sh.powers[q & 3u][tid] = wide ? TcPowers{(signed char)power(my_k), (signed char)(my_v ? power(my_v) : -128)}
+                                    : TcPowers{(signed char)ek, (signed char)(tv ? ev : -128)};
       if (tid == 0) {
         sh.step[q & 3u].ek2 = wide ? -1.f : pow2(ek);
         sh.step[q & 3u].ev = tv ? (float)ev : TC_NONE;

@@ -258,3 +258,27 @@ def test_largest_queries(gpu_ctx, size):
         q = (q.clamp(-3, 3).double() * size).bfloat16()
         k = (k.double() / size).bfloat16()
         run(gpu_ctx, kernel, q, k, v, [rows], [300])
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("size,spread", [(1e5, 1.0), (1e7, 1.0), (3e8, 1.0), (1e12, 1.0), (1e8, 1e8)])
+def test_large_scores(gpu_ctx, kernel, size, spread):
+    """Scores far beyond the range of the exponential: the key that wins by far gives the output, and nothing passes f16."""
+    rows, n = 90, 400
+    q, k, v = inputs([rows], [n], 4, 2, 64)
+    k = (k.float() * size * spread ** torch.linspace(-1, 0, n, device=DEV)[torch.randperm(n, device=DEV)][:, None, None]).bfloat16()
+    batch, pages = batch_for(kernel, [rows], [n], 16)
+    cache = Kv4Cache(pages, 16, 2, 64, ctx=gpu_ctx)
+    cache.append(k, v, SeqBatch(i32([0, n]), batch.kv_len, batch.page_table, max_q=n))
+    out = attend(kernel, cache, q, batch).double()
+    assert torch.isfinite(out).all()
+    hk, hv = R.held(k), R.held(v)
+    for h in range(4):
+        x = q[:, h].double() @ hk[:, h // 2].T / 8
+        at = torch.arange(n, device=DEV)[None] > torch.arange(n - rows, n, device=DEV)[:, None]
+        two = x.masked_fill(at, -float("inf")).topk(2, -1)
+        # a score is within 64 (2^-11 + 2^-20) |q| |K| / 8 of its own; where the second is further off it counts for nothing
+        clear = two.values[:, 0] - two.values[:, 1] > 30 + 2 * (B.F16 + 2.0**-20) / 8 * (q[:, h].double().abs() @ hk[:, h // 2].abs().T).amax(-1)
+        want = hv[two.indices[:, 0], h // 2]
+        tol = (B.BF16 + 2 * B.F16) * want.abs() + 3 * B.F16 * hv[two.indices[:, 0], h // 2].abs().amax(-1, keepdim=True)
+        assert clear.sum() > rows // 3 and ((out[:, h] - want).abs() <= tol)[clear].all()
