@@ -21,10 +21,10 @@
 // factor) and V.  V is held times 2^-ev, a row's O in units of 2^(unit - 6) of
 // its own, and P is 2^(6 + ev - unit) times the probability (to the reference),
 // 2^15 at most and with full precision down to 2^-14: the unit follows ev where
-// it grows by more than 1 or falls by more than 7 (O is rescaled with it), so
-// that neither zeros nor larger values in front leave later probabilities among
-// f16's subnormals.  (Following every growth: 502 us in place of 498.)  A step
-// whose keys or values are more than 2^16 apart in size is "wide": there every
+// it falls by more than 7, and rises where P would not fit (O is rescaled with
+// it), so that neither zeros nor larger values in front leave later probabilities
+// among f16's subnormals, and large values count by their probabilities.  A step
+// whose keys or values are more than 2^12 apart in size is "wide": there every
 // token has powers of two of its own, and each row takes its scores and its unit
 // from the tokens that it sees, so that those that it does not see cost it no
 // bits; tokens that no row of the block sees are zeros.
@@ -165,7 +165,9 @@ struct TcStep {
 struct TcPowers {
   signed char ek, ev;  // ev -128: its value is zero
 };
-constexpr int TC_SPREAD = 16;  // of a step that is not wide, as a power of two
+// Of a step that is not wide, as a power of two: P has steps of 2^-24 and is at least 2^-1 times the probability, so that a
+// value 2^12 larger than those that count errs by 2^-12 of them, as f16 does.
+constexpr int TC_SPREAD = 12;
 constexpr float TC_NONE = -10000.f;
 struct TcShared {
   uint64_t q_full, k_full[2], v_full[2], done;
@@ -415,9 +417,9 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
         continue;
       }
       float off = st.ev - unit;  // P is 2^(6 + off) times the probability
-      float grow = 1.f;          // of O by a change of its unit
-      if (!(off <= 1.f && off >= -7.f)) {
-        if (unit != TC_NONE && lift != -INFINITY) grow = st.ev == TC_NONE ? 1.f : pow2(max(-126, (int)-off));  // else O is zero
+      float grow = 1.f;          // of O by a fall of its unit
+      if (!(off >= -7.f && off < 1000.f) || lift == -INFINITY) {
+        if (unit != TC_NONE && st.ev != TC_NONE && lift != -INFINITY) grow = pow2((int)-off);  // else O is zero, or stays
         if (st.ev != TC_NONE) unit = st.ev, peak = fmaxf(peak, unit);
         off = 0.f;
       }
@@ -452,7 +454,7 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
           for (int c = 0; c < 4; ++c) tops[c] = fmaxf(tops[c], fmaxf(s[u + c], s[u + c + 4]));
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         if (top != -INFINITY) top *= f;
-        if (__any_sync(FULL, top > lift || grow != 1.f)) {
+        if (__any_sync(FULL, top > fminf(lift, lift + 1.f - off) || grow != 1.f)) {
           const bool first = lift == -INFINITY;
           const float now = top > lift - 8.f || first ? top : ref;
           float keep = 1.f;
@@ -462,6 +464,14 @@ __device__ __forceinline__ void tc_softmax(const AttendArgs& a, int chunks, TcSh
             lift = now + 8.f;
           }
           l *= keep;
+          // larger values than the unit's keep it as long as their keys' scores are as much lower
+          const float room = floorf(ref - top);
+          if (off > room + 1.f) {
+            keep *= pow2(max(-126, (int)(room - off)));
+            unit += off - room;
+            peak = fmaxf(peak, unit);
+            off = room;
+          }
 #pragma unroll
           for (int c = 0; c < 4; ++c) sum2[c] = mul2(sum2[c], pair(keep, keep));
           if (h == 1) {  // the step's first probabilities

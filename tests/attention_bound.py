@@ -6,6 +6,8 @@ output to bf16 (half a step 2^-8):
     the output by sum p_j d_j |V_j - o| <= sum p_j d_j |V_j| + |o| sum p_j d_j;
   * a value and its probability (many rows), 2^-11 of p |V| each; or a probability times its value's step (few rows),
     2^-11 of p s c = p (V - m), m the vector's smallest: together at most 2^-11 p (2 |V| + |m|);
+  * f16's smallest steps, 2^-24, where the largest of 128 keys or values in turn is 2^13 or more and a vector's largest at
+    most 2^12 below (many rows): half of one is 2^-26 of the vector's largest;
   * 32-bit sums of D products and of the keys, and the exponential's argument: 2^-20 and 1e-5.
 That is the worst case.  Roundings are independent, so over many outputs from values around zero their root mean
 square is far below it: 2^-7 / sqrt(12) = 0.00226 of the output for its bf16, a few 2^-10 / sqrt(12) = 0.0003 for the
@@ -41,9 +43,11 @@ def attend(q, k, v, first, window, scale):
         p = torch.where(seen.any(-1, keepdim=True), p / p.sum(-1, keepdim=True), 0.0)
         o, a = p @ vv, p @ vv.abs()
         low = (p @ vv.amin(-1).abs())[:, None]
-        moved = p * (abs(scale) * (F16 + 2.0**-20) * 1.05 * (q[:, h].abs() @ kk.abs().T))
+        fine = 2.0**-26 * (p @ vv.abs().amax(-1))[:, None]
+        moved = p * (abs(scale) * 1.05 * ((F16 + 2.0**-20) * (q[:, h].abs() @ kk.abs().T)
+                                          + 2.0**-26 * q[:, h].abs().sum(-1, keepdim=True) * kk.abs().amax(-1)))
         out[:, h] = o
-        tol[:, h] = (BF16 * o.abs() + F16 * (2 * a + low) + moved @ vv.abs() + o.abs() * moved.sum(-1, keepdim=True)
+        tol[:, h] = (BF16 * o.abs() + F16 * (2 * a + low) + fine + moved @ vv.abs() + o.abs() * moved.sum(-1, keepdim=True)
                      + 1.1e-5 * a + 1e-37)
     return out, tol
 

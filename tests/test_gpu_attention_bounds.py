@@ -2,6 +2,8 @@
 values whose size changes along a sequence, tokens that a row does not see.  ``few`` and ``many`` are the kernels for few
 and for many rows, chosen by the hints; ``many`` takes the keys in chunks of a step, ``whole`` all of a row's in one."""
 
+import math
+
 import pytest
 import torch
 
@@ -282,3 +284,19 @@ def test_large_scores(gpu_ctx, kernel, size, spread):
         want = hv[two.indices[:, 0], h // 2]
         tol = (B.BF16 + 2 * B.F16) * want.abs() + 3 * B.F16 * hv[two.indices[:, 0], h // 2].abs().amax(-1, keepdim=True)
         assert clear.sum() > rows // 3 and ((out[:, h] - want).abs() <= tol)[clear].all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("first,last", [(256, 384), (300, 428), (0, 128)])
+@pytest.mark.parametrize("big", [1e7, 1e10])
+def test_large_values_count_by_their_probabilities(gpu_ctx, kernel, first, last, big):
+    """A stretch of keys whose probabilities are about 1 / big of the others' and whose values are big times theirs: both
+    halves of the result count."""
+    n, rows = 900, 70
+    q, k, v = inputs([rows], [n], 4, 2, 64)
+    q *= 0.25
+    q[..., 0] = 32.0
+    k[:, :, 0] = 0.0
+    k[first:last, :, 0] = -math.log(big) / (32.0 * 64**-0.5)
+    v[first:last] = (v[first:last].float() * big).bfloat16()
+    run(gpu_ctx, kernel, q, k, v, [rows], [n])
