@@ -34,6 +34,8 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 
 def launch(ctx: Context, what: str, *args) -> None:
     """One C call on torch's current stream of the context's device."""
+    if not ctx.h:
+        raise RuntimeError("the context is closed")
     s = _raw_stream(ctx.device)
     lib, own = ctx.lib, ctx.stream.cuda_stream
     with ctx.launch_lock:

@@ -371,3 +371,17 @@ def test_numbers_past_31_bits(gpu_ctx):
     with pytest.raises(ValueError):
         cache.read(batch, 2**32)
     gpu_ctx.sync()
+
+
+def test_calls_after_their_context_is_closed():
+    ctx = Context(0)
+    cache = Kv4Cache(4, 16, 2, 64, ctx=ctx)
+    lin = Q8Linear.from_weights(torch.ones(4, 16), ctx=ctx)
+    batch = SeqBatch(i32([0, 4]), i32([4]), i32([[0]]), max_q=4)
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device=DEV)
+    codes, scales = torch.zeros(4, 16, dtype=torch.int8, device=DEV), torch.ones(4, device=DEV)
+    ctx.close()
+    for call in (lambda: cache.append(x, x, batch), lambda: cache.read(batch, 4), lambda: cache.attend(x, batch),
+                 lambda: lin.forward(codes, scales), lambda: quantize_rows_q8(x.flatten(1), ctx=ctx), lambda: RopeTable(64, 4, ctx=ctx)):
+        with pytest.raises(RuntimeError):
+            call()
