@@ -727,7 +727,7 @@ KL_API kl_status kl_kv4_destroy(kl_kv4_t cache);
  * A row whose token number is negative is padding in front.  Rows behind the
  * last sequence, and rows of no sequence, are left as they are in every output.
  * max_q and max_kv are the largest q_len and kv_len: they choose the launch
- * (a wrong one is slow, not wrong).  Page ids outside the cache, lengths beyond
+ * (a wrong one is slower, not wrong).  Page ids outside the cache, lengths beyond
  * the table and row ranges beyond num_tokens are reported as KL_EBOUNDS by the
  * next synchronising call; such tokens are neither written nor attended to. */
 typedef struct {

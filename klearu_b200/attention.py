@@ -115,8 +115,11 @@ class SeqBatch:
     ``page_table[b, j // page_size]``.
 
     ``max_q`` and ``max_kv`` are the largest numbers of new and of all tokens;
-    they choose the launch (too small or too large is slow, not wrong), so one
-    object, its tensors updated in place, serves a captured decode loop."""
+    they choose the launch (too small or too large is slower, not wrong; a
+    ``max_kv`` of the whole table costs a few us), so one object, its tensors
+    updated in place, serves a captured decode loop.  Tokens beyond the table or
+    the call's tensors are reported by ``Context.sync``, not written and not
+    attended to."""
 
     def __init__(self, cu_q: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, max_q: int,
                  max_kv: int | None = None):

@@ -752,7 +752,9 @@ void launch_q8_pack(const int8_t* src, int64_t ld, int n, int k, int8_t* dst, cu
 // 0.25 ns a row of its tile for a chunk of 128 bytes of K (one thread's loop), two
 // blocks share an SM up to 64 rows; the weights take 6.2 bytes a ns from memory
 // and 12 where other tiles of rows read them again; 2 us a further turn of blocks,
-// 3 us to join a split.  More tiles of 256 rows than SMs: the persistent kernel
+// 3 us to join a split.  Splits that the weights' stream bounds are priced alike,
+// and the fewest are taken (33 x 4096 of 11008: 4 of 4 to 8; others within 5%).
+// More tiles of 256 rows than SMs: the persistent kernel
 // (us, persistent and not; k 4096: 300 x 12288 30.6 33.8, 513 x 12288 32.9 39.2,
 // 1000 x 4096, 128 tiles, 20.6 20.7, 2000 x 4096 32.3 39.0).
 struct Q8Plan {
