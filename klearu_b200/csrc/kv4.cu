@@ -152,6 +152,8 @@ __device__ __forceinline__ void find_places(const Kv4View& cache, const SeqView&
   bool bad = false;
   const Place p = find_place(cache, seq, positions, b, t, table, max_pos, &bad);
   if (lane < n) places[lane] = p;
+  // sequences of which the call has no row at all
+  if (blockIdx.y == 0 && blockIdx.z == 0 && lane == 0 && seq.cu_q[ns] > seq.num_tokens) bad = true;
   if (bad && blockIdx.x == 0) atomicOr(err, DERR_BOUNDS);
 }
 

@@ -104,6 +104,22 @@ def test_rows_beyond_the_tensor(rows):
     assert ((out.double() - want).abs() <= tol).all()
 
 
+def test_sequences_without_a_row_in_the_tensor():
+    """A batch of which a whole sequence lies behind the call's tensors: reported by every call, the others served."""
+    ctx = Context(0)
+    cache = Kv4Cache(8, 16, 2, 64, ctx=ctx)
+    table = i32([[0, 1], [2, 3], [4, 5]])
+    k, v, q = randn(5, 2, 64, seed=1), randn(5, 2, 64, seed=2), randn(5, 4, 64, seed=3)
+    batch = SeqBatch(i32([0, 2, 5, 9]), i32([2, 3, 4]), table, max_q=4)
+    assert torch.equal(cache.append(k, v, batch, q=q), q)
+    assert reported(ctx)
+    gk, _ = cache.read(batch, 5)
+    assert reported(ctx) and torch.equal(gk, R.held(k).float().bfloat16())
+    cache.attend(q, batch)
+    assert reported(ctx)
+    ctx.sync()
+
+
 # ---------------------------------------------------------------------------
 # streams
 # ---------------------------------------------------------------------------
