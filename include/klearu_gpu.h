@@ -780,8 +780,8 @@ KL_API kl_status kl_kv4_attend(kl_kv4_t cache, const kl_seq_batch* seqs_host, in
  * scales[row] = max|u| / 127, codes = rint(127 u / max|u|).  x f32 or bf16
  * (x_dtype), residual and hidden f32 (nullable); hidden receives h and may be
  * residual (or x, in f32).  A row whose u is not finite, or with `norm` whose sum
- * of squares passes f32, gets scale NaN and codes 0; one whose products all
- * round to zero in f32 is zeros.  1 <= cols <= 49152 (KL_EUNSUPPORTED above). */
+ * of squares passes f32, gets scale NaN and codes 0.  1 <= cols <= 49152
+ * (KL_EUNSUPPORTED above). */
 KL_API kl_status kl_norm_q8(kl_ctx_t ctx, const void* x, int x_dtype, int64_t ldx, const float* residual, int64_t ldr,
                             const float* weight, int rows, int cols, float eps, int norm, int one_plus_weight,
                             float* hidden, int64_t ldh, int8_t* codes, int64_t ldc, float* scales);

@@ -166,13 +166,14 @@ __global__ void __launch_bounds__(1024) norm_q8_vec_kernel(NormQ8Args a) {
     }
   }
   __syncthreads();
-  const double top = __longlong_as_double((long long)top_s);
+  const unsigned long long top_bits = top_s;
+  const double top = __longlong_as_double((long long)top_bits);
   const bool good = finite32(mx) && (!a.norm || finite32(ss));
   auto put_scale = [&](bool small) {
     if (threadIdx.x == 0) a.scales[row] = good ? q8_scale(a, mx, top, ss, small) : __int_as_float(0x7fffffff);
   };
   if (!SMALL) put_scale(false);
-  const float inv = good && mx > 0.f ? 127.f / mx : 0.f;
+  const float inv = good && top_bits ? 127.f / mx : 0.f;  // infinite where the products are too small for f32
   int8_t* co = a.codes + row * a.ldc;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -256,7 +257,8 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
       atomicMax(&top_s, (unsigned long long)__double_as_longlong(fabs((double)nq_h[i] * (double)w)));
   }
   __syncthreads();
-  const double top = __longlong_as_double((long long)top_s);
+  const unsigned long long top_bits = top_s;
+  const double top = __longlong_as_double((long long)top_bits);
   const bool good = finite32(mx) && (!a.norm || finite32(ss)), small = q8_small(a, ss);
   if (small) {
     ss = 0.f;
@@ -264,7 +266,7 @@ __global__ void __launch_bounds__(NT) norm_q8_kernel(NormQ8Args a) {
     ss = block_reduce<NT>(ss, tmp, false);
   }
   if (threadIdx.x == 0) a.scales[row] = good ? q8_scale(a, mx, top, ss, small) : __int_as_float(0x7fffffff);
-  const float inv = good && mx > 0.f ? 127.f / mx : 0.f;
+  const float inv = good && top_bits ? 127.f / mx : 0.f;  // infinite where the products are too small for f32
   int8_t* co = a.codes + row * a.ldc;
   for (int i = threadIdx.x; i < a.cols; i += NT) {
     const float w = norm_weight(a, i);

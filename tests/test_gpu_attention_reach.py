@@ -267,6 +267,22 @@ def test_norm_of_small_rows_without_eps(gpu_ctx, cols, size):
 
 
 @pytest.mark.parametrize("cols", [256, 77])
+@pytest.mark.parametrize("x_size,w_size", [(1e-30, 1e-20), (1e-38, 1e-9), (1e-42, 1.0)])
+def test_products_below_32_bits(gpu_ctx, cols, x_size, w_size):
+    """Values times weights that are all zero in 32 bits: their codes and scale are those of the definition."""
+    x = (randn(4, cols, seed=1, dtype=torch.float32).double() * x_size).float()
+    x[1] = 0
+    w = (1 + 0.2 * randn(cols, seed=3, dtype=torch.float32)) * w_size
+    r = add_rms_norm_q8(x, w, eps=0.0, ctx=gpu_ctx)
+    u = x.double() * w.double()
+    top = u.abs().amax(-1, keepdim=True)
+    assert torch.equal(r.codes.double(), torch.where(top > 0, (u * 127 / top).round(), 0.0))
+    want = top[:, 0] / x.double().square().mean(-1).sqrt() / 127
+    live = [0, 2, 3]
+    assert ((r.scales.double() - want).abs() <= (cols / 2 + 6) * 2.0**-24 * want)[live].all()
+
+
+@pytest.mark.parametrize("cols", [256, 77])
 def test_codes_of_large_rows(gpu_ctx, cols):
     """Without a norm the sum of squares is nobody's business: rows whose squares pass 32 bits have codes."""
     x = randn(4, cols, seed=1, dtype=torch.float32) * 1e25
