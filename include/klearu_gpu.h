@@ -679,8 +679,10 @@ KL_API kl_status kl_ffn_stack_create(kl_ctx_t ctx, int n_layers, const kl_predic
 KL_API kl_status kl_ffn_stack_destroy(kl_ffn_stack_t s);
 /* hidden [n_tokens][hidden] (device f32), updated in place.  The second call
  * with the same (hidden pointer, n_tokens, k) captures the per-layer launches
- * in a CUDA graph, later calls replay it.  It cannot itself be captured
- * (KL_EUNSUPPORTED, the capture goes on). */
+ * in a CUDA graph, later calls replay it.  On a stream that the caller captures
+ * its kernels join that graph; as many tokens at that sparsity must have run
+ * before (else KL_EUNSUPPORTED, and the capture goes on).  Graphs that hold it
+ * must not run beside one another or beside the stack: its scratch is shared. */
 KL_API kl_status kl_ffn_stack_decode(kl_ffn_stack_t s, float* hidden, int n_tokens, float neuron_sparsity);
 
 /* ------------------------------------------------------------------------ */

@@ -63,15 +63,19 @@ void support(bool c, const std::string& m) {
 struct DBuf {
   void* p = nullptr;
   size_t bytes = 0;
+  bool in_graph = false;   // a captured graph may use what p was: a larger buffer does not free it
+  std::vector<void*> old;  // such
   DBuf() = default;
   DBuf(const DBuf&) = delete;
   DBuf& operator=(const DBuf&) = delete;
   ~DBuf() {
     if (p) cudaFree(p);
+    for (void* q : old) cudaFree(q);
   }
   void alloc(size_t n) {
     if (n <= bytes && p) return;
-    if (p) cudaFree(p);
+    if (p && in_graph) old.push_back(p);
+    else if (p) cudaFree(p);
     p = nullptr;
     bytes = 0;
     if (n == 0) n = 16;
@@ -3481,6 +3485,17 @@ extern "C" kl_status kl_sparse_mlp_destroy(kl_sparse_mlp_t m) {
   KL_API_END
 }
 
+// K splits of the down projection: at least 16 selected rows per split, and
+// up to enough blocks ((hidden / 2048) x splits x tokens) for 8 per SM
+static int sparse_mlp_splits(kl_sparse_mlp_t m, int n_tokens, int k) {
+  const int cols = (int)ceil_div(m->hid, 2048);
+  return std::max(1, std::min((int)ceil_div(k, 16), (int)ceil_div(1184, (int64_t)cols * n_tokens)));
+}
+// the gather path's scratch
+static size_t sparse_mlp_a_bytes(int n_tokens, int k) { return (size_t)n_tokens * k * 4; }
+static size_t sparse_mlp_part_bytes(kl_sparse_mlp_t m, int n_tokens, int k) {
+  return (size_t)n_tokens * sparse_mlp_splits(m, n_tokens, k) * m->ldw * 4;
+}
 // sparse_mlp::forward_sparse for T tokens on stream st (k >= 1).
 // accumulate (gather path only, n_tokens < KL_DENSE_MIN_TOKENS): out += the
 // MLP's output (a fused residual add) instead of out = it.
@@ -3500,12 +3515,9 @@ static void sparse_mlp_body(kl_sparse_mlp_t m, const float* x, int n_tokens, con
     }
     return;
   }
-  // K splits of the down projection: at least 16 selected rows per split, and
-  // up to enough blocks ((hidden / 2048) x splits x tokens) for 8 per SM
-  const int cols = (int)ceil_div(m->hid, 2048);
-  const int splits = std::max(1, std::min((int)ceil_div(k, 16), (int)ceil_div(1184, (int64_t)cols * n_tokens)));
-  m->a.alloc((size_t)n_tokens * k * 4);
-  m->part.alloc((size_t)n_tokens * splits * m->ldw * 4);
+  const int splits = sparse_mlp_splits(m, n_tokens, k);
+  m->a.alloc(sparse_mlp_a_bytes(n_tokens, k));
+  m->part.alloc(sparse_mlp_part_bytes(m, n_tokens, k));
   launch_sparse_mlp(m->gate.as<__nv_bfloat16>(), m->up.as<__nv_bfloat16>(), m->downT.as<__nv_bfloat16>(), m->hid,
                     m->ldw, m->inter, m->has_bias ? m->bias.as<float>() : nullptr, x, n_tokens, sel, k,
                     m->a.as<float>(), m->part.as<float>(), splits, out, accumulate, err, st);
@@ -3557,6 +3569,17 @@ struct kl_ffn_stack_s {
   ~kl_ffn_stack_s() {
     if (gexec) cudaGraphExecDestroy(gexec);
     if (cap_stream) cudaStreamDestroy(cap_stream);
+  }
+  // Whether body() would allocate nothing; and that what it uses outlives larger calls.
+  bool fits(int T, int k) const {
+    if (T > cap_T || k > cap_k) return false;
+    for (kl_sparse_mlp_t m : mlp)
+      if (T < KL_DENSE_MIN_TOKENS && (m->a.bytes < sparse_mlp_a_bytes(T, k) || m->part.bytes < sparse_mlp_part_bytes(m, T, k))) return false;
+    return true;
+  }
+  void keep_scratch() {
+    for (DBuf* b : {&norm, &out, &idx, &sc}) b->in_graph = true;
+    for (kl_sparse_mlp_t m : mlp) m->a.in_graph = m->part.in_graph = true;
   }
   void body(float* hidden, int T, int k, cudaStream_t st) {
     for (int l = 0; l < nl; ++l) {
@@ -3627,13 +3650,17 @@ extern "C" kl_status kl_ffn_stack_decode(kl_ffn_stack_t s, float* hidden, int n_
   support(k >= 1, "ffn stack decode: a sparsity that keeps no neuron is not supported");
   topk_check(s->pred[0], k);
   cudaStream_t st = ctx__->stream;
-  // a graph would keep scratch buffers that a larger call replaces
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) {
-    cudaGetLastError();  // the legacy stream while another one is captured
-    capture = cudaStreamCaptureStatusActive;
+    cudaGetLastError();
+    support(false, "ffn stack decode: the legacy stream cannot be used while another one is captured");
   }
-  support(capture == cudaStreamCaptureStatusNone, "ffn stack decode: cannot be captured (it replays a graph of its own)");
+  if (capture != cudaStreamCaptureStatusNone) {  // by the caller: no allocation, and scratch that stays for the graph
+    support(s->fits(n_tokens, k), "ffn stack decode: run as many tokens at this sparsity once before capturing them");
+    s->keep_scratch();
+    s->body(hidden, n_tokens, k, st);
+    return KL_OK;
+  }
   if (n_tokens > s->cap_T || k > s->cap_k) {
     s->cap_T = std::max(n_tokens, s->cap_T);
     s->cap_k = std::max(k, s->cap_k);

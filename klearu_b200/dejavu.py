@@ -146,7 +146,8 @@ class FfnStack:
         """Updates ``hidden`` [tokens][hidden] (a CUDA f32 tensor) in place and returns it.
 
         Runs on torch's current stream, as the calls of ``attention`` and ``quant`` do, in order with the context's
-        own (behind what it holds, in front of what follows there).  It cannot be captured in a CUDA graph."""
+        own (behind what it holds, in front of what follows there).  It can be captured in a CUDA graph once as many
+        tokens at that sparsity have run; such graphs share the stack's scratch, so one runs at a time."""
         assert hidden.is_cuda and hidden.dtype == torch.float32 and hidden.is_contiguous()
         args = ("kl_ffn_stack_decode", self.h, hidden.data_ptr(), hidden.shape[0], float(neuron_sparsity))
         own = self.ctx.stream

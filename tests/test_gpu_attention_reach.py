@@ -185,13 +185,34 @@ def test_both_halves_of_a_layer_on_another_stream(gpu_ctx):
     assert torch.equal(got, want)
 
 
-def test_the_mlp_half_is_not_captured(gpu_ctx):
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_the_mlp_half_in_a_captured_graph(gpu_ctx, tokens):
+    """Captured on another buffer than the one it ran on, replayed before and after larger calls replaced its scratch."""
+    stack = ffn(gpu_ctx, layers=2)
+    start = randn(tokens, 192, seed=1, dtype=torch.float32)
+    want = start.clone()
+    for _ in range(3):
+        stack.decode(want, 0.25)
+    hidden = start.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stack.decode(hidden, 0.25)
+    assert torch.equal(hidden, start)  # captured, not run
+    graph.replay()
+    graph.replay()
+    for big in (20, 300):
+        stack.decode(randn(big, 192, seed=2, dtype=torch.float32), 0.75)
+    junk = [torch.full((1 << 18,), float("nan"), device=DEV) for _ in range(8)]  # what was freed is somebody else's now
+    graph.replay()
+    assert torch.equal(hidden, want) and len(junk) == 8
+    gpu_ctx.sync()
+
+
+def test_a_capture_of_the_mlp_half_that_has_not_run(gpu_ctx):
     """Refused with an error that leaves the capture as it is."""
     stack = ffn(gpu_ctx, layers=2)
     hidden, x = randn(3, 192, seed=1, dtype=torch.float32), torch.zeros(4, device=DEV)
-    for _ in range(3):
-        stack.decode(hidden, 0.25)
-    want = hidden.clone()
+    before = hidden.clone()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         x.add_(1)
@@ -200,10 +221,10 @@ def test_the_mlp_half_is_not_captured(gpu_ctx):
                 stack.decode(hidden, 0.25)
         x.add_(1)
     graph.replay()
-    assert torch.equal(hidden, want) and (x == 2).all()
+    assert torch.equal(hidden, before) and (x == 2).all()
     stack.decode(hidden, 0.25)
     gpu_ctx.sync()
-    assert not torch.equal(hidden, want)
+    assert not torch.equal(hidden, before)
 
 
 def test_a_context_with_a_stream_of_its_own():
