@@ -3688,6 +3688,7 @@ extern "C" kl_status kl_ffn_stack_decode(kl_ffn_stack_t s, float* hidden, int n_
     cudaGraph_t g = nullptr;
     bool ok = cudaStreamBeginCapture(s->cap_stream, cudaStreamCaptureModeThreadLocal) == cudaSuccess;
     const unsigned long long n0 = g_launches.load();
+    for (kl_sparse_mlp_t m : s->mlp) m->a.in_graph = m->part.in_graph = true;  // larger calls of the MLP itself
     if (ok) {
       try {
         s->body(hidden, n_tokens, k, s->cap_stream);

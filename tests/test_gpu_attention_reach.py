@@ -208,6 +208,22 @@ def test_the_mlp_half_in_a_captured_graph(gpu_ctx, tokens):
     gpu_ctx.sync()
 
 
+def test_the_stack_beside_larger_calls_of_its_mlp(gpu_ctx):
+    """The stack's own graph goes on when a call of one of its MLPs needs more scratch than the graph's."""
+    stack, twin = ffn(gpu_ctx, layers=2), ffn(gpu_ctx, layers=2)
+    hidden = randn(3, 192, seed=1, dtype=torch.float32)
+    want = hidden.clone()
+    for step in range(5):
+        if step == 3:
+            mlp = stack._keep[1][0]
+            mlp.forward_sparse(randn(20, 192, seed=2, dtype=torch.float32), torch.arange(256, device=DEV).repeat(20, 1))
+            junk = [torch.full((1 << 18,), float("nan"), device=DEV) for _ in range(8)]
+        stack.decode(hidden, 0.25)
+        twin.decode(want, 0.25)
+        assert torch.equal(hidden, want), step
+    assert len(junk) == 8
+
+
 def test_a_capture_of_the_mlp_half_that_has_not_run(gpu_ctx):
     """Refused with an error that leaves the capture as it is."""
     stack = ffn(gpu_ctx, layers=2)
