@@ -16,6 +16,7 @@ from klearu_b200.core import Context
 from klearu_b200.dejavu import FfnStack, SparseMlp, SparsityPredictor
 from klearu_b200.quant import Q8Linear, add_rms_norm_q8, quantize_rows_q8
 from test_gpu_attention import DEV, i32, randn
+from test_gpu_decoder_layer import Layer
 from test_gpu_q8 import check_norm
 
 pytestmark = pytest.mark.gpu
@@ -222,6 +223,60 @@ def test_the_stack_beside_larger_calls_of_its_mlp(gpu_ctx):
         twin.decode(want, 0.25)
         assert torch.equal(hidden, want), step
     assert len(junk) == 8
+
+
+def test_a_whole_layer_in_a_captured_graph(gpu_ctx):
+    """Both halves of two layers in one graph, replayed token after token, against calls one by one; hints of the cache's
+    whole capacity; a prompt through the same layers between the tokens."""
+    def model():
+        return [(Layer(gpu_ctx, 2, 640), ffn(gpu_ctx)) for _ in range(2)]
+
+    def step(layers, hidden, batch_of):
+        for half, stack in layers:
+            half(hidden, batch_of(half))
+            stack.decode(hidden, 0.25)
+
+    def prompt(layers, q_len, length, seed):
+        hidden = 2 * randn(sum(q_len), Layer.hidden, seed=seed, dtype=torch.float32)
+        cu = i32([0, q_len[0], sum(q_len)])
+        step(layers, hidden, lambda half: SeqBatch(cu, i32(length), half.table, max_q=max(q_len)))
+
+    mine, twin = model(), model()
+    for x in (mine, twin):
+        prompt(x, [30, 200], [30, 200], 5)
+        first = 2 * randn(2, Layer.hidden, seed=6, dtype=torch.float32)
+        step(x, first, lambda half: SeqBatch(i32([0, 1, 2]), i32([31, 201]), half.table, max_q=1))
+    kv, cu = i32([32, 202]), i32([0, 1, 2])
+    hidden = torch.zeros(2, Layer.hidden, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    batches = {half: SeqBatch(cu, kv, half.table, max_q=1) for half, _ in mine}
+    with torch.cuda.graph(graph):
+        step(mine, hidden, batches.__getitem__)
+    for n in range(4):
+        start = 2 * randn(2, Layer.hidden, seed=10 + n, dtype=torch.float32)
+        hidden.copy_(start)
+        graph.replay()
+        plain = start.clone()
+        step(twin, plain, lambda half: SeqBatch(cu, kv.clone(), half.table, max_q=1))
+        assert torch.equal(hidden, plain), n
+        kv += 1
+        if n == 1:  # 40 and 90 more prompt tokens, whose scratch is larger than the graph's
+            for x in (mine, twin):
+                prompt(x, [40, 90], [73, 293], 20)
+            kv += torch.tensor([40, 90], dtype=torch.int32, device=DEV)
+    gpu_ctx.sync()
+
+
+def test_reading_into_one_given_output(gpu_ctx):
+    cache = Kv4Cache(2, 16, 2, 64, ctx=gpu_ctx)
+    batch = SeqBatch(i32([0, 9]), i32([9]), i32([[1]]), max_q=9)
+    k, v = randn(9, 2, 64, seed=1), randn(9, 2, 64, seed=2)
+    cache.append(k, v, batch)
+    wide = torch.full((9, 2, 72), 7.0, dtype=torch.bfloat16, device=DEV)
+    for name, other in (("k_out", 1), ("v_out", 0)):
+        got = cache.read(batch, 9, **{name: wide[..., :64]})
+        assert got[1 - other].data_ptr() == wide.data_ptr() and (wide[..., 64:] == 7).all()
+        assert torch.equal(got[0], R.held(k).float().bfloat16()) and torch.equal(got[1], R.held(v).float().bfloat16())
 
 
 def test_a_capture_of_the_mlp_half_that_has_not_run(gpu_ctx):
